@@ -437,6 +437,106 @@ typedef struct mb_greedy_args {
 
 int mb_greedy_advance(const mb_greedy_args* args, void* stream);
 
+/* ---- paged key-value cache -----------------------------------------------------------------
+ * No counterpart in the reference (its cache is one contiguous tensor per row with one length,
+ * fx_handler/hf_attention.py:194-196; paging is on its roadmap, docs/roadmap.md:178).  Keys and
+ * values live in pools [pages, page_size, kv_heads, head_dim]; row r of the block table lists the
+ * pages of request r in order (-1, or any other id outside 0..pages-1, is no page); `lengths` says
+ * how many tokens it holds; the unused pages are the first `free_count` entries of the stack
+ * `free_pages`.  Four entry points, all non-blocking, capturable, without allocation:
+ *
+ *   mb_paged_reserve    pages, slots and positions for the new tokens of every request
+ *   mb_paged_append     keys and values of tokens into their slots
+ *   mb_paged_attention  one new token a request
+ *   mb_paged_prefill    several new tokens a request, causal
+ *
+ * Strides are in elements, the last dimension is contiguous; tensors of 16-bit values start on 16-byte
+ * boundaries and their strides are multiples of 8 (MB_ERR_INVALID otherwise).  page_size: a power of two from 8 to
+ * 1024; head_dim in {64, 128, 256}; block_table is contiguous.                                       */
+enum mb_element { MB_BF16 = 0, MB_FP16 = 1 };
+
+/* counts[r] > 0: request r wants room for that many more tokens.  Requests are granted in order of their rows, all or
+ * nothing: r is granted if its tokens fit its row of the table, if the tokens wanted by rows 0..r (those that fit
+ * their rows) are at most max_tokens, and if the pages newly wanted by rows 0..r are at most those free, or r wants
+ * none.  counts[r] < 0: its last -counts[r] tokens are dropped (all of them at most) and pages without tokens
+ * go back on the stack before anything is granted, last row's last page first: dropping what a call
+ * granted restores the stack.  A page popped is stack[free - 1], then stack[free - 2], ...; entries
+ * above the new free count keep what they held.  Token j of the granted ones, places offsets[r] ..
+ * offsets[r + 1] - 1 for row r: its slot page * page_size + offset, position, and row; places behind the
+ * last: -1, 0, -1.  granted[r]: tokens granted, or dropped (negative).                            */
+typedef struct mb_paged_reserve_args {
+    int32_t requests;         /* rows, at most 8192                                       */
+    int32_t width;            /* pages per row of the table; width * page_size < 2^31     */
+    int32_t pages;            /* of the pool: entries of free_pages                       */
+    int32_t page_size;
+    int32_t max_tokens;       /* entries of slots, positions and rows; may be 0           */
+    int32_t reserved;
+    uint64_t counts;          /* int32 [requests]                                         */
+    uint64_t lengths;         /* int32 [requests], updated                                */
+    uint64_t block_table;     /* int32 [requests, width], updated                         */
+    uint64_t free_pages;      /* int32 [pages], updated                                   */
+    uint64_t free_count;      /* int32 [1], updated                                       */
+    uint64_t offsets;         /* int32 [requests + 1], written                            */
+    uint64_t slots;           /* int64 [max_tokens], written                              */
+    uint64_t positions;       /* int64 [max_tokens], written                              */
+    uint64_t rows;            /* int32 [max_tokens], written                              */
+    uint64_t granted;         /* int32 [requests], written                                */
+} mb_paged_reserve_args;
+
+int mb_paged_reserve(const mb_paged_reserve_args* args, void* stream);
+
+/* Token t goes to page slots[t] / page_size, place slots[t] % page_size; slots outside
+ * 0..pages * page_size - 1 are skipped.  Of two tokens with one slot either may end up there.   */
+typedef struct mb_paged_append_args {
+    int32_t tokens, kv_heads, head_dim, pages, page_size, reserved;
+    int64_t key_token, key_head, value_token, value_head;             /* strides          */
+    int64_t kpool_page, kpool_token, kpool_head, vpool_page, vpool_token, vpool_head;
+    uint64_t key, value;      /* [tokens, kv_heads, head_dim]                             */
+    uint64_t key_pages, value_pages;
+    uint64_t slots;           /* int64 [tokens]                                           */
+} mb_paged_append_args;
+
+int mb_paged_append(const mb_paged_append_args* args, void* stream);
+
+/* Query t belongs to request rows[t] (t where rows is 0; a row outside 0..requests-1: none) and attends all of its
+ * `lengths` keys that lie on pages of the pool; where there is none its output is zero.  With `key` and `value`
+ * the last of them is the token's own and is written to its place in the pools first; rows then name a request
+ * once.  Scores, softmax statistics and sums are fp32; outputs are rounded once.
+ *
+ * mb_paged_prefill: request r has the queries offsets[r] .. offsets[r + 1] - 1, its last positions, already
+ * appended: the one at position p attends the keys 0..p.  A query before position 0 has none.  Queries of
+ * no request: zero where zero_rest is set, else left as they were.  offsets do not fall and lie in 0..tokens.
+ *
+ * workspace: as many bytes as the _workspace call says (0: none), 256-byte aligned, not shared by calls that
+ * may overlap; negative: MB_ERR_*.  status: optional int32 [1], receives an enum mb_status_code if a wait of the
+ * kernel ran out (it is not written otherwise); the outputs are then not valid.                  */
+typedef struct mb_paged_attention_args {
+    int32_t element;          /* enum mb_element of query, key, value, pools and out      */
+    int32_t tokens;           /* rows of query                                            */
+    int32_t requests;         /* rows of the block table                                  */
+    int32_t heads, kv_heads, head_dim;
+    int32_t width, pages, page_size;
+    int32_t zero_rest;        /* mb_paged_prefill                                         */
+    float scale;
+    int32_t reserved;
+    int64_t query_token, query_head, key_token, key_head, value_token, value_head;
+    int64_t kpool_page, kpool_token, kpool_head, vpool_page, vpool_token, vpool_head;
+    uint64_t query;           /* [tokens, heads, head_dim]                                */
+    uint64_t key, value;      /* [tokens, kv_heads, head_dim] or 0; 0 for mb_paged_prefill */
+    uint64_t key_pages, value_pages;
+    uint64_t block_table;     /* int32 [requests, width]                                  */
+    uint64_t lengths;         /* int32 [requests]                                         */
+    uint64_t index;           /* rows: int32 [tokens] or 0; mb_paged_prefill: offsets int32 [requests + 1] */
+    uint64_t out;             /* [tokens, heads, head_dim], contiguous                    */
+    uint64_t workspace;
+    uint64_t status;
+} mb_paged_attention_args;
+
+int64_t mb_paged_attention_workspace(const mb_paged_attention_args* args);
+int mb_paged_attention(const mb_paged_attention_args* args, void* stream);
+int64_t mb_paged_prefill_workspace(const mb_paged_attention_args* args);
+int mb_paged_prefill(const mb_paged_attention_args* args, void* stream);
+
 const char* mb_strerror(int code);
 const char* mb_status_string(int status_code);
 const char* mb_last_cuda_error(void);

@@ -12,6 +12,8 @@ parts of it this backend keeps):
 ``PrefillLogits``                   ids -> logits prefill wrapper over ``megabake::attention``
 ``StatefulPrefill``                 prefill that also fills the explicit decode state
 ``GreedyGenerator``                 compiled prefill + decode loop over one KV state
+``PagedState``                      the tensors of a paged key-value cache, and its operators:
+``paged_reserve``, ``paged_append``, ``paged_kv_attention``, ``paged_prefill_attention``
 ``bucketed`` / ``PaddingDependence`` prompts of any length through a few fixed-shape compiles
 ``register_transformers_attention`` the ``"megabake"`` attention implementation for HF models
 ``CompilerError``                   every refusal, with a staged diagnostic
@@ -22,9 +24,10 @@ from .ops import attention, kv_attention
 
 __all__ = [
     "CompilerDiagnostic", "CompilerError", "DecodeStep", "GreedyGenerator", "GroupedStateDecoder",
-    "PaddingDependence",
+    "PaddingDependence", "PagedBatch", "PagedState",
     "PrefillLogits", "StatefulDecoder", "StatefulPrefill", "attention", "bucketed",
-    "graphed", "kv_attention", "make_backend", "register_transformers_attention",
+    "graphed", "kv_attention", "make_backend", "paged_append", "paged_kv_attention",
+    "paged_prefill_attention", "paged_reserve", "register_transformers_attention",
 ]
 
 
@@ -43,6 +46,10 @@ def __getattr__(name):
     if name in ("bucketed", "PaddingDependence"):
         from . import buckets
         return getattr(buckets, name)
+    if name in ("PagedBatch", "PagedState", "paged_append", "paged_kv_attention", "paged_prefill_attention",
+                "paged_reserve"):
+        from . import paged
+        return getattr(paged, name)
     if name == "GreedyGenerator":
         from .generate import GreedyGenerator
         return GreedyGenerator

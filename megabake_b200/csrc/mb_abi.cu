@@ -56,6 +56,14 @@ struct Relay {
 
 }  // namespace
 
+int mb::cuda_error(cudaError_t err, const char* what) noexcept {
+    try {
+        return cuda_fail(err, what);
+    } catch (...) {  // no memory for the text
+        return MB_ERR_CUDA;
+    }
+}
+
 struct mb_plan {
     int device = 0;
     int mode = MB_MODE_DECODE;

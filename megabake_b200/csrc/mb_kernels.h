@@ -11,6 +11,9 @@ struct KernelParams;
 struct Control;
 union StreamDesc;
 
+// MB_ERR_CUDA, with the text that mb_last_cuda_error() returns.
+int cuda_error(cudaError_t err, const char* what) noexcept;
+
 int decode_threads();
 int decode_fixed_smem();
 int decode_stage_bytes();

@@ -1,0 +1,508 @@
+// Operators around a paged key-value cache: pages and slots for new tokens (mb_paged_reserve), keys and
+// values into their slots (mb_paged_append), attention of one new token a request (mb_paged_attention) and of
+// several (mb_paged_prefill).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <initializer_list>
+
+#include "mb_device.cuh"
+#include "mb_kernels.h"
+#include "mb_paged.cuh"
+
+namespace mb {
+namespace paged {
+
+// ---------------------------------------------------------------------------------------
+// Pages and slots from request lengths
+//
+// Three exclusive sums over the requests decide everything: pages given back by the rows behind r (where r's pages
+// go on the stack), tokens and pages wanted by the rows up to r (whether r is granted), tokens and pages granted
+// before r (its places, and which entries of the stack are its pages).  A thread sums a run of neighbouring rows, the
+// block scans the threads.  What a row looks up afterwards lies in shared memory.
+// ---------------------------------------------------------------------------------------
+constexpr int kReserveThreads = 1024;
+
+struct ReserveArgs {
+    int requests, width, pages, page_shift, max_tokens;
+    const int* counts;
+    int *lengths, *table, *stack, *free_count, *offsets, *rows, *granted;
+    long long *slots, *positions;
+};
+
+struct Pair {
+    long long a, b;
+};
+
+// Exclusive sums over the threads of the block, and the totals.  Every thread calls it.
+__device__ __forceinline__ Pair exclusive_sums(Pair v, Pair* warp_sums, Pair& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Pair inclusive = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long a = __shfl_up_sync(0xffffffffu, inclusive.a, d);
+        const long long b = __shfl_up_sync(0xffffffffu, inclusive.b, d);
+        if (lane >= d) {
+            inclusive.a += a;
+            inclusive.b += b;
+        }
+    }
+    __syncthreads();  // the sums of a call before have been read
+    if (lane == 31) warp_sums[warp] = inclusive;
+    __syncthreads();
+    Pair before = {0, 0};
+    total = {0, 0};
+    for (int w = 0; w < kReserveThreads / 32; ++w) {
+        if (w == warp) before = total;
+        total.a += warp_sums[w].a;
+        total.b += warp_sums[w].b;
+    }
+    return {before.a + inclusive.a - v.a, before.b + inclusive.b - v.b};
+}
+
+__global__ void __launch_bounds__(kReserveThreads) reserve_kernel(const ReserveArgs p) {
+    extern __shared__ int rows_smem[];
+    const int R = p.requests, page = 1 << p.page_shift;
+    int* kept_tokens = rows_smem;       // [R] tokens that stay before any are granted
+    int* first_page = rows_smem + R;    // [R] pages given back by later rows, then pages granted to earlier ones
+    int* offset = rows_smem + 2 * R;    // [R + 1]
+    __shared__ Pair warp_sums[kReserveThreads / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per_thread = (R + kReserveThreads - 1) / kReserveThreads;
+    const int r0 = min(tid * per_thread, R), r1 = min(r0 + per_thread, R);
+    const int capacity = p.width << p.page_shift;
+    auto pages_of = [&](long long tokens) { return static_cast<int>((tokens + page - 1) >> p.page_shift); };
+    auto held_tokens = [&](int r) { return min(max(p.lengths[r], 0), capacity); };
+
+    // what is given back
+    Pair sum = {0, 0}, total;
+    for (int r = r0; r < r1; ++r) {
+        const int count = p.counts[r], held = held_tokens(r);
+        const int kept = count < 0 ? static_cast<int>(max(static_cast<long long>(held) + count, 0ll)) : held;
+        kept_tokens[r] = kept;
+        sum.a += pages_of(held) - pages_of(kept);
+    }
+    Pair before = exclusive_sums(sum, warp_sums, total);
+    long long behind = total.a - before.a;
+    for (int r = r0; r < r1; ++r) {
+        behind -= pages_of(held_tokens(r)) - pages_of(kept_tokens[r]);
+        first_page[r] = static_cast<int>(behind);
+    }
+    const int free_before = *p.free_count;
+    const long long available = free_before + total.a;
+    __syncthreads();
+    for (int r = warp; r < R; r += kReserveThreads / 32) {
+        const int held = pages_of(held_tokens(r)), kept = pages_of(kept_tokens[r]);
+        int* row = p.table + static_cast<size_t>(r) * p.width;
+        for (int j = kept + lane; j < held; j += 32) {
+            const long long at = static_cast<long long>(free_before) + first_page[r] + held - 1 - j;
+            if (at >= 0 && at < p.pages) p.stack[at] = row[j];
+            row[j] = -1;
+        }
+    }
+
+    // who is granted what he wants
+    sum = {0, 0};
+    for (int r = r0; r < r1; ++r) {
+        const int count = p.counts[r];
+        const long long after = static_cast<long long>(kept_tokens[r]) + count;
+        if (count > 0 && after <= capacity) {
+            sum.a += count;
+            sum.b += pages_of(after) - pages_of(kept_tokens[r]);
+        }
+    }
+    before = exclusive_sums(sum, warp_sums, total);
+    sum = {0, 0};
+    for (int r = r0; r < r1; ++r) {
+        const int count = p.counts[r];
+        const long long after = static_cast<long long>(kept_tokens[r]) + count;
+        offset[r] = 0;
+        if (count > 0 && after <= capacity) {
+            const int need = pages_of(after) - pages_of(kept_tokens[r]);
+            before.a += count;
+            before.b += need;
+            if (before.a <= p.max_tokens && (need == 0 || before.b <= available)) {
+                offset[r] = count;
+                sum.a += count;
+                sum.b += need;
+            }
+        }
+    }
+    before = exclusive_sums(sum, warp_sums, total);
+    for (int r = r0; r < r1; ++r) {
+        const int count = offset[r];
+        offset[r] = static_cast<int>(before.a);
+        first_page[r] = static_cast<int>(before.b);
+        before.a += count;
+        before.b += pages_of(static_cast<long long>(kept_tokens[r]) + count) - pages_of(kept_tokens[r]);
+    }
+    if (tid == 0) offset[R] = static_cast<int>(total.a);
+    __syncthreads();  // the pages given back are on the stack, too
+    for (int r = warp; r < R; r += kReserveThreads / 32) {
+        const int kept = pages_of(kept_tokens[r]);
+        const int last = pages_of(static_cast<long long>(kept_tokens[r]) + offset[r + 1] - offset[r]);
+        int* row = p.table + static_cast<size_t>(r) * p.width;
+        for (int j = kept + lane; j < last; j += 32) {
+            const long long at = available - 1 - (first_page[r] + j - kept);
+            row[j] = at >= 0 && at < p.pages ? p.stack[at] : -1;
+        }
+    }
+    __syncthreads();
+    for (int r = tid; r < R; r += kReserveThreads) {
+        const int got = offset[r + 1] - offset[r];
+        const int count = p.counts[r];
+        p.granted[r] = count < 0 ? kept_tokens[r] - held_tokens(r) : got;
+        p.lengths[r] = kept_tokens[r] + got;
+        p.offsets[r] = offset[r];
+    }
+    if (tid == 0) {
+        p.offsets[R] = offset[R];
+        *p.free_count = static_cast<int>(available - total.b);
+    }
+    for (int t = tid; t < p.max_tokens; t += kReserveThreads) {
+        long long slot = -1, position = 0;
+        int r = -1;
+        if (t < offset[R]) {
+            int low = 0, high = R;  // offset[low] <= t < offset[high]
+            while (high - low > 1) {
+                const int middle = (low + high) >> 1;
+                if (offset[middle] <= t)
+                    low = middle;
+                else
+                    high = middle;
+            }
+            r = low;
+            const int at = kept_tokens[r] + t - offset[r];
+            position = at;
+            const int entry = p.table[static_cast<size_t>(r) * p.width + (at >> p.page_shift)];
+            if (entry >= 0 && entry < p.pages)
+                slot = (static_cast<long long>(entry) << p.page_shift) + (at & (page - 1));
+        }
+        p.slots[t] = slot;
+        p.positions[t] = position;
+        p.rows[t] = r;
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// Keys and values into their slots: 16 bytes a thread
+// ---------------------------------------------------------------------------------------
+struct AppendArgs {
+    int tokens, kv_heads, vectors;   // vectors: of 16 bytes in a head's row
+    int page_shift;
+    long long slots_end;
+    Strides2 key, value;
+    Strides3 kpool, vpool;
+    const unsigned short *k, *v;
+    unsigned short *key_pages, *value_pages;
+    const long long* slots;
+};
+
+__global__ void __launch_bounds__(256) append_kernel(const AppendArgs p) {
+    const long long per_token = static_cast<long long>(p.kv_heads) * p.vectors;
+    const long long all = per_token * p.tokens;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
+        const int t = static_cast<int>(i / per_token), rest = static_cast<int>(i % per_token);
+        const int h = rest / p.vectors, c = rest % p.vectors * 8;
+        const long long slot = p.slots[t];
+        if (slot < 0 || slot >= p.slots_end) continue;
+        const long long at = slot >> p.page_shift, in_page = slot & ((1 << p.page_shift) - 1);
+        const uint4 k = *reinterpret_cast<const uint4*>(p.k + t * p.key.token + h * p.key.head + c);
+        const uint4 v = *reinterpret_cast<const uint4*>(p.v + t * p.value.token + h * p.value.head + c);
+        *reinterpret_cast<uint4*>(p.key_pages + at * p.kpool.page + in_page * p.kpool.token + h * p.kpool.head + c) = k;
+        *reinterpret_cast<uint4*>(p.value_pages + at * p.vpool.page + in_page * p.vpool.token + h * p.vpool.head + c) =
+            v;
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// Attention, a warp per query and head: keys one after the other, a running maximum and sum
+// ---------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ float widen(T v);
+template <>
+__device__ __forceinline__ float widen(__nv_bfloat16 v) {
+    return __bfloat162float(v);
+}
+template <>
+__device__ __forceinline__ float widen(__half v) {
+    return __half2float(v);
+}
+template <typename T>
+__device__ __forceinline__ T narrow(float v);
+template <>
+__device__ __forceinline__ __nv_bfloat16 narrow(float v) {
+    return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half narrow(float v) {
+    return __float2half_rn(v);
+}
+
+// Weights are 2^(log2(e) (score - highest) + shift).  fp16: up by 2^15, so that small ones keep their digits when they
+// are rounded to 16 bits; bf16: down by 2^31, so that no sum over a context, which has fewer than 2^31 keys,
+// overflows whatever the values are (fp16 values cannot).
+constexpr float kLog2e = 1.4426950408889634f;
+template <typename T>
+constexpr float kWeightShift = 15.f;
+template <>
+constexpr float kWeightShift<__nv_bfloat16> = -31.f;
+
+// The last key and value of every query's request, where they belong.
+template <typename T>
+__global__ void __launch_bounds__(128) append_last_kernel(const AttentionArgs p) {
+    const int t = blockIdx.x, r = p.index != nullptr ? p.index[t] : t;
+    if (r < 0 || r >= p.requests) return;
+    const int length = min(p.lengths[r], p.width << p.page_shift);
+    if (length < 1) return;
+    const int last = length - 1, entry = p.table[static_cast<size_t>(r) * p.width + (last >> p.page_shift)];
+    if (entry < 0 || entry >= p.pages) return;
+    const long long in_page = last & ((1 << p.page_shift) - 1);
+    for (int i = threadIdx.x; i < p.kv_heads * p.head_dim; i += 128) {
+        const int h = i / p.head_dim, c = i % p.head_dim;
+        const_cast<unsigned short*>(p.key_pages)[entry * p.kpool.page + in_page * p.kpool.token + h * p.kpool.head + c] =
+            p.key[t * p.k.token + h * p.k.head + c];
+        const_cast<unsigned short*>(
+            p.value_pages)[entry * p.vpool.page + in_page * p.vpool.token + h * p.vpool.head + c] =
+            p.value[t * p.v.token + h * p.v.head + c];
+    }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(128) attention_kernel(const AttentionArgs p, const bool prefill) {
+    constexpr int kLane = D / 32;
+    const int t = blockIdx.x, lane = threadIdx.x & 31;
+    int r = -1, keys = 0;
+    if (prefill) {
+        int low = 0, high = p.requests;
+        while (high - low > 1) {
+            const int middle = (low + high) >> 1;
+            if (p.index[middle] <= t)
+                low = middle;
+            else
+                high = middle;
+        }
+        const int first = p.index[low], end = p.index[low + 1];
+        if (t >= first && t < end) {
+            r = low;
+            keys = min(p.lengths[r], p.width << p.page_shift) - (end - 1 - t);
+        } else if (!p.zero_rest) {
+            return;
+        }
+    } else {
+        r = p.index != nullptr ? p.index[t] : t;
+        if (r >= 0 && r < p.requests) keys = min(p.lengths[r], p.width << p.page_shift);
+    }
+    const T* pools[2] = {reinterpret_cast<const T*>(p.key_pages), reinterpret_cast<const T*>(p.value_pages)};
+    for (int h = threadIdx.x >> 5; h < p.heads; h += 4) {
+        const int kvh = h / (p.heads / p.kv_heads);
+        float q[kLane], o[kLane], m = -INFINITY, l = 0.f;
+        for (int i = 0; i < kLane; ++i) {
+            q[i] = widen(reinterpret_cast<const T*>(p.query)[t * p.q.token + h * p.q.head + lane * kLane + i]) * p.scale;
+            o[i] = 0.f;
+        }
+        for (int j = 0; j < keys; ++j) {
+            const int entry = p.table[static_cast<size_t>(r) * p.width + (j >> p.page_shift)];
+            if (entry < 0 || entry >= p.pages) continue;
+            const long long in_page = j & ((1 << p.page_shift) - 1);
+            const T* k = pools[0] + entry * p.kpool.page + in_page * p.kpool.token + kvh * p.kpool.head + lane * kLane;
+            const T* v = pools[1] + entry * p.vpool.page + in_page * p.vpool.token + kvh * p.vpool.head + lane * kLane;
+            float s = 0.f;
+            for (int i = 0; i < kLane; ++i) s = fmaf(q[i], widen(k[i]), s);
+            for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+            const float highest = fmaxf(m, s), base = highest == -INFINITY ? 0.f : highest;
+            const float before = __expf(m - base), weight = exp2f((s - base) * kLog2e + kWeightShift<T>);
+            l = l * before + weight;
+            for (int i = 0; i < kLane; ++i) o[i] = fmaf(weight, widen(v[i]), o[i] * before);
+            m = highest;
+        }
+        T* out = reinterpret_cast<T*>(p.out) + (static_cast<size_t>(t) * p.heads + h) * D + lane * kLane;
+        for (int i = 0; i < kLane; ++i) out[i] = narrow<T>(l == 0.f ? 0.f : o[i] / l);
+    }
+}
+
+template <typename T>
+cudaError_t launch_attention(const AttentionArgs& p, bool prefill, cudaStream_t stream) {
+    if (p.key != nullptr) append_last_kernel<T><<<p.tokens, 128, 0, stream>>>(p);
+    if (p.head_dim == 64)
+        attention_kernel<T, 64><<<p.tokens, 128, 0, stream>>>(p, prefill);
+    else if (p.head_dim == 128)
+        attention_kernel<T, 128><<<p.tokens, 128, 0, stream>>>(p, prefill);
+    else
+        attention_kernel<T, 256><<<p.tokens, 128, 0, stream>>>(p, prefill);
+    return cudaGetLastError();
+}
+
+// ---------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------
+bool page_size_covered(int page_size) {
+    return page_size >= 8 && page_size <= 1024 && (page_size & (page_size - 1)) == 0;
+}
+
+int shift_of(int page_size) {
+    int shift = 0;
+    while ((1 << shift) < page_size) ++shift;
+    return shift;
+}
+
+// Rows of 16-bit values that the kernels read 16 bytes at a time.
+bool aligned(uint64_t address, std::initializer_list<int64_t> strides) {
+    if (address % 16 != 0) return false;
+    for (const int64_t s : strides)
+        if (s < 0 || s % 8 != 0) return false;
+    return true;
+}
+
+int attention_args(const mb_paged_attention_args* a, bool prefill, AttentionArgs& p) {
+    if (a == nullptr) return MB_ERR_INVALID;
+    if (a->tokens < 1 || a->requests < 1 || a->kv_heads < 1 || a->heads < 1 || a->heads % a->kv_heads != 0 ||
+        a->width < 1 || a->pages < 1 || a->query == 0 || a->key_pages == 0 || a->value_pages == 0 || a->block_table == 0 ||
+        a->lengths == 0 || a->out == 0 || (a->key == 0) != (a->value == 0) ||
+        (prefill && (a->index == 0 || a->key != 0)))
+        return MB_ERR_INVALID;
+    if ((a->element != MB_BF16 && a->element != MB_FP16) || !page_size_covered(a->page_size) ||
+        (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) ||
+        static_cast<int64_t>(a->width) * a->page_size > 0x7fffffffll)
+        return MB_ERR_UNSUPPORTED;
+    if (!aligned(a->query, {a->query_token, a->query_head}) || !aligned(a->out, {}) ||
+        !aligned(a->key_pages, {a->kpool_page, a->kpool_token, a->kpool_head}) ||
+        !aligned(a->value_pages, {a->vpool_page, a->vpool_token, a->vpool_head}) ||
+        (a->key != 0 && (!aligned(a->key, {a->key_token, a->key_head}) ||
+                         !aligned(a->value, {a->value_token, a->value_head}))) ||
+        a->block_table % 4 || a->lengths % 4 || a->index % 4 || a->status % 4)
+        return MB_ERR_INVALID;
+    p.tokens = a->tokens;
+    p.requests = a->requests;
+    p.heads = a->heads;
+    p.kv_heads = a->kv_heads;
+    p.head_dim = a->head_dim;
+    p.width = a->width;
+    p.pages = a->pages;
+    p.page_shift = shift_of(a->page_size);
+    p.zero_rest = a->zero_rest;
+    p.scale = a->scale;
+    p.q = {a->query_token, a->query_head};
+    p.k = {a->key_token, a->key_head};
+    p.v = {a->value_token, a->value_head};
+    p.kpool = {a->kpool_page, a->kpool_token, a->kpool_head};
+    p.vpool = {a->vpool_page, a->vpool_token, a->vpool_head};
+    p.query = reinterpret_cast<const unsigned short*>(a->query);
+    p.key = reinterpret_cast<const unsigned short*>(a->key);
+    p.value = reinterpret_cast<const unsigned short*>(a->value);
+    p.key_pages = reinterpret_cast<const unsigned short*>(a->key_pages);
+    p.value_pages = reinterpret_cast<const unsigned short*>(a->value_pages);
+    p.table = reinterpret_cast<const int*>(a->block_table);
+    p.lengths = reinterpret_cast<const int*>(a->lengths);
+    p.index = reinterpret_cast<const int*>(a->index);
+    p.out = reinterpret_cast<unsigned short*>(a->out);
+    p.status = reinterpret_cast<int*>(a->status);
+    return MB_OK;
+}
+
+int attention(const mb_paged_attention_args* a, bool prefill, void* stream) {
+    AttentionArgs p;
+    const int rc = attention_args(a, prefill, p);
+    if (rc != MB_OK) return rc;
+    const cudaError_t err = a->element == MB_BF16
+                                ? launch_attention<__nv_bfloat16>(p, prefill, static_cast<cudaStream_t>(stream))
+                                : launch_attention<__half>(p, prefill, static_cast<cudaStream_t>(stream));
+    return err == cudaSuccess ? MB_OK : cuda_error(err, prefill ? "mb_paged_prefill" : "mb_paged_attention");
+}
+
+}  // namespace paged
+}  // namespace mb
+
+extern "C" {
+
+int mb_paged_reserve(const mb_paged_reserve_args* a, void* stream) {
+    using namespace mb::paged;
+    if (a == nullptr || a->requests < 1 || a->width < 1 || a->pages < 1 || a->max_tokens < 0 || a->counts == 0 ||
+        a->lengths == 0 || a->block_table == 0 || a->free_pages == 0 || a->free_count == 0 || a->offsets == 0 ||
+        a->granted == 0 || (a->max_tokens > 0 && (a->slots == 0 || a->positions == 0 || a->rows == 0)))
+        return MB_ERR_INVALID;
+    if ((a->counts | a->lengths | a->block_table | a->free_pages | a->free_count | a->offsets | a->rows | a->granted) % 4 ||
+        (a->slots | a->positions) % 8)
+        return MB_ERR_INVALID;
+    if (a->requests > 8192 || !page_size_covered(a->page_size) ||
+        static_cast<int64_t>(a->width) * a->page_size > 0x7fffffffll)
+        return MB_ERR_UNSUPPORTED;
+    ReserveArgs p;
+    p.requests = a->requests;
+    p.width = a->width;
+    p.pages = a->pages;
+    p.page_shift = shift_of(a->page_size);
+    p.max_tokens = a->max_tokens;
+    p.counts = reinterpret_cast<const int*>(a->counts);
+    p.lengths = reinterpret_cast<int*>(a->lengths);
+    p.table = reinterpret_cast<int*>(a->block_table);
+    p.stack = reinterpret_cast<int*>(a->free_pages);
+    p.free_count = reinterpret_cast<int*>(a->free_count);
+    p.offsets = reinterpret_cast<int*>(a->offsets);
+    p.rows = reinterpret_cast<int*>(a->rows);
+    p.granted = reinterpret_cast<int*>(a->granted);
+    p.slots = reinterpret_cast<long long*>(a->slots);
+    p.positions = reinterpret_cast<long long*>(a->positions);
+    const int smem = (3 * a->requests + 1) * 4;
+    if (smem > 48 * 1024) {
+        const cudaError_t err =
+            cudaFuncSetAttribute(reserve_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (err != cudaSuccess) return mb::cuda_error(err, "mb_paged_reserve");
+    }
+    reserve_kernel<<<1, kReserveThreads, smem, static_cast<cudaStream_t>(stream)>>>(p);
+    const cudaError_t err = cudaGetLastError();
+    return err == cudaSuccess ? MB_OK : mb::cuda_error(err, "mb_paged_reserve");
+}
+
+int mb_paged_append(const mb_paged_append_args* a, void* stream) {
+    using namespace mb::paged;
+    if (a == nullptr || a->tokens < 1 || a->kv_heads < 1 || a->pages < 1 || a->key == 0 || a->value == 0 ||
+        a->key_pages == 0 || a->value_pages == 0 || a->slots == 0 || a->slots % 8)
+        return MB_ERR_INVALID;
+    if (!page_size_covered(a->page_size) || (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256))
+        return MB_ERR_UNSUPPORTED;
+    if (!aligned(a->key, {a->key_token, a->key_head}) || !aligned(a->value, {a->value_token, a->value_head}) ||
+        !aligned(a->key_pages, {a->kpool_page, a->kpool_token, a->kpool_head}) ||
+        !aligned(a->value_pages, {a->vpool_page, a->vpool_token, a->vpool_head}))
+        return MB_ERR_INVALID;
+    AppendArgs p;
+    p.tokens = a->tokens;
+    p.kv_heads = a->kv_heads;
+    p.vectors = a->head_dim / 8;
+    p.page_shift = shift_of(a->page_size);
+    p.slots_end = static_cast<long long>(a->pages) * a->page_size;
+    p.key = {a->key_token, a->key_head};
+    p.value = {a->value_token, a->value_head};
+    p.kpool = {a->kpool_page, a->kpool_token, a->kpool_head};
+    p.vpool = {a->vpool_page, a->vpool_token, a->vpool_head};
+    p.k = reinterpret_cast<const unsigned short*>(a->key);
+    p.v = reinterpret_cast<const unsigned short*>(a->value);
+    p.key_pages = reinterpret_cast<unsigned short*>(a->key_pages);
+    p.value_pages = reinterpret_cast<unsigned short*>(a->value_pages);
+    p.slots = reinterpret_cast<const long long*>(a->slots);
+    const long long blocks = (static_cast<long long>(a->tokens) * a->kv_heads * p.vectors + 255) / 256;
+    append_kernel<<<static_cast<int>(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        p);
+    const cudaError_t err = cudaGetLastError();
+    return err == cudaSuccess ? MB_OK : mb::cuda_error(err, "mb_paged_append");
+}
+
+int64_t mb_paged_attention_workspace(const mb_paged_attention_args* a) {
+    mb::paged::AttentionArgs p;
+    const int rc = mb::paged::attention_args(a, false, p);
+    return rc == MB_OK ? 0 : -rc;
+}
+
+int mb_paged_attention(const mb_paged_attention_args* a, void* stream) { return mb::paged::attention(a, false, stream); }
+
+int64_t mb_paged_prefill_workspace(const mb_paged_attention_args* a) {
+    mb::paged::AttentionArgs p;
+    const int rc = mb::paged::attention_args(a, true, p);
+    return rc == MB_OK ? 0 : -rc;
+}
+
+int mb_paged_prefill(const mb_paged_attention_args* a, void* stream) { return mb::paged::attention(a, true, stream); }
+
+}  // extern "C"

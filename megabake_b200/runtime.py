@@ -147,6 +147,42 @@ class GreedyArgs(ctypes.Structure):
     ]
 
 
+class PagedReserveArgs(ctypes.Structure):
+    """``mb_paged_reserve_args``."""
+
+    _fields_ = [(name, ctypes.c_int32) for name in
+                ("requests", "width", "pages", "page_size", "max_tokens", "reserved")] + [
+        (name, ctypes.c_uint64) for name in
+        ("counts", "lengths", "block_table", "free_pages", "free_count", "offsets", "slots",
+         "positions", "rows", "granted")]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    """``mb_paged_append_args``."""
+
+    _fields_ = [(name, ctypes.c_int32) for name in
+                ("tokens", "kv_heads", "head_dim", "pages", "page_size", "reserved")] + [
+        (name, ctypes.c_int64) for name in
+        ("key_token", "key_head", "value_token", "value_head", "kpool_page", "kpool_token",
+         "kpool_head", "vpool_page", "vpool_token", "vpool_head")] + [
+        (name, ctypes.c_uint64) for name in ("key", "value", "key_pages", "value_pages", "slots")]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    """``mb_paged_attention_args``."""
+
+    _fields_ = [(name, ctypes.c_int32) for name in
+                ("element", "tokens", "requests", "heads", "kv_heads", "head_dim", "width", "pages",
+                 "page_size", "zero_rest")] + [
+        ("scale", ctypes.c_float), ("reserved", ctypes.c_int32)] + [
+        (name, ctypes.c_int64) for name in
+        ("query_token", "query_head", "key_token", "key_head", "value_token", "value_head",
+         "kpool_page", "kpool_token", "kpool_head", "vpool_page", "vpool_token", "vpool_head")] + [
+        (name, ctypes.c_uint64) for name in
+        ("query", "key", "value", "key_pages", "value_pages", "block_table", "lengths", "index",
+         "out", "workspace", "status")]
+
+
 class Status(ctypes.Structure):
     _fields_ = [
         ("code", ctypes.c_int32),
@@ -172,6 +208,8 @@ EXPORTS = (
     "mb_plan_reset", "mb_plan_set_trace", "mb_prefill_cuts", "mb_plan_destroy", "mb_strerror", "mb_status_string", "mb_last_cuda_error",
     "mb_abi_version", "mb_fixed_smem_bytes", "mb_stage_bytes", "mb_max_smem_bytes",
     "mb_attention_decode_static", "mb_greedy_advance",
+    "mb_paged_reserve", "mb_paged_append", "mb_paged_attention_workspace", "mb_paged_attention",
+    "mb_paged_prefill_workspace", "mb_paged_prefill",
 )
 
 _library = None
@@ -231,6 +269,14 @@ def load_library(path: Path | None = None) -> ctypes.CDLL:
         lib.mb_attention_decode_static.restype = ctypes.c_int
         lib.mb_greedy_advance.argtypes = [ctypes.POINTER(GreedyArgs), ctypes.c_void_p]
         lib.mb_greedy_advance.restype = ctypes.c_int
+        for name, args in (("mb_paged_reserve", PagedReserveArgs), ("mb_paged_append", PagedAppendArgs),
+                           ("mb_paged_attention", PagedAttentionArgs),
+                           ("mb_paged_prefill", PagedAttentionArgs)):
+            getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+            getattr(lib, name).restype = ctypes.c_int
+        for name in ("mb_paged_attention_workspace", "mb_paged_prefill_workspace"):
+            getattr(lib, name).argtypes = [ctypes.POINTER(PagedAttentionArgs)]
+            getattr(lib, name).restype = ctypes.c_int64
         if lib.mb_abi_version() != MB_ABI_VERSION:
             raise _native_error(
                 f"{target} speaks ABI {lib.mb_abi_version()}, the host expects {MB_ABI_VERSION}"
