@@ -465,7 +465,7 @@ enum mb_element { MB_BF16 = 0, MB_FP16 = 1 };
  * offsets[r + 1] - 1 for row r: its slot page * page_size + offset, position, and row; places behind the
  * last: -1, 0, -1.  granted[r]: tokens granted, or dropped (negative).                            */
 typedef struct mb_paged_reserve_args {
-    int32_t requests;         /* rows, at most 8192                                       */
+    int32_t requests;         /* rows, at most 2048                                       */
     int32_t width;            /* pages per row of the table; width * page_size < 2^31     */
     int32_t pages;            /* of the pool: entries of free_pages                       */
     int32_t page_size;
@@ -507,7 +507,8 @@ int mb_paged_append(const mb_paged_append_args* args, void* stream);
  * appended: the one at position p attends the keys 0..p.  A query before position 0 has none.  Queries of
  * no request: zero where zero_rest is set, else left as they were.  offsets do not fall and lie in 0..tokens.
  *
- * workspace: as many bytes as the _workspace call says (0: none), 256-byte aligned, not shared by calls that
+ * At most 2048 requests and, for mb_paged_attention, 2048 tokens, whose rows of the table hold fewer than 2^37
+ * positions together.  workspace: as many bytes as the _workspace call says (0: none), 256-byte aligned, not shared by calls that
  * may overlap; negative: MB_ERR_*.  status: optional int32 [1], receives an enum mb_status_code if a wait of the
  * kernel ran out (it is not written otherwise); the outputs are then not valid.                  */
 typedef struct mb_paged_attention_args {

@@ -241,59 +241,25 @@ __device__ __forceinline__ __half narrow(float v) {
     return __float2half_rn(v);
 }
 
-// Weights are 2^(log2(e) (score - highest) + shift).  fp16: up by 2^15, so that small ones keep their digits when they
-// are rounded to 16 bits; bf16: down by 2^31, so that no sum over a context, which has fewer than 2^31 keys,
-// overflows whatever the values are (fp16 values cannot).
-constexpr float kLog2e = 1.4426950408889634f;
-template <typename T>
-constexpr float kWeightShift = 15.f;
-template <>
-constexpr float kWeightShift<__nv_bfloat16> = -31.f;
-
-// The last key and value of every query's request, where they belong.
-template <typename T>
-__global__ void __launch_bounds__(128) append_last_kernel(const AttentionArgs p) {
-    const int t = blockIdx.x, r = p.index != nullptr ? p.index[t] : t;
-    if (r < 0 || r >= p.requests) return;
-    const int length = min(p.lengths[r], p.width << p.page_shift);
-    if (length < 1) return;
-    const int last = length - 1, entry = p.table[static_cast<size_t>(r) * p.width + (last >> p.page_shift)];
-    if (entry < 0 || entry >= p.pages) return;
-    const long long in_page = last & ((1 << p.page_shift) - 1);
-    for (int i = threadIdx.x; i < p.kv_heads * p.head_dim; i += 128) {
-        const int h = i / p.head_dim, c = i % p.head_dim;
-        const_cast<unsigned short*>(p.key_pages)[entry * p.kpool.page + in_page * p.kpool.token + h * p.kpool.head + c] =
-            p.key[t * p.k.token + h * p.k.head + c];
-        const_cast<unsigned short*>(
-            p.value_pages)[entry * p.vpool.page + in_page * p.vpool.token + h * p.vpool.head + c] =
-            p.value[t * p.v.token + h * p.v.head + c];
-    }
-}
-
 template <typename T, int D>
-__global__ void __launch_bounds__(128) attention_kernel(const AttentionArgs p, const bool prefill) {
+__global__ void __launch_bounds__(128) attention_kernel(const AttentionArgs p) {
     constexpr int kLane = D / 32;
     const int t = blockIdx.x, lane = threadIdx.x & 31;
     int r = -1, keys = 0;
-    if (prefill) {
-        int low = 0, high = p.requests;
-        while (high - low > 1) {
-            const int middle = (low + high) >> 1;
-            if (p.index[middle] <= t)
-                low = middle;
-            else
-                high = middle;
-        }
-        const int first = p.index[low], end = p.index[low + 1];
-        if (t >= first && t < end) {
-            r = low;
-            keys = min(p.lengths[r], p.width << p.page_shift) - (end - 1 - t);
-        } else if (!p.zero_rest) {
-            return;
-        }
-    } else {
-        r = p.index != nullptr ? p.index[t] : t;
-        if (r >= 0 && r < p.requests) keys = min(p.lengths[r], p.width << p.page_shift);
+    int low = 0, high = p.requests;
+    while (high - low > 1) {
+        const int middle = (low + high) >> 1;
+        if (p.index[middle] <= t)
+            low = middle;
+        else
+            high = middle;
+    }
+    const int first = p.index[low], end = p.index[low + 1];
+    if (t >= first && t < end) {
+        r = low;
+        keys = min(p.lengths[r], p.width << p.page_shift) - (end - 1 - t);
+    } else if (!p.zero_rest) {
+        return;
     }
     const T* pools[2] = {reinterpret_cast<const T*>(p.key_pages), reinterpret_cast<const T*>(p.value_pages)};
     for (int h = threadIdx.x >> 5; h < p.heads; h += 4) {
@@ -324,14 +290,13 @@ __global__ void __launch_bounds__(128) attention_kernel(const AttentionArgs p, c
 }
 
 template <typename T>
-cudaError_t launch_attention(const AttentionArgs& p, bool prefill, cudaStream_t stream) {
-    if (p.key != nullptr) append_last_kernel<T><<<p.tokens, 128, 0, stream>>>(p);
+cudaError_t launch_attention(const AttentionArgs& p, cudaStream_t stream) {
     if (p.head_dim == 64)
-        attention_kernel<T, 64><<<p.tokens, 128, 0, stream>>>(p, prefill);
+        attention_kernel<T, 64><<<p.tokens, 128, 0, stream>>>(p);
     else if (p.head_dim == 128)
-        attention_kernel<T, 128><<<p.tokens, 128, 0, stream>>>(p, prefill);
+        attention_kernel<T, 128><<<p.tokens, 128, 0, stream>>>(p);
     else
-        attention_kernel<T, 256><<<p.tokens, 128, 0, stream>>>(p, prefill);
+        attention_kernel<T, 256><<<p.tokens, 128, 0, stream>>>(p);
     return cudaGetLastError();
 }
 
@@ -374,6 +339,7 @@ int attention_args(const mb_paged_attention_args* a, bool prefill, AttentionArgs
                          !aligned(a->value, {a->value_token, a->value_head}))) ||
         a->block_table % 4 || a->lengths % 4 || a->index % 4 || a->status % 4)
         return MB_ERR_INVALID;
+    if (a->requests > kMaxRows) return MB_ERR_UNSUPPORTED;
     p.tokens = a->tokens;
     p.requests = a->requests;
     p.heads = a->heads;
@@ -399,17 +365,7 @@ int attention_args(const mb_paged_attention_args* a, bool prefill, AttentionArgs
     p.index = reinterpret_cast<const int*>(a->index);
     p.out = reinterpret_cast<unsigned short*>(a->out);
     p.status = reinterpret_cast<int*>(a->status);
-    return MB_OK;
-}
-
-int attention(const mb_paged_attention_args* a, bool prefill, void* stream) {
-    AttentionArgs p;
-    const int rc = attention_args(a, prefill, p);
-    if (rc != MB_OK) return rc;
-    const cudaError_t err = a->element == MB_BF16
-                                ? launch_attention<__nv_bfloat16>(p, prefill, static_cast<cudaStream_t>(stream))
-                                : launch_attention<__half>(p, prefill, static_cast<cudaStream_t>(stream));
-    return err == cudaSuccess ? MB_OK : cuda_error(err, prefill ? "mb_paged_prefill" : "mb_paged_attention");
+    return prefill ? MB_OK : decode_admitted(p);
 }
 
 }  // namespace paged
@@ -426,7 +382,7 @@ int mb_paged_reserve(const mb_paged_reserve_args* a, void* stream) {
     if ((a->counts | a->lengths | a->block_table | a->free_pages | a->free_count | a->offsets | a->rows | a->granted) % 4 ||
         (a->slots | a->positions) % 8)
         return MB_ERR_INVALID;
-    if (a->requests > 8192 || !page_size_covered(a->page_size) ||
+    if (a->requests > kMaxRows || !page_size_covered(a->page_size) ||
         static_cast<int64_t>(a->width) * a->page_size > 0x7fffffffll)
         return MB_ERR_UNSUPPORTED;
     ReserveArgs p;
@@ -492,10 +448,16 @@ int mb_paged_append(const mb_paged_append_args* a, void* stream) {
 int64_t mb_paged_attention_workspace(const mb_paged_attention_args* a) {
     mb::paged::AttentionArgs p;
     const int rc = mb::paged::attention_args(a, false, p);
-    return rc == MB_OK ? 0 : -rc;
+    return rc == MB_OK ? mb::paged::decode_workspace(p) : -rc;
 }
 
-int mb_paged_attention(const mb_paged_attention_args* a, void* stream) { return mb::paged::attention(a, false, stream); }
+int mb_paged_attention(const mb_paged_attention_args* a, void* stream) {
+    mb::paged::AttentionArgs p;
+    const int rc = mb::paged::attention_args(a, false, p);
+    if (rc != MB_OK) return rc;
+    return mb::paged::decode_attention(p, a->element, reinterpret_cast<void*>(a->workspace),
+                                       static_cast<cudaStream_t>(stream));
+}
 
 int64_t mb_paged_prefill_workspace(const mb_paged_attention_args* a) {
     mb::paged::AttentionArgs p;
@@ -503,6 +465,15 @@ int64_t mb_paged_prefill_workspace(const mb_paged_attention_args* a) {
     return rc == MB_OK ? 0 : -rc;
 }
 
-int mb_paged_prefill(const mb_paged_attention_args* a, void* stream) { return mb::paged::attention(a, true, stream); }
+int mb_paged_prefill(const mb_paged_attention_args* a, void* stream) {
+    using namespace mb::paged;
+    AttentionArgs p;
+    const int rc = attention_args(a, true, p);
+    if (rc != MB_OK) return rc;
+    const cudaError_t err = a->element == MB_BF16
+                                ? launch_attention<__nv_bfloat16>(p, static_cast<cudaStream_t>(stream))
+                                : launch_attention<__half>(p, static_cast<cudaStream_t>(stream));
+    return err == cudaSuccess ? MB_OK : mb::cuda_error(err, "mb_paged_prefill");
+}
 
 }  // extern "C"

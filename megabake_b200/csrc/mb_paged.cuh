@@ -1,10 +1,17 @@
 // What the kernels around the paged key-value cache share.
 #pragma once
 
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
 
 namespace mb {
 namespace paged {
+
+constexpr int kMaxRows = 2048;   // requests of a table, and tokens of a step of one token a request
 
 struct Strides2 {
     long long token, head;   // elements
@@ -24,6 +31,37 @@ struct AttentionArgs {
     unsigned short* out;
     int* status;
 };
+
+// Weights are 2^(log2(e) (score - highest) + shift).  fp16: up by 2^15, so that small ones keep their digits when they
+// are rounded to 16 bits; bf16: down by 2^31, so that no sum over a context, which has fewer than 2^31 keys,
+// overflows whatever the values are (fp16 values cannot).
+constexpr float kLog2e = 1.4426950408889634f;
+template <typename T>
+constexpr float kWeightShift = 15.f;
+template <>
+constexpr float kWeightShift<__nv_bfloat16> = -31.f;
+
+// Four neighbouring outputs from sums of weighted values and the sum of weights; no weight at all: zero.
+template <typename T>
+__device__ __forceinline__ void store_output(unsigned short* to, float4 sum, float total) {
+    const float inverse = total == 0.f ? 0.f : 1.f / total;
+    uint2 packed;
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 a = __floats2half2_rn(sum.x * inverse, sum.y * inverse);
+        const __half2 b = __floats2half2_rn(sum.z * inverse, sum.w * inverse);
+        packed = make_uint2(*reinterpret_cast<const unsigned int*>(&a), *reinterpret_cast<const unsigned int*>(&b));
+    } else {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(sum.x * inverse, sum.y * inverse);
+        const __nv_bfloat162 b = __floats2bfloat162_rn(sum.z * inverse, sum.w * inverse);
+        packed = make_uint2(*reinterpret_cast<const unsigned int*>(&a), *reinterpret_cast<const unsigned int*>(&b));
+    }
+    *reinterpret_cast<uint2*>(to) = packed;
+}
+
+// mb_paged_decode.cu
+int decode_admitted(const AttentionArgs& a);
+int64_t decode_workspace(const AttentionArgs& a);
+int decode_attention(const AttentionArgs& a, int element, void* workspace, cudaStream_t stream);
 
 }  // namespace paged
 }  // namespace mb

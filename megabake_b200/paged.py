@@ -37,7 +37,7 @@ __all__ = ["PagedBatch", "PagedState", "paged_append", "paged_kv_attention", "pa
 
 _ELEMENTS = {torch.bfloat16: 0, torch.float16: 1}
 _HEAD_DIMS = (64, 128, 256)
-_MAX_REQUESTS = 8192
+_MAX_REQUESTS = 2048
 _ready: set[int] = set()   # devices that are known to be sm_100
 
 

@@ -72,7 +72,7 @@ def _run_reserve(counts, state, page, max_tokens):
 
 @pytest.mark.parametrize("requests,width,page,pages", [(1, 1, 8, 1), (1, 40, 16, 64), (7, 5, 8, 30), (33, 9, 64, 200),
                                                        (300, 6, 8, 900), (1024, 3, 16, 2500), (1025, 4, 8, 3000),
-                                                       (8192, 2, 8, 9000)])
+                                                       (2048, 2, 8, 2500)])
 def test_reserve_against_the_definition(requests, width, page, pages):
     rng = random.Random(requests)
     stack = list(range(pages))

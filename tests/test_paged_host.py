@@ -41,7 +41,7 @@ def _attention_args(**changes):
 @pytest.mark.parametrize("changes,code", [
     (dict(requests=0), INVALID), (dict(width=0), INVALID), (dict(pages=0), INVALID), (dict(max_tokens=-1), INVALID),
     (dict(counts=0), INVALID), (dict(free_count=0), INVALID), (dict(slots=0), INVALID), (dict(rows=0), INVALID),
-    (dict(slots=4100), INVALID), (dict(lengths=4097), INVALID), (dict(requests=8193), UNSUPPORTED),
+    (dict(slots=4100), INVALID), (dict(lengths=4097), INVALID), (dict(requests=2049), UNSUPPORTED),
     (dict(page_size=4), UNSUPPORTED), (dict(page_size=48), UNSUPPORTED), (dict(page_size=2048), UNSUPPORTED),
     (dict(width=1 << 27, page_size=16), UNSUPPORTED),
 ])
@@ -102,7 +102,7 @@ def test_state_tensors():
 
 
 @pytest.mark.parametrize("changes", [dict(page_size=12), dict(page_size=4), dict(head_dim=96), dict(layers=0),
-                                     dict(requests=0), dict(requests=8193), dict(capacity=0), dict(pages=0),
+                                     dict(requests=0), dict(requests=2049), dict(capacity=0), dict(pages=0),
                                      dict(dtype=torch.float32)])
 def test_state_refuses(changes):
     with pytest.raises(ValueError):
