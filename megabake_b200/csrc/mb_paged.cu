@@ -21,9 +21,14 @@ namespace paged {
 // Three exclusive sums over the requests decide everything: pages given back by the rows behind r (where r's pages
 // go on the stack), tokens and pages wanted by the rows up to r (whether r is granted), tokens and pages granted
 // before r (its places, and which entries of the stack are its pages).  A thread sums a run of neighbouring rows, the
-// block scans the threads.  What a row looks up afterwards lies in shared memory.
+// block scans the threads; what a row looks up afterwards lies in shared memory.
+//
+// Latency bounds it: one trip to L2 after the other (lengths, pages given back, pages granted, slots), and with many
+// tokens 20 bytes for each of their places.  A thread-block cluster shares the rows and places, and every block of it
+// works the sums out for itself: its barrier is all that tables which are read and updated in one launch need.
 // ---------------------------------------------------------------------------------------
-constexpr int kReserveThreads = 1024;
+constexpr int kReserveThreads = 256;
+constexpr int kReserveCluster = 8;
 
 struct ReserveArgs {
     int requests, width, pages, page_shift, max_tokens;
@@ -36,101 +41,112 @@ struct Pair {
     long long a, b;
 };
 
-// Exclusive sums over the threads of the block, and the totals.  Every thread calls it.
-__device__ __forceinline__ Pair exclusive_sums(Pair v, Pair* warp_sums, Pair& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    Pair inclusive = v;
+__device__ __forceinline__ Pair inclusive_sums(Pair v, int lane) {
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const long long a = __shfl_up_sync(0xffffffffu, inclusive.a, d);
-        const long long b = __shfl_up_sync(0xffffffffu, inclusive.b, d);
+        const long long a = __shfl_up_sync(0xffffffffu, v.a, d);
+        const long long b = __shfl_up_sync(0xffffffffu, v.b, d);
         if (lane >= d) {
-            inclusive.a += a;
-            inclusive.b += b;
+            v.a += a;
+            v.b += b;
         }
     }
+    return v;
+}
+
+// Exclusive sums over the threads of the block, and the totals.  Every thread calls it.
+__device__ __forceinline__ Pair exclusive_sums(Pair v, Pair* warp_sums, Pair& total) {
+    constexpr int kWarps = kReserveThreads / 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const Pair mine = inclusive_sums(v, lane);
     __syncthreads();  // the sums of a call before have been read
-    if (lane == 31) warp_sums[warp] = inclusive;
+    if (lane == 31) warp_sums[warp] = mine;
     __syncthreads();
-    Pair before = {0, 0};
-    total = {0, 0};
-    for (int w = 0; w < kReserveThreads / 32; ++w) {
-        if (w == warp) before = total;
-        total.a += warp_sums[w].a;
-        total.b += warp_sums[w].b;
-    }
-    return {before.a + inclusive.a - v.a, before.b + inclusive.b - v.b};
+    const Pair warps = inclusive_sums(lane < kWarps ? warp_sums[lane] : Pair{0, 0}, lane);
+    total = {__shfl_sync(0xffffffffu, warps.a, kWarps - 1), __shfl_sync(0xffffffffu, warps.b, kWarps - 1)};
+    const Pair before = {__shfl_sync(0xffffffffu, warps.a, (warp + 31) & 31),
+                         __shfl_sync(0xffffffffu, warps.b, (warp + 31) & 31)};
+    return {(warp > 0 ? before.a : 0) + mine.a - v.a, (warp > 0 ? before.b : 0) + mine.b - v.b};
+}
+
+// Everything the cluster wrote before is seen by all of it afterwards; what lies in L1 from before is not used again.
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 __global__ void __launch_bounds__(kReserveThreads) reserve_kernel(const ReserveArgs p) {
     extern __shared__ int rows_smem[];
     const int R = p.requests, page = 1 << p.page_shift;
-    int* kept_tokens = rows_smem;       // [R] tokens that stay before any are granted
-    int* first_page = rows_smem + R;    // [R] pages given back by later rows, then pages granted to earlier ones
-    int* offset = rows_smem + 2 * R;    // [R + 1]
+    int* held_tokens = rows_smem;           // [R] tokens at first
+    int* kept_tokens = rows_smem + R;       // [R] that stay before any are granted
+    int* first_page = rows_smem + 2 * R;    // [R] pages given back by later rows, then pages granted to earlier ones
+    int* offset = rows_smem + 3 * R;        // [R + 1]
     __shared__ Pair warp_sums[kReserveThreads / 32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // gridDim.x is the cluster
+    const int tid = threadIdx.x, lane = tid & 31, rank = blockIdx.x;
+    const int warp = rank * (kReserveThreads / 32) + (tid >> 5), warps = gridDim.x * (kReserveThreads / 32);
     const int per_thread = (R + kReserveThreads - 1) / kReserveThreads;
     const int r0 = min(tid * per_thread, R), r1 = min(r0 + per_thread, R);
     const int capacity = p.width << p.page_shift;
     auto pages_of = [&](long long tokens) { return static_cast<int>((tokens + page - 1) >> p.page_shift); };
-    auto held_tokens = [&](int r) { return min(max(p.lengths[r], 0), capacity); };
 
-    // what is given back
-    Pair sum = {0, 0}, total;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int free_before = *p.free_count;
+    Pair back = {0, 0}, wanted = {0, 0}, total;
     for (int r = r0; r < r1; ++r) {
-        const int count = p.counts[r], held = held_tokens(r);
+        const int count = p.counts[r], held = min(max(p.lengths[r], 0), capacity);
         const int kept = count < 0 ? static_cast<int>(max(static_cast<long long>(held) + count, 0ll)) : held;
+        held_tokens[r] = held;
         kept_tokens[r] = kept;
-        sum.a += pages_of(held) - pages_of(kept);
+        offset[r] = 0;
+        back.a += pages_of(held) - pages_of(kept);
+        const long long after = static_cast<long long>(kept) + count;
+        if (count > 0 && after <= capacity) {
+            offset[r] = count;   // what it wants
+            wanted.a += count;
+            wanted.b += pages_of(after) - pages_of(kept);
+        }
     }
-    Pair before = exclusive_sums(sum, warp_sums, total);
+    // what is given back
+    Pair before = exclusive_sums(back, warp_sums, total);
+    const long long given = total.a, available = free_before + given;
     long long behind = total.a - before.a;
     for (int r = r0; r < r1; ++r) {
-        behind -= pages_of(held_tokens(r)) - pages_of(kept_tokens[r]);
+        behind -= pages_of(held_tokens[r]) - pages_of(kept_tokens[r]);
         first_page[r] = static_cast<int>(behind);
     }
-    const int free_before = *p.free_count;
-    const long long available = free_before + total.a;
-    __syncthreads();
-    for (int r = warp; r < R; r += kReserveThreads / 32) {
-        const int held = pages_of(held_tokens(r)), kept = pages_of(kept_tokens[r]);
-        int* row = p.table + static_cast<size_t>(r) * p.width;
-        for (int j = kept + lane; j < held; j += 32) {
-            const long long at = static_cast<long long>(free_before) + first_page[r] + held - 1 - j;
-            if (at >= 0 && at < p.pages) p.stack[at] = row[j];
-            row[j] = -1;
+    if (given > 0) {
+        __syncthreads();
+        for (int r = warp; r < R; r += warps) {
+            const int held = pages_of(held_tokens[r]), kept = pages_of(kept_tokens[r]);
+            int* row = p.table + static_cast<size_t>(r) * p.width;
+            for (int j = kept + lane; j < held; j += 32) {
+                const long long at = static_cast<long long>(free_before) + first_page[r] + held - 1 - j;
+                if (at >= 0 && at < p.pages) p.stack[at] = row[j];
+                row[j] = -1;
+            }
         }
     }
 
     // who is granted what he wants
-    sum = {0, 0};
+    before = exclusive_sums(wanted, warp_sums, total);
+    Pair got = {0, 0};
     for (int r = r0; r < r1; ++r) {
-        const int count = p.counts[r];
-        const long long after = static_cast<long long>(kept_tokens[r]) + count;
-        if (count > 0 && after <= capacity) {
-            sum.a += count;
-            sum.b += pages_of(after) - pages_of(kept_tokens[r]);
-        }
-    }
-    before = exclusive_sums(sum, warp_sums, total);
-    sum = {0, 0};
-    for (int r = r0; r < r1; ++r) {
-        const int count = p.counts[r];
-        const long long after = static_cast<long long>(kept_tokens[r]) + count;
-        offset[r] = 0;
-        if (count > 0 && after <= capacity) {
-            const int need = pages_of(after) - pages_of(kept_tokens[r]);
+        const int count = offset[r];
+        if (count > 0) {
+            const int need = pages_of(static_cast<long long>(kept_tokens[r]) + count) - pages_of(kept_tokens[r]);
             before.a += count;
             before.b += need;
             if (before.a <= p.max_tokens && (need == 0 || before.b <= available)) {
-                offset[r] = count;
-                sum.a += count;
-                sum.b += need;
+                got.a += count;
+                got.b += need;
+            } else {
+                offset[r] = 0;
             }
         }
     }
-    before = exclusive_sums(sum, warp_sums, total);
+    before = exclusive_sums(got, warp_sums, total);
     for (int r = r0; r < r1; ++r) {
         const int count = offset[r];
         offset[r] = static_cast<int>(before.a);
@@ -139,29 +155,32 @@ __global__ void __launch_bounds__(kReserveThreads) reserve_kernel(const ReserveA
         before.b += pages_of(static_cast<long long>(kept_tokens[r]) + count) - pages_of(kept_tokens[r]);
     }
     if (tid == 0) offset[R] = static_cast<int>(total.a);
-    __syncthreads();  // the pages given back are on the stack, too
-    for (int r = warp; r < R; r += kReserveThreads / 32) {
-        const int kept = pages_of(kept_tokens[r]);
-        const int last = pages_of(static_cast<long long>(kept_tokens[r]) + offset[r + 1] - offset[r]);
-        int* row = p.table + static_cast<size_t>(r) * p.width;
-        for (int j = kept + lane; j < last; j += 32) {
-            const long long at = available - 1 - (first_page[r] + j - kept);
-            row[j] = at >= 0 && at < p.pages ? p.stack[at] : -1;
+    cluster_barrier();  // lengths, counts and the free count have been read; the pages given back are on the stack
+    if (total.b > 0) {
+        for (int r = warp; r < R; r += warps) {
+            const int kept = pages_of(kept_tokens[r]);
+            const int last = pages_of(static_cast<long long>(kept_tokens[r]) + offset[r + 1] - offset[r]);
+            int* row = p.table + static_cast<size_t>(r) * p.width;
+            for (int j = kept + lane; j < last; j += 32) {
+                const long long at = available - 1 - (first_page[r] + j - kept);
+                row[j] = at >= 0 && at < p.pages ? __ldcg(p.stack + at) : -1;
+            }
         }
     }
-    __syncthreads();
-    for (int r = tid; r < R; r += kReserveThreads) {
-        const int got = offset[r + 1] - offset[r];
-        const int count = p.counts[r];
-        p.granted[r] = count < 0 ? kept_tokens[r] - held_tokens(r) : got;
-        p.lengths[r] = kept_tokens[r] + got;
-        p.offsets[r] = offset[r];
+    if (rank == 0) {
+        for (int r = tid; r < R; r += kReserveThreads) {
+            const int count = offset[r + 1] - offset[r];
+            p.granted[r] = count > 0 ? count : kept_tokens[r] - held_tokens[r];
+            p.lengths[r] = kept_tokens[r] + count;
+            p.offsets[r] = offset[r];
+        }
+        if (tid == 0) {
+            p.offsets[R] = offset[R];
+            *p.free_count = static_cast<int>(available - total.b);
+        }
     }
-    if (tid == 0) {
-        p.offsets[R] = offset[R];
-        *p.free_count = static_cast<int>(available - total.b);
-    }
-    for (int t = tid; t < p.max_tokens; t += kReserveThreads) {
+    if (total.b > 0) cluster_barrier();  // the table is complete
+    for (int t = rank * kReserveThreads + tid; t < p.max_tokens; t += gridDim.x * kReserveThreads) {
         long long slot = -1, position = 0;
         int r = -1;
         if (t < offset[R]) {
@@ -176,7 +195,7 @@ __global__ void __launch_bounds__(kReserveThreads) reserve_kernel(const ReserveA
             r = low;
             const int at = kept_tokens[r] + t - offset[r];
             position = at;
-            const int entry = p.table[static_cast<size_t>(r) * p.width + (at >> p.page_shift)];
+            const int entry = __ldcg(p.table + static_cast<size_t>(r) * p.width + (at >> p.page_shift));
             if (entry >= 0 && entry < p.pages)
                 slot = (static_cast<long long>(entry) << p.page_shift) + (at & (page - 1));
         }
@@ -201,6 +220,7 @@ struct AppendArgs {
 };
 
 __global__ void __launch_bounds__(256) append_kernel(const AppendArgs p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const long long per_token = static_cast<long long>(p.kv_heads) * p.vectors;
     const long long all = per_token * p.tokens;
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
@@ -401,14 +421,11 @@ int mb_paged_reserve(const mb_paged_reserve_args* a, void* stream) {
     p.granted = reinterpret_cast<int*>(a->granted);
     p.slots = reinterpret_cast<long long*>(a->slots);
     p.positions = reinterpret_cast<long long*>(a->positions);
-    const int smem = (3 * a->requests + 1) * 4;
-    if (smem > 48 * 1024) {
-        const cudaError_t err =
-            cudaFuncSetAttribute(reserve_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (err != cudaSuccess) return mb::cuda_error(err, "mb_paged_reserve");
-    }
-    reserve_kernel<<<1, kReserveThreads, smem, static_cast<cudaStream_t>(stream)>>>(p);
-    const cudaError_t err = cudaGetLastError();
+    static_assert((4 * kMaxRows + 1) * 4 <= 47 * 1024, "the rows fit without asking for more shared memory");
+    const bool large = a->max_tokens > 1024 || a->requests > 64;
+    const int cluster = large ? kReserveCluster : 1;
+    const cudaError_t err = launch_early(reserve_kernel, dim3(cluster), kReserveThreads, (4 * a->requests + 1) * 4, cluster,
+                                         static_cast<cudaStream_t>(stream), p);
     return err == cudaSuccess ? MB_OK : mb::cuda_error(err, "mb_paged_reserve");
 }
 
@@ -439,9 +456,8 @@ int mb_paged_append(const mb_paged_append_args* a, void* stream) {
     p.value_pages = reinterpret_cast<unsigned short*>(a->value_pages);
     p.slots = reinterpret_cast<const long long*>(a->slots);
     const long long blocks = (static_cast<long long>(a->tokens) * a->kv_heads * p.vectors + 255) / 256;
-    append_kernel<<<static_cast<int>(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-        p);
-    const cudaError_t err = cudaGetLastError();
+    const cudaError_t err = launch_early(append_kernel, dim3(static_cast<int>(blocks < 148 * 8 ? blocks : 148 * 8)), 256, 0, 1,
+                                         static_cast<cudaStream_t>(stream), p);
     return err == cudaSuccess ? MB_OK : mb::cuda_error(err, "mb_paged_append");
 }
 

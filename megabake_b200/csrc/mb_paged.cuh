@@ -58,6 +58,28 @@ __device__ __forceinline__ void store_output(unsigned short* to, float4 sum, flo
     *reinterpret_cast<uint2*>(to) = packed;
 }
 
+// A launch that may begin while the kernel before it in the stream ends: every kernel here waits (griddepcontrol.wait)
+// before it touches global memory, and then that kernel is complete.
+template <typename... Params, typename... Args>
+cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream,
+                         const Args&... args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = cluster;
+    attributes[1].val.clusterDim.y = 1;
+    attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
 // mb_paged_decode.cu
 int decode_admitted(const AttentionArgs& a);
 int64_t decode_workspace(const AttentionArgs& a);

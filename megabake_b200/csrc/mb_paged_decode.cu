@@ -28,6 +28,8 @@ constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kMaxStages = 16;
 constexpr int kSmemLimit = 227 * 1024;
 constexpr int kConsumerBarrier = 1;
+constexpr int kLeastBlocks = 2;     // of a run
+constexpr int kWholeBlocks = 8;     // rows of the table that hold no more are not cut
 
 // What a CTA leaves behind about the unit that it began and others finish.
 struct Split {
@@ -84,6 +86,13 @@ __device__ __forceinline__ Piece piece_at(const Deal& d, long long at, long long
     p.begin = static_cast<int>(rest - static_cast<long long>(p.unit) * p.blocks);
     p.end = static_cast<int>(min(static_cast<long long>(p.blocks), p.begin + (run_end - at)));
     return p;
+}
+
+// The first end or begin of a unit from `at` on.
+__device__ __forceinline__ long long unit_boundary(const Deal& d, long long at) {
+    if (at >= d.total) return at;
+    const Piece p = piece_at(d, at, d.total);
+    return p.begin == 0 ? at : at + p.blocks - p.begin;
 }
 
 __device__ __forceinline__ unsigned int movmatrix(unsigned int v) {
@@ -224,9 +233,13 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
     deal.tokens = p.a.tokens;
     deal.units = p.a.kv_heads * p.subgroups;
     deal.total = static_cast<long long>(first_block[p.a.tokens]) * deal.units;
-    deal.per = max((deal.total + gridDim.x - 1) / gridDim.x, 2ll);
-    const long long run_begin = min(blockIdx.x * deal.per, deal.total);
-    const long long run_end = min(run_begin + deal.per, deal.total);
+    deal.per = max((deal.total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kLeastBlocks));
+    long long run_begin = min(blockIdx.x * deal.per, deal.total);
+    long long run_end = min(run_begin + deal.per, deal.total);
+    if (p.splits == nullptr) {   // no unit is cut: runs go from unit to unit
+        run_begin = unit_boundary(deal, run_begin);
+        run_end = unit_boundary(deal, run_end);
+    }
 
     if (warp == kWarps) {
         // ---- copies
@@ -615,7 +628,7 @@ Shape shape_of(const AttentionArgs& a, int sms) {
     const int blocks = ((a.width << a.page_shift) + kBlock - 1) / kBlock;   // of a full row
     const long long most = static_cast<long long>(a.tokens) * a.kv_heads * s.subgroups * blocks;
     s.ctas = static_cast<int>(most < sms ? most : sms);
-    s.joined = blocks > 1;   // one block is never cut
+    s.joined = blocks > kWholeBlocks;
     const int tile = 2 * kBlock * a.head_dim * 2;
     const int rest = kWarps * s.rows * (a.head_dim + 4) * 4 + static_cast<int>(sizeof(Control4)) + (3 * a.tokens + 1) * 4;
     s.stages = (kSmemLimit - rest) / tile;
@@ -631,16 +644,8 @@ Shape shape_of(const AttentionArgs& a, int sms) {
 template <typename T, int D>
 cudaError_t launch_join(const DecodeArgs& args, const Shape& s, cudaStream_t stream) {
     const int group = args.a.heads / args.a.kv_heads;
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(s.ctas, group < s.rows ? group : s.rows);
-    config.blockDim = dim3(kJoinThreads);
-    config.stream = stream;
-    cudaLaunchAttribute early;
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &early;
-    config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, join_kernel<T, D>, args, s.rows);
+    return launch_early(join_kernel<T, D>, dim3(s.ctas, group < s.rows ? group : s.rows), kJoinThreads, 0, 1, stream, args,
+                        s.rows);
 }
 
 template <typename T, int D, int N>
@@ -653,17 +658,8 @@ cudaError_t launch_decode(const CUtensorMap& keys, const CUtensorMap& values, co
         if (err != cudaSuccess) return err;
         if (device < 64) configured.fetch_or(1ull << device, std::memory_order_relaxed);
     }
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(s.ctas);
-    config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = s.smem;
-    config.stream = stream;
-    cudaLaunchAttribute early;
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &early;
-    config.numAttrs = 1;
-    cudaError_t err = cudaLaunchKernelEx(&config, decode_attention_kernel<T, D, N>, keys, values, args);
+    cudaError_t err = launch_early(decode_attention_kernel<T, D, N>, dim3(s.ctas), kThreads, s.smem, 1, stream, keys, values,
+                                   args);
     if (err == cudaSuccess && s.joined) err = launch_join<T, D>(args, s, stream);
     return err;
 }

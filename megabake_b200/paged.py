@@ -24,7 +24,7 @@ per-request state is a step of its roadmap (``docs/roadmap.md:178``).
 
 from __future__ import annotations
 
-import ctypes
+import struct
 from typing import NamedTuple
 
 import torch
@@ -38,7 +38,6 @@ __all__ = ["PagedBatch", "PagedState", "paged_append", "paged_kv_attention", "pa
 _ELEMENTS = {torch.bfloat16: 0, torch.float16: 1}
 _HEAD_DIMS = (64, 128, 256)
 _MAX_REQUESTS = 2048
-_ready: set[int] = set()   # devices that are known to be sm_100
 
 
 class PagedBatch(NamedTuple):
@@ -99,48 +98,68 @@ def _page_size_covered(page_size: int) -> bool:
     return 8 <= page_size <= 1024 and page_size & (page_size - 1) == 0
 
 
-def _device_ready(device: torch.device) -> int:
-    index = device.index
-    if index not in _ready:
-        from .engine import _require_native_device
+# ---------------------------------------------------------------------------------------
+# What a call costs the host decides what a small one takes.  All that follows from the tensors' types, shapes, strides
+# and devices -- whether they fit, the fields of the native arguments, the size of the scratch -- is worked out once for
+# every combination of them and found again under it; what is left for a call are addresses.  (One
+# token of one request, 9/3 heads of 64: 27.8 -> {DECODE_HOST} us a call; 32 requests reserved: 19.6 -> {RESERVE_HOST}.)
+# ---------------------------------------------------------------------------------------
+_known: dict[tuple, tuple] = {}
+_MAX_KNOWN = 1024
+_raw_stream = torch._C._cuda_getCurrentRawStream   # torch.cuda.current_stream(index).cuda_stream without its object
 
-        _require_native_device(device)
-        _ready.add(index)
-    return index
+
+def _remember(signature: tuple, found: tuple) -> tuple:
+    if len(_known) >= _MAX_KNOWN:   # a program whose shapes never come back
+        _known.clear()
+    _known[signature] = found
+    return found
 
 
-def _whole(name: str, tensor: torch.Tensor, dtype: torch.dtype, numel: int, device: torch.device) -> int:
-    """Address of a contiguous tensor of whole numbers."""
+def _optional(tensor: torch.Tensor | None):
+    return None if tensor is None else (tensor.dtype, tensor.get_device(), tensor.shape, tensor.stride())
+
+
+def _native_device(device: torch.device) -> int:
+    from .engine import _require_native_device
+
+    _require_native_device(device)
+    return device.index
+
+
+def _whole(name: str, tensor: torch.Tensor, dtype: torch.dtype, numel: int, device: torch.device) -> None:
+    """A contiguous tensor of whole numbers."""
     if tensor.dtype != dtype or tensor.device != device or tensor.numel() != numel or not tensor.is_contiguous():
         fail("input-binding", f"{name} must be a contiguous {dtype} tensor of {numel} on {device}, got "
                               f"{tensor.dtype} {tuple(tensor.shape)} on {tensor.device}")
-    return tensor.data_ptr()
 
 
 def _rows(name: str, tensor: torch.Tensor, shape: tuple, like: torch.Tensor) -> tuple:
-    """Address and strides of ``[..., head_dim]`` values that are read 16 bytes at a time."""
+    """Strides of ``[..., head_dim]`` values that are read 16 bytes at a time."""
     if tensor.dtype != like.dtype or tensor.device != like.device or tensor.shape != shape:
         fail("input-binding", f"{name} must be {like.dtype} {tuple(shape)} on {like.device}, got {tensor.dtype} "
                               f"{tuple(tensor.shape)} on {tensor.device}")
-    return _strided(name, tensor)
+    strides = tensor.stride()
+    if strides[-1] != 1 or any(stride % 8 for stride in strides[:-1]):
+        _misaligned(name)
+    return strides[:-1]
 
 
-def _strided(name: str, tensor: torch.Tensor) -> tuple:
-    pointer, strides = tensor.data_ptr(), tensor.stride()
-    bits = pointer >> 1
-    for stride in strides[:-1]:
-        bits |= stride
-    if bits & 7 or pointer & 1 or strides[-1] != 1:
-        fail("input-binding", f"{name} must have a contiguous last dimension and start, in every dimension, on "
-                              "16-byte boundaries")
-    return (pointer, *strides[:-1])
+def _misaligned(name: str) -> None:
+    fail("input-binding", f"{name} must have a contiguous last dimension and start, in every dimension, on 16-byte "
+                          "boundaries")
+
+
+def _check_aligned(**addresses: int) -> None:
+    for name, address in addresses.items():
+        if address & 15:
+            _misaligned(name)
 
 
 def _inference_only(*tensors) -> None:
-    if torch.is_grad_enabled():
-        for tensor in tensors:
-            if tensor is not None and tensor.requires_grad:
-                raise RuntimeError("MegaBake supports inference only")
+    for tensor in tensors:
+        if tensor is not None and tensor.requires_grad:
+            raise RuntimeError("MegaBake supports inference only")
 
 
 def _pools(key_pages: torch.Tensor, value_pages: torch.Tensor) -> tuple:
@@ -149,19 +168,19 @@ def _pools(key_pages: torch.Tensor, value_pages: torch.Tensor) -> tuple:
         fail("input-binding", "key_pages must be bf16 or fp16 [pages, page_size, kv_heads, head_dim] with head_dim 64, "
                               "128 or 256 and page_size a power of two from 8 to 1024, got "
                               f"{key_pages.dtype} {tuple(key_pages.shape)}")
-    return _strided("key_pages", key_pages), _rows("value_pages", value_pages, key_pages.shape, key_pages)
+    return (_rows("key_pages", key_pages, key_pages.shape, key_pages),
+            _rows("value_pages", value_pages, key_pages.shape, key_pages))
 
 
-def _call(function, args, index: int, what: str) -> None:
-    lib = rt.load_library()
-    stream = torch.cuda.current_stream(index).cuda_stream
+def _call(function, args: bytes, index: int, what: str) -> None:
+    stream = _raw_stream(index)
     if index == torch.cuda.current_device():
-        code = function(ctypes.byref(args), stream)
+        code = function(args, stream)
     else:
         with torch.cuda.device(index):
-            code = function(ctypes.byref(args), stream)
+            code = function(args, stream)
     if code:
-        rt._check(lib, code, "runtime", what)
+        rt._check(rt.load_library(), code, "runtime", what)
 
 
 def paged_reserve(counts: torch.Tensor, lengths: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
@@ -176,6 +195,27 @@ def paged_reserve(counts: torch.Tensor, lengths: torch.Tensor, block_table: torc
 
     ``lengths``, ``block_table``, ``free_pages`` and ``free_count`` are updated.  ``max_tokens`` fixes the shapes of the
     result, so that a captured step can be replayed with other counts."""
+    page_size, max_tokens = int(page_size), int(max_tokens)
+    signature = (counts.dtype, counts.get_device(), counts.shape, counts.stride(), lengths.dtype, lengths.get_device(),
+                 lengths.shape, lengths.stride(), block_table.dtype, block_table.get_device(), block_table.shape,
+                 block_table.stride(), free_pages.dtype, free_pages.get_device(), free_pages.shape, free_pages.stride(),
+                 free_count.dtype, free_count.get_device(), free_count.shape, page_size, max_tokens)
+    fields, index = _known.get(signature) or _remember(signature, _reserve_fields(
+        counts, lengths, block_table, free_pages, free_count, page_size, max_tokens))
+    slots = torch.empty(max_tokens, dtype=torch.int64, device=counts.device)
+    batch = PagedBatch(counts.new_empty(counts.shape[0] + 1), slots, torch.empty_like(slots),
+                       counts.new_empty(max_tokens), torch.empty_like(counts))
+    args = fields + _RESERVE_ADDRESSES.pack(
+        counts.data_ptr(), lengths.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
+        batch[0].data_ptr(), slots.data_ptr(), batch[2].data_ptr(), batch[3].data_ptr(), batch[4].data_ptr())
+    _call(rt.load_library().mb_paged_reserve, args, index, "mb_paged_reserve")
+    return batch
+
+
+_RESERVE_ADDRESSES = struct.Struct("=10Q")
+
+
+def _reserve_fields(counts, lengths, block_table, free_pages, free_count, page_size, max_tokens) -> tuple:
     if block_table.dim() != 2:
         fail("input-binding", f"block_table must be [requests, width], got {tuple(block_table.shape)}")
     device = counts.device
@@ -185,22 +225,12 @@ def paged_reserve(counts: torch.Tensor, lengths: torch.Tensor, block_table: torc
         fail("input-binding", f"paged_reserve needs 1..{_MAX_REQUESTS} requests on a CUDA device, pages of 8 to 1024 tokens "
                               "(a power of two), rows below 2**31 tokens and max_tokens >= 0, got "
                               f"{tuple(block_table.shape)} pages of {page_size} on {device}, max_tokens {max_tokens}")
-    index = _device_ready(device)
-    int32 = torch.int32
-    args = rt.PagedReserveArgs(
-        requests, width, free_pages.numel(), page_size, max_tokens, 0,
-        _whole("counts", counts, int32, requests, device), _whole("lengths", lengths, int32, requests, device),
-        _whole("block_table", block_table, int32, requests * width, device),
-        _whole("free_pages", free_pages, int32, free_pages.numel(), device),
-        _whole("free_count", free_count, int32, 1, device))
-    batch = PagedBatch(torch.empty(requests + 1, dtype=int32, device=device),
-                       torch.empty(max_tokens, dtype=torch.int64, device=device),
-                       torch.empty(max_tokens, dtype=torch.int64, device=device),
-                       torch.empty(max_tokens, dtype=int32, device=device),
-                       torch.empty(requests, dtype=int32, device=device))
-    args.offsets, args.slots, args.positions, args.rows, args.granted = (t.data_ptr() for t in batch)
-    _call(rt.load_library().mb_paged_reserve, args, index, "mb_paged_reserve")
-    return batch
+    for name, tensor, numel in (("counts", counts, requests), ("lengths", lengths, requests),
+                                ("block_table", block_table, requests * width),
+                                ("free_pages", free_pages, free_pages.numel()), ("free_count", free_count, 1)):
+        _whole(name, tensor, torch.int32, numel, device)
+    args = rt.PagedReserveArgs(requests, width, free_pages.numel(), page_size, max_tokens)
+    return bytes(args)[:rt.PagedReserveArgs.counts.offset], _native_device(device)
 
 
 def paged_append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
@@ -208,26 +238,75 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor
     """Write ``key`` and ``value`` (``[tokens, kv_heads, head_dim]``) into the slots (int64 ``[tokens]``) of the pools.
     A slot outside the pool, as -1 behind the last token, is skipped; slots of one call are distinct (of two tokens
     with one slot either may be the one that stays)."""
+    if torch.is_grad_enabled():
+        _inference_only(key, value, key_pages, value_pages)
+    signature = (key.dtype, key.get_device(), key.shape, key.stride(), value.dtype, value.get_device(), value.shape,
+                 value.stride(), key_pages.dtype, key_pages.get_device(), key_pages.shape, key_pages.stride(),
+                 value_pages.dtype, value_pages.get_device(), value_pages.shape, value_pages.stride(), slots.dtype,
+                 slots.get_device(), slots.shape, slots.stride())
+    fields, index = _known.get(signature) or _remember(signature, _append_fields(key, value, key_pages, value_pages, slots))
+    if key.shape[0] == 0:
+        return
+    addresses = (key.data_ptr(), value.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr())
+    if (addresses[0] | addresses[1] | addresses[2] | addresses[3]) & 15:
+        _check_aligned(key=addresses[0], value=addresses[1], key_pages=addresses[2], value_pages=addresses[3])
+    _call(rt.load_library().mb_paged_append, fields + _APPEND_ADDRESSES.pack(*addresses, slots.data_ptr()), index,
+          "mb_paged_append")
+
+
+_APPEND_ADDRESSES = struct.Struct("=5Q")
+
+
+def _append_fields(key, value, key_pages, value_pages, slots) -> tuple:
     kpool, vpool = _pools(key_pages, value_pages)
     pages, page_size, kv_heads, head_dim = key_pages.shape
     if key.dim() != 3 or key.device.type != "cuda":
         fail("input-binding", f"key must be [tokens, kv_heads, head_dim] on a CUDA device, got {tuple(key.shape)} on "
                               f"{key.device}")
     tokens = key.shape[0]
-    _inference_only(key, value, key_pages, value_pages)
     k = _rows("key", key, (tokens, kv_heads, head_dim), key_pages)
     v = _rows("value", value, (tokens, kv_heads, head_dim), key_pages)
-    at = _whole("slots", slots, torch.int64, tokens, key.device)
-    index = _device_ready(key.device)
-    if tokens == 0:
-        return
-    args = rt.PagedAppendArgs(tokens, kv_heads, head_dim, pages, page_size, 0, k[1], k[2], v[1], v[2], *kpool[1:],
-                              *vpool[1:], k[0], v[0], kpool[0], vpool[0], at)
-    _call(rt.load_library().mb_paged_append, args, index, "mb_paged_append")
+    _whole("slots", slots, torch.int64, tokens, key.device)
+    args = rt.PagedAppendArgs(tokens, kv_heads, head_dim, pages, page_size, 0, *k, *v, *kpool, *vpool)
+    return bytes(args)[:rt.PagedAppendArgs.key.offset], _native_device(key.device)
 
 
-def _attention(what, function, workspace_of, query, key, value, key_pages, value_pages, block_table, lengths, index,
-               index_name, index_numel, scale, out, status):
+_ATTENTION_ADDRESSES = struct.Struct("=11Q")
+
+
+def _attention(what, query, key, value, key_pages, value_pages, block_table, lengths, index, scale, out, status):
+    if torch.is_grad_enabled():
+        _inference_only(query, key, value, key_pages, value_pages)
+    if scale is not None:
+        scale = float(scale)
+    signature = (what, query.dtype, query.get_device(), query.shape, query.stride(), key_pages.dtype,
+                 key_pages.get_device(), key_pages.shape, key_pages.stride(), value_pages.dtype, value_pages.get_device(),
+                 value_pages.shape, value_pages.stride(), block_table.dtype, block_table.get_device(), block_table.shape,
+                 block_table.stride(), lengths.dtype, lengths.get_device(), lengths.shape, lengths.stride(), scale,
+                 _optional(key), _optional(value), _optional(index), _optional(out), _optional(status))
+    fields, workspace_bytes, device_index = _known.get(signature) or _remember(
+        signature, _attention_fields(what, query, key, value, key_pages, value_pages, block_table, lengths, index, scale,
+                                     out, status))
+    if out is None:
+        out = query.new_empty(query.shape)
+    if query.shape[0] == 0:
+        return out
+    q, kpool, vpool, to = query.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), out.data_ptr()
+    k, v = (0, 0) if key is None else (key.data_ptr(), value.data_ptr())
+    if (q | k | v | kpool | vpool | to) & 15:
+        _check_aligned(query=q, key=k, value=v, key_pages=kpool, value_pages=vpool, out=to)
+    workspace = query.new_empty(workspace_bytes, dtype=torch.uint8) if workspace_bytes else None
+    args = fields + _ATTENTION_ADDRESSES.pack(
+        q, k, v, kpool, vpool, block_table.data_ptr(), lengths.data_ptr(), 0 if index is None else index.data_ptr(), to,
+        0 if workspace is None else workspace.data_ptr(), 0 if status is None else status.data_ptr())
+    _call(getattr(rt.load_library(), what), args, device_index, what)
+    return out
+
+
+def _attention_fields(what, query, key, value, key_pages, value_pages, block_table, lengths, index, scale, out,
+                      status) -> tuple:
+    prefill = what == "mb_paged_prefill"
+    index_name = "offsets" if prefill else "rows"
     kpool, vpool = _pools(key_pages, value_pages)
     pages, page_size, kv_heads, head_dim = key_pages.shape
     device = query.device
@@ -235,48 +314,48 @@ def _attention(what, function, workspace_of, query, key, value, key_pages, value
             device.type != "cuda":
         fail("input-binding", f"query must be [tokens, heads, {head_dim}] on a CUDA device with heads a multiple of "
                               f"{kv_heads}, got {tuple(query.shape)} on {device}")
+    tokens, heads = query.shape[0], query.shape[1]
     if block_table.dim() != 2 or min(block_table.shape) < 1 or block_table.shape[1] * page_size > 0x7fffffff:
         fail("input-binding", f"block_table must be [requests, width] with rows below 2**31 tokens, got "
                               f"{tuple(block_table.shape)} pages of {page_size}")
-    _inference_only(query, key, value, key_pages, value_pages)
-    tokens, heads = query.shape[0], query.shape[1]
     requests, width = block_table.shape
-    if index is None and requests != tokens:
+    if requests > _MAX_REQUESTS or (not prefill and tokens > _MAX_REQUESTS):
+        fail("input-binding", f"a call takes at most {_MAX_REQUESTS} requests, got {max(requests, tokens)}")
+    if index is None and (prefill or requests != tokens):
         fail("input-binding", f"{tokens} queries need a row of the table each, or {index_name}; the table has {requests}")
     q = _rows("query", query, query.shape, key_pages)
-    k = v = (0, 0, 0)
+    k = v = (0, 0)
     if key is not None or value is not None:
         if key is None or value is None:
             fail("input-binding", "key and value come together")
         k = _rows("key", key, (tokens, kv_heads, head_dim), key_pages)
         v = _rows("value", value, (tokens, kv_heads, head_dim), key_pages)
-    int32 = torch.int32
-    table = _whole("block_table", block_table, int32, requests * width, device)
-    held = _whole("lengths", lengths, int32, requests, device)
-    at = 0 if index is None else _whole(index_name, index, int32, index_numel, device)
-    zero_rest = out is None
-    if out is None:
-        out = torch.empty((tokens, heads, head_dim), dtype=query.dtype, device=device)
-    elif out.dtype != query.dtype or out.shape != query.shape or out.device != device or not out.is_contiguous() or \
-            out.data_ptr() % 16:
-        fail("input-binding", f"out must be a contiguous {query.dtype} {tuple(query.shape)} tensor on {device} that "
-                              "starts on a 16-byte boundary")
-    device_index = _device_ready(device)
-    if tokens == 0:
-        return out
-    args = rt.PagedAttentionArgs(
-        _ELEMENTS[query.dtype], tokens, requests, heads, kv_heads, head_dim, width, pages, page_size, zero_rest,
-        head_dim ** -0.5 if scale is None else scale, 0, q[1], q[2], k[1], k[2], v[1], v[2], *kpool[1:], *vpool[1:],
-        q[0], k[0], v[0], kpool[0], vpool[0], table, held, at, out.data_ptr(), 0,
-        0 if status is None else _whole("status", status, int32, 1, device))
-    need = workspace_of(ctypes.byref(args))
-    if need < 0:
-        rt._check(rt.load_library(), -need, "resource-admission", what)
-    if need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-        args.workspace = workspace.data_ptr()
-    _call(function, args, device_index, what)
-    return out
+    _whole("block_table", block_table, torch.int32, requests * width, device)
+    _whole("lengths", lengths, torch.int32, requests, device)
+    if index is not None:
+        _whole(index_name, index, torch.int32, requests + 1 if prefill else tokens, device)
+    if out is not None and (out.dtype != query.dtype or out.shape != query.shape or out.device != device or
+                            not out.is_contiguous()):
+        fail("input-binding", f"out must be a contiguous {query.dtype} {tuple(query.shape)} tensor on {device}")
+    if status is not None:
+        _whole("status", status, torch.int32, 1, device)
+    device_index = _native_device(device)
+    args = rt.PagedAttentionArgs(_ELEMENTS[query.dtype], tokens, requests, heads, kv_heads, head_dim, width, pages, page_size,
+                                 out is None, head_dim ** -0.5 if scale is None else scale, 0, *q, *k, *v, *kpool, *vpool)
+    workspace_bytes = 0
+    if tokens:
+        # the size does not depend on addresses: any that are aligned as they have to be
+        for name in ("query", "key_pages", "value_pages", "block_table", "lengths", "out"):
+            setattr(args, name, 4096)
+        args.key = args.value = 4096 if key is not None else 0
+        args.index = 4096 if index is not None else 0
+        lib = rt.load_library()
+        with torch.cuda.device(device_index):
+            workspace_bytes = getattr(lib, what + "_workspace")(bytes(args))
+        if workspace_bytes < 0:
+            rt._check(lib, -workspace_bytes, "resource-admission", what)
+    fields = bytes(args)[:rt.PagedAttentionArgs.query.offset]
+    return fields, workspace_bytes, device_index
 
 
 def paged_kv_attention(query: torch.Tensor, key: torch.Tensor | None, value: torch.Tensor | None,
@@ -293,9 +372,8 @@ def paged_kv_attention(query: torch.Tensor, key: torch.Tensor | None, value: tor
     (``paged_reserve`` does), and ``rows`` names no request twice.  Without them several queries may read one
     request.  ``scale`` defaults to ``head_dim ** -0.5``.  ``status`` (int32 ``[1]``) receives a status code if a wait
     inside the kernel ran out."""
-    lib = rt.load_library()
-    return _attention("mb_paged_attention", lib.mb_paged_attention, lib.mb_paged_attention_workspace, query, key, value,
-                      key_pages, value_pages, block_table, lengths, rows, "rows", query.shape[0], scale, out, status)
+    return _attention("mb_paged_attention", query, key, value, key_pages, value_pages, block_table, lengths, rows, scale,
+                      out, status)
 
 
 def paged_prefill_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
@@ -310,7 +388,5 @@ def paged_prefill_attention(query: torch.Tensor, key_pages: torch.Tensor, value_
     keys ``0 .. p`` that lie on pages of the pool: whole prompts, or a chunk after what is cached.  Queries behind
     the last request are zero in a new output; rows of an ``out`` that is given stay as they were there.  ``scale`` and
     ``status`` as for ``paged_kv_attention``."""
-    lib = rt.load_library()
-    return _attention("mb_paged_prefill", lib.mb_paged_prefill, lib.mb_paged_prefill_workspace, query, None, None,
-                      key_pages, value_pages, block_table, lengths, offsets, "offsets", block_table.shape[0] + 1, scale,
+    return _attention("mb_paged_prefill", query, None, None, key_pages, value_pages, block_table, lengths, offsets, scale,
                       out, status)

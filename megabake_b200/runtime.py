@@ -269,13 +269,12 @@ def load_library(path: Path | None = None) -> ctypes.CDLL:
         lib.mb_attention_decode_static.restype = ctypes.c_int
         lib.mb_greedy_advance.argtypes = [ctypes.POINTER(GreedyArgs), ctypes.c_void_p]
         lib.mb_greedy_advance.restype = ctypes.c_int
-        for name, args in (("mb_paged_reserve", PagedReserveArgs), ("mb_paged_append", PagedAppendArgs),
-                           ("mb_paged_attention", PagedAttentionArgs),
-                           ("mb_paged_prefill", PagedAttentionArgs)):
-            getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+        # the arguments of these come as a structure or as its bytes
+        for name in ("mb_paged_reserve", "mb_paged_append", "mb_paged_attention", "mb_paged_prefill"):
+            getattr(lib, name).argtypes = [ctypes.c_void_p, ctypes.c_void_p]
             getattr(lib, name).restype = ctypes.c_int
         for name in ("mb_paged_attention_workspace", "mb_paged_prefill_workspace"):
-            getattr(lib, name).argtypes = [ctypes.POINTER(PagedAttentionArgs)]
+            getattr(lib, name).argtypes = [ctypes.c_void_p]
             getattr(lib, name).restype = ctypes.c_int64
         if lib.mb_abi_version() != MB_ABI_VERSION:
             raise _native_error(

@@ -82,6 +82,15 @@ def test_prefill_entry_needs_offsets_and_appended_keys():
     assert lib.mb_paged_prefill(ctypes.byref(_attention_args(key=0, value=0, index=0)), None) == INVALID
 
 
+def test_addresses_follow_the_fields():
+    from megabake_b200 import paged
+
+    for struct_type, first, addresses in ((rt.PagedReserveArgs, "counts", paged._RESERVE_ADDRESSES),
+                                          (rt.PagedAppendArgs, "key", paged._APPEND_ADDRESSES),
+                                          (rt.PagedAttentionArgs, "query", paged._ATTENTION_ADDRESSES)):
+        assert getattr(struct_type, first).offset + addresses.size == ctypes.sizeof(struct_type)
+
+
 def test_entries_refuse_null():
     lib = rt.load_library()
     for name in ("mb_paged_reserve", "mb_paged_append", "mb_paged_attention", "mb_paged_prefill"):
