@@ -477,7 +477,7 @@ typedef struct mb_paged_reserve_args {
     uint64_t free_pages;      /* int32 [pages], updated                                   */
     uint64_t free_count;      /* int32 [1], updated                                       */
     uint64_t offsets;         /* int32 [requests + 1], written                            */
-    uint64_t slots;           /* int64 [max_tokens], written                              */
+    uint64_t slots;           /* int64 [max_tokens], written; 16-byte aligned, as the next two */
     uint64_t positions;       /* int64 [max_tokens], written                              */
     uint64_t rows;            /* int32 [max_tokens], written                              */
     uint64_t granted;         /* int32 [requests], written                                */

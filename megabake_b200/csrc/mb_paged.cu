@@ -27,7 +27,7 @@ namespace paged {
 // tokens 20 bytes for each of their places.  A thread-block cluster shares the rows and places, and every block of it
 // works the sums out for itself: its barrier is all that tables which are read and updated in one launch need.
 // ---------------------------------------------------------------------------------------
-constexpr int kReserveThreads = 256;
+constexpr int kReserveThreads = 512;
 constexpr int kReserveCluster = 8;
 
 struct ReserveArgs {
@@ -180,28 +180,52 @@ __global__ void __launch_bounds__(kReserveThreads) reserve_kernel(const ReserveA
         }
     }
     if (total.b > 0) cluster_barrier();  // the table is complete
-    for (int t = rank * kReserveThreads + tid; t < p.max_tokens; t += gridDim.x * kReserveThreads) {
-        long long slot = -1, position = 0;
-        int r = -1;
-        if (t < offset[R]) {
-            int low = 0, high = R;  // offset[low] <= t < offset[high]
+    // four places a thread: one search, and as a rule one entry of the table
+    for (int t0 = 4 * (rank * kReserveThreads + tid); t0 < p.max_tokens; t0 += 4 * gridDim.x * kReserveThreads) {
+        long long slot[4] = {-1, -1, -1, -1}, position[4] = {0, 0, 0, 0};
+        int row[4] = {-1, -1, -1, -1};
+        if (t0 < offset[R]) {
+            int low = 0, high = R;  // offset[low] <= t0 < offset[high]
             while (high - low > 1) {
                 const int middle = (low + high) >> 1;
-                if (offset[middle] <= t)
+                if (offset[middle] <= t0)
                     low = middle;
                 else
                     high = middle;
             }
-            r = low;
-            const int at = kept_tokens[r] + t - offset[r];
-            position = at;
-            const int entry = __ldcg(p.table + static_cast<size_t>(r) * p.width + (at >> p.page_shift));
-            if (entry >= 0 && entry < p.pages)
-                slot = (static_cast<long long>(entry) << p.page_shift) + (at & (page - 1));
+            int loaded = -1, entry = -1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (t0 + i >= offset[R]) break;
+                while (offset[low + 1] <= t0 + i) {
+                    ++low;
+                    loaded = -1;
+                }
+                const int at = kept_tokens[low] + t0 + i - offset[low];
+                if (at >> p.page_shift != loaded) {
+                    loaded = at >> p.page_shift;
+                    entry = __ldcg(p.table + static_cast<size_t>(low) * p.width + loaded);
+                }
+                if (entry >= 0 && entry < p.pages)
+                    slot[i] = (static_cast<long long>(entry) << p.page_shift) + (at & (page - 1));
+                position[i] = at;
+                row[i] = low;
+            }
         }
-        p.slots[t] = slot;
-        p.positions[t] = position;
-        p.rows[t] = r;
+        if (t0 + 4 <= p.max_tokens) {
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                *reinterpret_cast<longlong2*>(p.slots + t0 + i) = make_longlong2(slot[i], slot[i + 1]);
+                *reinterpret_cast<longlong2*>(p.positions + t0 + i) = make_longlong2(position[i], position[i + 1]);
+            }
+            *reinterpret_cast<int4*>(p.rows + t0) = make_int4(row[0], row[1], row[2], row[3]);
+        } else {
+            for (int i = 0; t0 + i < p.max_tokens; ++i) {
+                p.slots[t0 + i] = slot[i];
+                p.positions[t0 + i] = position[i];
+                p.rows[t0 + i] = row[i];
+            }
+        }
     }
 }
 
@@ -235,89 +259,6 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs p) {
         *reinterpret_cast<uint4*>(p.value_pages + at * p.vpool.page + in_page * p.vpool.token + h * p.vpool.head + c) =
             v;
     }
-}
-
-// ---------------------------------------------------------------------------------------
-// Attention, a warp per query and head: keys one after the other, a running maximum and sum
-// ---------------------------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ float widen(T v);
-template <>
-__device__ __forceinline__ float widen(__nv_bfloat16 v) {
-    return __bfloat162float(v);
-}
-template <>
-__device__ __forceinline__ float widen(__half v) {
-    return __half2float(v);
-}
-template <typename T>
-__device__ __forceinline__ T narrow(float v);
-template <>
-__device__ __forceinline__ __nv_bfloat16 narrow(float v) {
-    return __float2bfloat16_rn(v);
-}
-template <>
-__device__ __forceinline__ __half narrow(float v) {
-    return __float2half_rn(v);
-}
-
-template <typename T, int D>
-__global__ void __launch_bounds__(128) attention_kernel(const AttentionArgs p) {
-    constexpr int kLane = D / 32;
-    const int t = blockIdx.x, lane = threadIdx.x & 31;
-    int r = -1, keys = 0;
-    int low = 0, high = p.requests;
-    while (high - low > 1) {
-        const int middle = (low + high) >> 1;
-        if (p.index[middle] <= t)
-            low = middle;
-        else
-            high = middle;
-    }
-    const int first = p.index[low], end = p.index[low + 1];
-    if (t >= first && t < end) {
-        r = low;
-        keys = min(p.lengths[r], p.width << p.page_shift) - (end - 1 - t);
-    } else if (!p.zero_rest) {
-        return;
-    }
-    const T* pools[2] = {reinterpret_cast<const T*>(p.key_pages), reinterpret_cast<const T*>(p.value_pages)};
-    for (int h = threadIdx.x >> 5; h < p.heads; h += 4) {
-        const int kvh = h / (p.heads / p.kv_heads);
-        float q[kLane], o[kLane], m = -INFINITY, l = 0.f;
-        for (int i = 0; i < kLane; ++i) {
-            q[i] = widen(reinterpret_cast<const T*>(p.query)[t * p.q.token + h * p.q.head + lane * kLane + i]) * p.scale;
-            o[i] = 0.f;
-        }
-        for (int j = 0; j < keys; ++j) {
-            const int entry = p.table[static_cast<size_t>(r) * p.width + (j >> p.page_shift)];
-            if (entry < 0 || entry >= p.pages) continue;
-            const long long in_page = j & ((1 << p.page_shift) - 1);
-            const T* k = pools[0] + entry * p.kpool.page + in_page * p.kpool.token + kvh * p.kpool.head + lane * kLane;
-            const T* v = pools[1] + entry * p.vpool.page + in_page * p.vpool.token + kvh * p.vpool.head + lane * kLane;
-            float s = 0.f;
-            for (int i = 0; i < kLane; ++i) s = fmaf(q[i], widen(k[i]), s);
-            for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-            const float highest = fmaxf(m, s), base = highest == -INFINITY ? 0.f : highest;
-            const float before = __expf(m - base), weight = exp2f((s - base) * kLog2e + kWeightShift<T>);
-            l = l * before + weight;
-            for (int i = 0; i < kLane; ++i) o[i] = fmaf(weight, widen(v[i]), o[i] * before);
-            m = highest;
-        }
-        T* out = reinterpret_cast<T*>(p.out) + (static_cast<size_t>(t) * p.heads + h) * D + lane * kLane;
-        for (int i = 0; i < kLane; ++i) out[i] = narrow<T>(l == 0.f ? 0.f : o[i] / l);
-    }
-}
-
-template <typename T>
-cudaError_t launch_attention(const AttentionArgs& p, cudaStream_t stream) {
-    if (p.head_dim == 64)
-        attention_kernel<T, 64><<<p.tokens, 128, 0, stream>>>(p);
-    else if (p.head_dim == 128)
-        attention_kernel<T, 128><<<p.tokens, 128, 0, stream>>>(p);
-    else
-        attention_kernel<T, 256><<<p.tokens, 128, 0, stream>>>(p);
-    return cudaGetLastError();
 }
 
 // ---------------------------------------------------------------------------------------
@@ -385,7 +326,7 @@ int attention_args(const mb_paged_attention_args* a, bool prefill, AttentionArgs
     p.index = reinterpret_cast<const int*>(a->index);
     p.out = reinterpret_cast<unsigned short*>(a->out);
     p.status = reinterpret_cast<int*>(a->status);
-    return prefill ? MB_OK : decode_admitted(p);
+    return prefill ? prompt_admitted(p) : decode_admitted(p);
 }
 
 }  // namespace paged
@@ -399,8 +340,8 @@ int mb_paged_reserve(const mb_paged_reserve_args* a, void* stream) {
         a->lengths == 0 || a->block_table == 0 || a->free_pages == 0 || a->free_count == 0 || a->offsets == 0 ||
         a->granted == 0 || (a->max_tokens > 0 && (a->slots == 0 || a->positions == 0 || a->rows == 0)))
         return MB_ERR_INVALID;
-    if ((a->counts | a->lengths | a->block_table | a->free_pages | a->free_count | a->offsets | a->rows | a->granted) % 4 ||
-        (a->slots | a->positions) % 8)
+    if ((a->counts | a->lengths | a->block_table | a->free_pages | a->free_count | a->offsets | a->granted) % 4 ||
+        (a->slots | a->positions | a->rows) % 16)
         return MB_ERR_INVALID;
     if (a->requests > kMaxRows || !page_size_covered(a->page_size) ||
         static_cast<int64_t>(a->width) * a->page_size > 0x7fffffffll)
@@ -478,18 +419,15 @@ int mb_paged_attention(const mb_paged_attention_args* a, void* stream) {
 int64_t mb_paged_prefill_workspace(const mb_paged_attention_args* a) {
     mb::paged::AttentionArgs p;
     const int rc = mb::paged::attention_args(a, true, p);
-    return rc == MB_OK ? 0 : -rc;
+    return rc == MB_OK ? mb::paged::prompt_workspace(p) : -rc;
 }
 
 int mb_paged_prefill(const mb_paged_attention_args* a, void* stream) {
-    using namespace mb::paged;
-    AttentionArgs p;
-    const int rc = attention_args(a, true, p);
+    mb::paged::AttentionArgs p;
+    const int rc = mb::paged::attention_args(a, true, p);
     if (rc != MB_OK) return rc;
-    const cudaError_t err = a->element == MB_BF16
-                                ? launch_attention<__nv_bfloat16>(p, static_cast<cudaStream_t>(stream))
-                                : launch_attention<__half>(p, static_cast<cudaStream_t>(stream));
-    return err == cudaSuccess ? MB_OK : mb::cuda_error(err, "mb_paged_prefill");
+    return mb::paged::prompt_attention(p, a->element, reinterpret_cast<void*>(a->workspace),
+                                       static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -84,6 +84,12 @@ cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, size
 int decode_admitted(const AttentionArgs& a);
 int64_t decode_workspace(const AttentionArgs& a);
 int decode_attention(const AttentionArgs& a, int element, void* workspace, cudaStream_t stream);
+int multiprocessors(int* device, cudaError_t* err);   // of the current device
+
+// mb_paged_prompt.cu
+int prompt_admitted(const AttentionArgs& a);
+int64_t prompt_workspace(const AttentionArgs& a);
+int prompt_attention(const AttentionArgs& a, int element, void* workspace, cudaStream_t stream);
 
 }  // namespace paged
 }  // namespace mb

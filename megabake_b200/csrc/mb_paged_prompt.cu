@@ -1,0 +1,937 @@
+// Causal attention of several new tokens a request over a paged key-value cache (mb_paged_prefill): the formula of
+// mb_paged_decode.cu for every query, whose position is the last key that it sees.
+//
+// Tensor cores bound it: 4 head_dim operations a pair of a query and a key it sees.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstdint>
+
+#include "mb_device.cuh"
+#include "mb_kernels.h"
+#include "mb_paged.cuh"
+#include "mb_tensor.cuh"
+
+namespace mb {
+namespace paged {
+namespace {
+
+constexpr int kRows = 128;             // of a query tile: tokens times the query heads of a key head
+constexpr int kThreads = 384;          // 4 + 4 softmax warps, one that copies, one that issues products, two idle
+constexpr int kMaxTiles = 12;          // of the ring: keys and values in turn
+constexpr int kInfos = 8;              // blocks whose masks are kept
+constexpr int kSmemLimit = 227 * 1024;
+constexpr int kTileCost = 128;         // what a unit costs besides its keys, in keys
+constexpr int kLeastKeys = 512;        // of a run
+constexpr int kWholeKeys = 1024;       // rows of the table that hold no more are not cut
+constexpr unsigned int kTmemColumns = 512;
+// A row's maximum may lag behind by this many powers of two before its sums are rescaled.
+constexpr float kLag = 8.f;
+// As kWeightShift, with room for the lag.
+template <typename T>
+constexpr float kPromptShift = 7.f;
+template <>
+constexpr float kPromptShift<__nv_bfloat16> = -39.f;
+
+template <int D>
+struct Config {
+    static constexpr int kBlock = D == 256 ? 64 : 128;       // keys of a block
+    static constexpr int kTiles = D == 256 ? 1 : 2;          // query tiles that share it
+    static constexpr int kChunks = D / 64;                   // 128-byte columns
+    static constexpr int kQueryBytes = kRows * D * 2;        // of one query tile
+    static constexpr int kTileBytes = kBlock * D * 2;        // of a block's keys, and of its values
+    static constexpr int kColumnO = 2 * kBlock;              // tensor memory: two score buffers, then the outputs
+};
+
+struct Split {
+    int request, head, tile, pieces;
+};
+
+struct PromptArgs {
+    AttentionArgs a;
+    int tile_tokens;       // of one query tile
+    int ring;              // tiles
+    float scale_log2;
+    Split* splits;         // [ctas]
+    float* stats;          // [ctas][2][tiles * 128][2]
+    float* partial;        // [ctas][2][tiles * 128][D]
+};
+
+struct PromptControl {
+    unsigned long long full[kMaxTiles], empty[kMaxTiles];
+    unsigned long long q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_empty[2];   // [slot], [tile] the last
+    unsigned long long half_ready, half_taken;
+    float half[kRows][2];        // maximum and sum of the second half of a lone query tile's keys
+    unsigned int mask[kInfos][4];
+    long long warp_sums[kThreads / 32];
+    unsigned int tmem;
+    int abort_flag;
+};
+
+struct Request {
+    int first, tokens, length;   // its queries, and its keys
+};
+
+// ---------------------------------------------------------------------------------------
+// The deal: units (a request, a key head, a pair of query tiles) one after the other, each as long as the keys its last
+// query sees and a constant, in equal runs over the CTAs.  A run begins and ends anywhere in a unit, at the nearest
+// block.  Lengths before a unit of a request are an arithmetic series, so a place is found by bisection.
+// ---------------------------------------------------------------------------------------
+struct Deal {
+    const long long* before;     // [requests + 1] lengths of the requests before, for one head
+    const Request* requests;
+    int count, heads, unit_tokens;
+    long long total, per;
+};
+
+__device__ __forceinline__ int units_of(const Request& q, int unit_tokens) {
+    return (q.tokens + unit_tokens - 1) / unit_tokens;
+}
+// Lengths of the first `j` of the request's units, all of them full.
+__device__ __forceinline__ long long length_before(const Request& q, int unit_tokens, long long j) {
+    return j * (max(q.length - q.tokens, 0) + kTileCost) + j * (j + 1) / 2 * unit_tokens;
+}
+__device__ __forceinline__ long long request_length(const Request& q, int unit_tokens) {
+    const int units = units_of(q, unit_tokens);
+    if (units == 0) return 0;
+    return length_before(q, unit_tokens, units - 1) + max(q.length - q.tokens, 0) + q.tokens + kTileCost;
+}
+
+template <int kBlock>
+struct Piece {
+    int request, head, tile;
+    int begin, end, blocks;      // blocks of this piece, and of the unit
+    int first, tokens;           // queries of the unit
+    int position;                // of its first query
+    long long unit_end;          // in the deal
+    long long next;              // where this piece ends in the deal
+    bool at_start;               // of the unit
+
+    __device__ __forceinline__ Piece(const Deal& d, long long at, long long run_end) {
+        int low = 0, high = d.count;   // before[low] * heads <= at < before[high] * heads
+        while (high - low > 1) {
+            const int middle = (low + high) >> 1;
+            if (d.before[middle] * d.heads <= at)
+                low = middle;
+            else
+                high = middle;
+        }
+        request = low;
+        const Request q = d.requests[low];
+        const long long length = d.before[low + 1] - d.before[low];
+        long long rest = at - d.before[low] * d.heads;
+        head = static_cast<int>(rest / length);
+        rest -= head * length;
+        int units = units_of(q, d.unit_tokens);
+        int lower = 0, upper = units;
+        while (upper - lower > 1) {
+            const int middle = (lower + upper) >> 1;
+            if (length_before(q, d.unit_tokens, middle) <= rest)
+                lower = middle;
+            else
+                upper = middle;
+        }
+        tile = lower;
+        const long long start = length_before(q, d.unit_tokens, tile);
+        const long long end_of = tile + 1 == units ? length : length_before(q, d.unit_tokens, tile + 1);
+        const long long unit_begin = at - (rest - start);
+        unit_end = unit_begin + (end_of - start);
+        next = min(unit_end, run_end);
+        first = q.first + tile * d.unit_tokens;
+        tokens = min(q.tokens - tile * d.unit_tokens, d.unit_tokens);
+        position = q.length - q.tokens + tile * d.unit_tokens;
+        blocks = max((position + tokens + kBlock - 1) / kBlock, 1);
+        begin = block_at(at - unit_begin, end_of - start);
+        end = block_at(next - unit_begin, end_of - start);
+        at_start = rest == start;
+    }
+    __device__ __forceinline__ int block_at(long long offset, long long length) const {
+        if (offset >= length) return blocks;
+        return static_cast<int>(min((offset + kBlock / 2) / kBlock, static_cast<long long>(blocks)));
+    }
+};
+
+// The first end or begin of a unit from `at` on.
+template <int kBlock>
+__device__ __forceinline__ long long unit_boundary(const Deal& d, long long at) {
+    if (at >= d.total) return at;
+    const Piece<kBlock> u(d, at, d.total);
+    return u.at_start ? at : u.unit_end;
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z,
+                                            unsigned long long* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_column(void* dst, const CUtensorMap* map, int column, int place, int head, int page,
+                                                unsigned long long* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(column), "r"(place), "r"(head), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+// D[tmem] (+)= A[tmem] . B[smem]: A's 16-bit elements two to a column, a row a lane.
+__device__ __forceinline__ void umma_from_tmem(unsigned int tmem_d, unsigned int tmem_a, unsigned long long desc_b,
+                                               unsigned int idesc, unsigned int accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Shared-memory operand whose rows are the reduction: [column of 64 elements][row], 128-byte swizzle; rows in groups of
+// 8 that lie 1024 bytes apart, columns `column_bytes` apart.
+__device__ __forceinline__ unsigned long long umma_desc_rows(unsigned int smem_addr, unsigned int column_bytes) {
+    unsigned long long d = 0;
+    d |= static_cast<unsigned long long>((smem_addr & 0x3ffffu) >> 4);
+    d |= static_cast<unsigned long long>(column_bytes >> 4) << 16;
+    d |= static_cast<unsigned long long>(1024 >> 4) << 32;
+    d |= 1ull << 46;
+    d |= 2ull << 61;
+    return d;
+}
+// 32 columns of this thread's lane, not waited for.
+__device__ __forceinline__ void tmem_load32_async(unsigned int taddr, float* v) {
+    unsigned int* r = reinterpret_cast<unsigned int*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_store16(unsigned int taddr, const unsigned int (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ unsigned int pack_pair(float x, float y) {
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const unsigned int*>(&h);
+    } else {
+        return prefill::pack_bf16_pair(x, y);
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// The kernel.  Two query tiles of 128 rows (tokens x the query heads of a key head) share every block of 128 keys:
+// while the softmax warps of one tile work on its scores, the tensor core multiplies for the other.  Scores come out in
+// tensor memory, weights go back there as 16-bit numbers over the scores they were made of and are the first
+// operand of the second product, values are taken as they lie in the pages (rows are the reduction).  A thread has a
+// row: no shuffles.  Outputs stay in tensor memory and are rescaled only when a row's maximum has grown by
+// more than 2^8 since the last time.  256-wide heads: one query tile, blocks of 64 keys, whose scores have two buffers.
+// ---------------------------------------------------------------------------------------
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __grid_constant__ CUtensorMap key_map,
+                        const __grid_constant__ CUtensorMap value_map, const __grid_constant__ PromptArgs p) {
+    using C = Config<D>;
+    constexpr int kBlock = C::kBlock, kTiles = C::kTiles, kChunks = C::kChunks;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    unsigned char* queries = smem;                                   // [tiles][chunks][128 rows][128 bytes]
+    unsigned char* ring = queries + kTiles * C::kQueryBytes;         // [ring][chunks][block rows][128 bytes]
+    PromptControl* ctl = reinterpret_cast<PromptControl*>(ring + static_cast<size_t>(p.ring) * C::kTileBytes);
+    long long* before = reinterpret_cast<long long*>(ctl + 1);       // [requests + 1]
+    Request* requests = reinterpret_cast<Request*>(before + p.a.requests + 1);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int shift = p.a.page_shift, page = 1 << shift;
+    const int group = p.a.heads / p.a.kv_heads;
+    if (tid == 0) {
+        for (int s = 0; s < p.ring; ++s) {
+            mbar_init(&ctl->full[s], 1);
+            mbar_init(&ctl->empty[s], 1);
+        }
+        mbar_init(&ctl->q_full, 1);
+        mbar_init(&ctl->q_empty, 1);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&ctl->s_full[s], 1);
+            mbar_init(&ctl->p_full[s], 4);
+            mbar_init(&ctl->pv_done[s], 1);
+            mbar_init(&ctl->o_empty[s], 4);
+        }
+        mbar_init(&ctl->half_ready, 4);
+        mbar_init(&ctl->half_taken, 4);
+        ctl->abort_flag = 0;
+        mbar_init_fence();
+    }
+    if (warp == 9) prefill::tmem_alloc(&ctl->tmem, kTmemColumns);
+    prefill::tc_fence_before();
+    __syncthreads();
+    prefill::tc_fence_after();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const unsigned int tmem = ctl->tmem;
+
+    Deal deal;
+    deal.before = before;
+    deal.requests = requests;
+    deal.count = p.a.requests;
+    deal.heads = p.a.kv_heads;
+    deal.unit_tokens = p.tile_tokens * kTiles;
+    {
+        const int each = (p.a.requests + kThreads - 1) / kThreads;
+        const int r0 = min(tid * each, p.a.requests), r1 = min(r0 + each, p.a.requests);
+        const int capacity = p.a.width << shift;
+        long long sum = 0;
+        for (int r = r0; r < r1; ++r) {
+            const int first = min(max(p.a.index[r], 0), p.a.tokens), end = min(max(p.a.index[r + 1], first), p.a.tokens);
+            const Request q = {first, end - first, min(max(p.a.lengths[r], 0), capacity)};
+            requests[r] = q;
+            sum += request_length(q, deal.unit_tokens);
+        }
+        long long inclusive = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long other = __shfl_up_sync(0xffffffffu, inclusive, d);
+            if (lane >= d) inclusive += other;
+        }
+        if (lane == 31) ctl->warp_sums[warp] = inclusive;
+        __syncthreads();
+        long long mine = inclusive - sum;
+        for (int w = 0; w < warp; ++w) mine += ctl->warp_sums[w];
+        for (int r = r0; r < r1; ++r) {
+            before[r] = mine;
+            mine += request_length(requests[r], deal.unit_tokens);
+        }
+        if (r0 < p.a.requests && r1 == p.a.requests) before[p.a.requests] = mine;
+        __syncthreads();
+    }
+    deal.total = before[p.a.requests] * deal.heads;
+    deal.per = max((deal.total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kLeastKeys));
+    long long run_begin = min(blockIdx.x * deal.per, deal.total);
+    long long run_end = min(run_begin + deal.per, deal.total);
+    if (p.splits == nullptr) {   // no unit is cut: runs go from unit to unit
+        run_begin = unit_boundary<kBlock>(deal, run_begin);
+        run_end = unit_boundary<kBlock>(deal, run_end);
+    }
+    volatile int* abort_flag = &ctl->abort_flag;
+    bool ok = true;
+
+    // A unit of two query tiles: each takes the blocks up to the one its last query lies in.  A lone tile of a pair takes
+    // the place of both, which share its blocks in turn and meet at the end.
+    auto lone = [&](const Piece<kBlock>& u) { return kTiles == 1 || u.tokens <= p.tile_tokens; };
+    auto tile_end = [&](const Piece<kBlock>& u, int t) {
+        if (t == 1 || lone(u)) return u.end;
+        return min(max((u.position + p.tile_tokens + kBlock - 1) / kBlock, 1), u.end);
+    };
+    auto takes = [&](const Piece<kBlock>& u, int t, int b) {
+        return kTiles == 1 ? t == 0 : lone(u) ? ((b - u.begin) & 1) == t : b < tile_end(u, t);
+    };
+
+    if (warp == 8) {
+        // ---- copies
+        int stage = 0, info = 0;
+        unsigned int round = 0, units = 0;
+        const int rows = min(page, kBlock);
+        const int per_block = kBlock / rows;
+        const int batch = 32 / per_block;
+        for (long long at = run_begin; ok && at < run_end;) {
+            const Piece<kBlock> u(deal, at, run_end);
+            at = u.next;
+            if (u.begin >= u.end) continue;
+            if (units > 0) ok = prefill::mbar_wait_warp(&ctl->q_empty, (units - 1) & 1, abort_flag);
+            if (!ok) break;
+            ++units;
+            const int tiles = u.tokens > p.tile_tokens ? 2 : 1;
+            if (elect_one()) {
+                mbar_arrive_expect_tx(&ctl->q_full, tiles * kChunks * p.tile_tokens * group * 128);
+                for (int t = 0; t < tiles; ++t)
+                    for (int c = 0; c < kChunks; ++c)
+                        tma_load_3d(queries + t * C::kQueryBytes + c * kRows * 128, &query_map, c * 64, u.head * group,
+                                    u.first + t * p.tile_tokens, &ctl->q_full);
+            }
+            __syncwarp();
+            const int n = max(min(u.position + u.tokens, p.a.width << shift), 0);   // keys that the unit sees
+            const int* entries = p.a.table + static_cast<size_t>(u.request) * p.a.width;
+            const int entries_end = (n + page - 1) >> shift;
+            auto entry_of = [&](int block) {
+                const int b = block + lane / per_block;
+                const int e = (b * kBlock + lane % per_block * rows) >> shift;
+                const int id = b < u.end && e < entries_end ? entries[e] : -1;
+                return id >= 0 && id < p.a.pages ? id : -1;
+            };
+            int next = entry_of(u.begin);
+            for (int b = u.begin; ok && b < u.end;) {
+                const int mine = next;
+                next = entry_of(b + batch);
+                for (int j = 0; ok && j < batch && b < u.end; ++j, ++b) {
+                    const int place = page > kBlock ? (b * kBlock) & (page - 1) : 0;
+                    const unsigned int valid = __ballot_sync(0xffffffffu, mine >= 0) >> (j * per_block);
+                    int boxes = 0;
+                    for (int i = 0; i < per_block; ++i) boxes += (valid >> i) & 1u;
+                    for (int kind = 0; kind < 2; ++kind) {   // keys, then values
+                        if (round > 0) ok = prefill::mbar_wait_warp(&ctl->empty[stage], (round - 1) & 1, abort_flag);
+                        if (!ok) break;
+                        if (kind == 0 && lane < kBlock / 32) {
+                            // which keys of the block count: on a page, and seen by any query of the unit
+                            unsigned int word = 0;
+                            for (int i = 0; i < 32; i += 8)
+                                if ((valid >> ((lane * 32 + i) / rows)) & 1u) word |= 0xffu << i;
+                            const int left = n - b * kBlock - lane * 32;
+                            if (left < 32) word &= left <= 0 ? 0u : (1u << left) - 1;
+                            ctl->mask[info][lane] = word;
+                        }
+                        __syncwarp();
+                        if (elect_one())
+                            mbar_arrive_expect_tx(&ctl->full[stage], boxes * kChunks * rows * 128);
+                        __syncwarp();
+                        unsigned char* to = ring + static_cast<size_t>(stage) * C::kTileBytes;
+                        for (int i = 0; i < per_block; ++i) {
+                            const int id = __shfl_sync(0xffffffffu, mine, j * per_block + i);
+                            if (id >= 0 && elect_one()) {
+#pragma unroll
+                                for (int c = 0; c < kChunks; ++c)
+                                    tma_load_column(to + c * kBlock * 128 + i * rows * 128,
+                                                    kind == 0 ? &key_map : &value_map, c * 64, place, u.head, id,
+                                                    &ctl->full[stage]);
+                            }
+                            __syncwarp();
+                        }
+                        if (++stage == p.ring) {
+                            stage = 0;
+                            ++round;
+                        }
+                    }
+                    info = (info + 1) % kInfos;
+                }
+            }
+        }
+    } else if (warp == 9) {
+        // ---- products: the scores of a step are issued before the weights of the step before are waited for
+        constexpr unsigned int kFormat = std::is_same_v<T, __half> ? 0u : (1u << 7) | (1u << 10);
+        constexpr unsigned int kIdescS = (1u << 4) | kFormat | (static_cast<unsigned int>(kBlock >> 3) << 17) |
+                                         (static_cast<unsigned int>(kRows >> 4) << 24);
+        constexpr unsigned int kIdescO = (1u << 4) | kFormat | (1u << 16) | (static_cast<unsigned int>(D >> 3) << 17) |
+                                         (static_cast<unsigned int>(kRows >> 4) << 24);
+        int stage = 0, info = 0;
+        unsigned int round = 0, units = 0;
+        unsigned int p_phase[2] = {0, 0}, opened[2] = {0, 0};
+        for (long long at = run_begin; ok && at < run_end;) {
+            const Piece<kBlock> u(deal, at, run_end);
+            at = u.next;
+            if (u.begin >= u.end) continue;
+            ok = prefill::mbar_wait_warp(&ctl->q_full, units & 1, abort_flag);
+            if (!ok) break;
+            ++units;
+            int key_stage = 0, value_stage = 0;          // of the block whose scores were issued last
+            unsigned int key_round = 0, value_round = 0;
+            bool first[2] = {true, true};                // no product into the outputs of the tile yet
+            int pending_tile = -1, pending_slot = 0, pending_stage = 0, pending_info = 0;
+            unsigned int pending_round = 0;
+            bool pending_last = false;                   // of its block
+
+            auto weights_times_values = [&]() {
+                if (first[pending_tile] && opened[pending_tile] > 0)   // the outputs before have been taken
+                    ok = prefill::mbar_wait_warp(&ctl->o_empty[pending_tile], (opened[pending_tile] - 1) & 1, abort_flag);
+                ok = ok && prefill::mbar_wait_warp(&ctl->full[pending_stage], pending_round & 1, abort_flag);
+                if (!ok) return;
+                unsigned char* values = ring + static_cast<size_t>(pending_stage) * C::kTileBytes;
+                // values of keys that do not count may be anything: 0 * NaN is NaN
+                bool partial = false;
+#pragma unroll
+                for (int w = 0; w < kBlock / 32; ++w) partial |= ctl->mask[pending_info][w] != 0xffffffffu;
+                if (partial) {
+                    for (int i = lane; i < kBlock * kChunks * 8; i += 32) {
+                        const int row = i >> 3 & (kBlock - 1);
+                        if (!((ctl->mask[pending_info][row >> 5] >> (row & 31)) & 1u))
+                            *reinterpret_cast<uint4*>(values + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                ok = prefill::mbar_wait_warp(&ctl->p_full[pending_slot], p_phase[pending_slot] & 1, abort_flag);
+                if (!ok) return;
+                ++p_phase[pending_slot];
+                prefill::tc_fence_after();
+                const bool fresh = first[pending_tile];
+                if (fresh) {
+                    first[pending_tile] = false;
+                    ++opened[pending_tile];
+                }
+                if (elect_one()) {
+                    const unsigned int base = smem_u32(values);
+#pragma unroll
+                    for (int k = 0; k < kBlock / 16; ++k)
+                        umma_from_tmem(tmem + C::kColumnO + pending_tile * D, tmem + pending_slot * kBlock + k * 8,
+                                       umma_desc_rows(base + k * 16 * 128, kBlock * 128), kIdescO,
+                                       fresh && k == 0 ? 0u : 1u);
+                    prefill::umma_commit(&ctl->pv_done[pending_slot]);
+                    if (pending_last) prefill::umma_commit(&ctl->empty[pending_stage]);
+                }
+                __syncwarp();
+            };
+
+            for (int b = u.begin; ok && b < u.end; ++b) {
+                key_stage = stage;
+                key_round = round;
+                if (++stage == p.ring) {
+                    stage = 0;
+                    ++round;
+                }
+                value_stage = stage;
+                value_round = round;
+                if (++stage == p.ring) {
+                    stage = 0;
+                    ++round;
+                }
+                ok = prefill::mbar_wait_warp(&ctl->full[key_stage], key_round & 1, abort_flag);
+                if (!ok) break;
+                const int last_tile = takes(u, 1, b) ? 1 : 0;
+                for (int t = 0; ok && t < kTiles; ++t) {
+                    if (!takes(u, t, b)) continue;
+                    const int slot = kTiles == 2 ? t : b & 1;
+                    if (pending_tile >= 0 && pending_slot == slot) {   // its weights lie where these scores go
+                        weights_times_values();
+                        pending_tile = -1;
+                        if (!ok) break;
+                    }
+                    prefill::tc_fence_after();
+                    if (elect_one()) {
+                        const unsigned int q = smem_u32(queries + (lone(u) ? 0 : t * C::kQueryBytes));
+                        const unsigned int k0 = smem_u32(ring + static_cast<size_t>(key_stage) * C::kTileBytes);
+#pragma unroll
+                        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                prefill::umma_bf16(tmem + slot * kBlock, prefill::umma_desc(q + c * kRows * 128) + 2 * k,
+                                                   prefill::umma_desc(k0 + c * kBlock * 128) + 2 * k, kIdescS,
+                                                   (c | k) != 0 ? 1u : 0u);
+                        prefill::umma_commit(&ctl->s_full[slot]);
+                        if (t == last_tile) {
+                            prefill::umma_commit(&ctl->empty[key_stage]);
+                            if (b == u.end - 1) prefill::umma_commit(&ctl->q_empty);
+                        }
+                    }
+                    __syncwarp();
+                    if (pending_tile >= 0) weights_times_values();
+                    pending_tile = t;
+                    pending_slot = slot;
+                    pending_stage = value_stage;
+                    pending_round = value_round;
+                    pending_info = info;
+                    pending_last = t == last_tile;
+                }
+                info = (info + 1) % kInfos;
+            }
+            if (ok && pending_tile >= 0) weights_times_values();
+        }
+    } else if (warp < 4 * kTiles) {
+        // ---- softmax and outputs of one query tile: a thread has a row
+        const int tile = warp >> 2, r = (warp & 3) * 32 + lane;
+        const int token = r / group, query = r % group;          // of the tile
+        const unsigned int lanes = tmem + (static_cast<unsigned int>((warp & 3) * 32) << 16);
+        const unsigned int outputs = lanes + C::kColumnO + tile * D;
+        int info = 0;
+        unsigned int steps[2] = {0, 0};                 // of every slot so far
+        unsigned int halves = 0;                        // lone tiles so far
+        Split split = {0, 0, 0, 0};
+        const bool premultiply = p.scale_log2 <= 0.f;   // the largest score is not that of the largest product
+        const float multiplier = premultiply ? 1.f : p.scale_log2;
+        for (long long at = run_begin; at < run_end;) {
+            const Piece<kBlock> u(deal, at, run_end);
+            at = u.next;
+            const int slot_out = (blockIdx.x * 2 + (u.begin == 0 && u.end > 0 ? 1 : 0)) * kTiles * kRows + tile * kRows + r;
+            if (u.begin >= u.end) {
+                if (!u.at_start && p.splits != nullptr)   // counted as a piece
+                    *reinterpret_cast<float2*>(p.stats + static_cast<size_t>(slot_out) * 2) = make_float2(-INFINITY, 0.f);
+                continue;
+            }
+            const bool alone = kTiles == 2 && lone(u);
+            const int own = alone ? 0 : tile;                    // query tile
+            const int first_block = alone ? u.begin + tile : u.begin, blocks = tile_end(u, tile);
+            const int mine = own * p.tile_tokens + token;        // token of the unit
+            const int position = u.position + mine, first_position = u.position + own * p.tile_tokens;
+            float m = -INFINITY, l = 0.f;
+            for (int b = first_block; b < blocks; b += alone ? 2 : 1) {
+                const int slot = kTiles == 2 ? tile : b & 1;
+                ok = ok && prefill::mbar_wait_warp(&ctl->s_full[slot], steps[slot] & 1, abort_flag);
+                if (!ok) break;
+                ++steps[slot];
+                prefill::tc_fence_after();
+                const unsigned int scores = lanes + slot * kBlock;
+                float s[kBlock];
+#pragma unroll
+                for (int c = 0; c < kBlock; c += 32) tmem_load32_async(scores + c, s + c);
+                unsigned int word[kBlock / 32];
+                bool partial = b * kBlock + kBlock - 1 > first_position;
+#pragma unroll
+                for (int w = 0; w < kBlock / 32; ++w) {
+                    word[w] = ctl->mask[(info + b - u.begin) % kInfos][w];
+                    partial |= word[w] != 0xffffffffu;
+                }
+                tmem_wait_load();
+                if (premultiply) {
+#pragma unroll
+                    for (int c = 0; c < kBlock; ++c) s[c] *= p.scale_log2;
+                }
+                if (partial) {
+#pragma unroll
+                    for (int w = 0; w < kBlock / 32; ++w) {
+                        const int seen = position - b * kBlock - w * 32;   // the last key of the word that counts
+                        const unsigned int keep = word[w] & (seen < 0 ? 0u : seen >= 31 ? ~0u : (2u << seen) - 1);
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) s[w * 32 + c] = (keep >> c) & 1u ? s[w * 32 + c] : -INFINITY;
+                    }
+                }
+                float highest[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int c = 4; c < kBlock; c += 4)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) highest[i] = fmaxf(highest[i], s[c + i]);
+                const float now = fmaxf(fmaxf(highest[0], highest[1]), fmaxf(highest[2], highest[3])) * multiplier;
+                if (b == first_block) {
+                    m = now;
+                } else if (__any_sync(0xffffffffu, now > m + kLag || (m == -INFINITY && now > m))) {
+                    const float grown = fmaxf(m, now);
+                    const float base = grown == -INFINITY ? 0.f : grown;
+                    const float factor = prefill::exp2_approx(m - base);
+                    m = grown;
+                    l *= factor;
+                    // the product before is in the outputs; the one before that is, since these scores are there
+                    const int slot_before = kTiles == 2 ? slot : slot ^ 1;
+                    ok = prefill::mbar_wait_warp(&ctl->pv_done[slot_before],
+                                                 (steps[slot_before] - (kTiles == 2 ? 2 : 1)) & 1, abort_flag);
+                    if (!ok) break;
+                    prefill::tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 16) {
+                        float o[16];
+                        unsigned int raw[16];
+                        prefill::tmem_load16(outputs + c, o);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) raw[i] = __float_as_uint(o[i] * factor);
+                        tmem_store16(outputs + c, raw);
+                    }
+                    tmem_wait_store();
+                }
+                const float base = (m == -INFINITY ? 0.f : m) - kPromptShift<T>;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < kBlock; c += 32) {
+                    unsigned int packed[16];
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float x = prefill::exp2_approx(fmaf(s[c + i], multiplier, -base));
+                        const float y = prefill::exp2_approx(fmaf(s[c + i + 1], multiplier, -base));
+                        sum[i & 2] += x;
+                        sum[(i & 2) + 1] += y;
+                        packed[i / 2] = pack_pair<T>(x, y);
+                    }
+                    tmem_store16(scores + c / 2, packed);
+                }
+                tmem_wait_store();
+                prefill::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl->p_full[slot]);
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            }
+            info = (info + u.end - u.begin) % kInfos;
+            // the outputs of the piece
+            const bool any = first_block < blocks;
+            if (any) {
+                const int slot = kTiles == 2 ? tile : (blocks - 1) & 1;
+                ok = ok && prefill::mbar_wait_warp(&ctl->pv_done[slot], (steps[slot] - 1) & 1, abort_flag);
+                prefill::tc_fence_after();
+            }
+            float keep = 1.f, other = 0.f;   // factors of these outputs and of the other half's
+            bool other_any = false;
+            if (alone) {
+                if (tile == 1) {
+                    if (halves > 0) ok = ok && prefill::mbar_wait_warp(&ctl->half_taken, (halves - 1) & 1, abort_flag);
+                    ++halves;
+                    ctl->half[r][0] = m;
+                    ctl->half[r][1] = l;
+                    prefill::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ctl->half_ready);
+                    continue;
+                }
+                ok = ok && prefill::mbar_wait_warp(&ctl->half_ready, halves & 1, abort_flag);
+                ++halves;
+                prefill::tc_fence_after();
+                other_any = u.end - u.begin > 1;
+                const float m1 = ctl->half[r][0], grown = fmaxf(m, m1), base = grown == -INFINITY ? 0.f : grown;
+                keep = prefill::exp2_approx(m - base);
+                other = prefill::exp2_approx(m1 - base);
+                l = l * keep + ctl->half[r][1] * other;
+                m = grown;
+            }
+            const bool whole = u.begin == 0 && u.end == u.blocks;
+            const bool stored = ok && any && mine < u.tokens && token < p.tile_tokens;
+            const float inverse = l == 0.f ? 0.f : 1.f / l;
+            if (whole) keep *= inverse, other *= inverse;
+            if (!whole)
+                *reinterpret_cast<float2*>(p.stats + static_cast<size_t>(slot_out) * 2) =
+                    make_float2(any && l != 0.f ? m : -INFINITY, l);
+            unsigned short* to = p.a.out + (static_cast<size_t>(u.first + mine) * p.a.heads + u.head * group + query) * D;
+            float* partial = p.partial + static_cast<size_t>(slot_out) * D;
+            if (ok && any) {
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    float o[32];
+                    tmem_load32_async(outputs + c, o);
+                    tmem_wait_load();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] *= keep;
+                    if (other_any) {
+                        float o1[32];
+                        tmem_load32_async(outputs + D + c, o1);
+                        tmem_wait_load();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = fmaf(o1[i], other, o[i]);
+                    }
+                    if (!stored) continue;
+                    if (whole) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8)
+                            *reinterpret_cast<uint4*>(to + c + i) =
+                                l == 0.f ? make_uint4(0u, 0u, 0u, 0u)
+                                         : make_uint4(pack_pair<T>(o[i], o[i + 1]), pack_pair<T>(o[i + 2], o[i + 3]),
+                                                      pack_pair<T>(o[i + 4], o[i + 5]), pack_pair<T>(o[i + 6], o[i + 7]));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<float4*>(partial + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    }
+                }
+            }
+            if (!whole && u.begin == 0)
+                split = {u.request, u.head, u.tile, static_cast<int>((u.unit_end - 1) / deal.per - blockIdx.x) + 1};
+            prefill::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (any) mbar_arrive(&ctl->o_empty[tile]);
+                if (other_any) mbar_arrive(&ctl->o_empty[1]);
+                if (alone) mbar_arrive(&ctl->half_taken);
+            }
+        }
+        if (tid == 0 && p.splits != nullptr)
+            *reinterpret_cast<int4*>(p.splits + blockIdx.x) = make_int4(split.request, split.head, split.tile, split.pieces);
+    } else if (p.a.zero_rest != 0 && warp >= 10) {
+        // queries of no request
+        const size_t row = static_cast<size_t>(p.a.heads) * D / 8;
+        int end = 0;
+        for (int r = 0; r < p.a.requests; ++r) end = max(end, requests[r].first + requests[r].tokens);
+        uint4* to = reinterpret_cast<uint4*>(p.a.out) + end * row;
+        const size_t all = (p.a.tokens - end) * row;
+        for (size_t i = blockIdx.x * 64 + (tid - 320); i < all; i += gridDim.x * 64) to[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (!ok && lane == 0) {
+        *abort_flag = 1;
+        if (p.a.status != nullptr) *p.a.status = MB_ST_PIPE_TIMEOUT;
+    }
+    prefill::tc_fence_before();
+    __syncthreads();
+    if (*abort_flag != 0) {   // copies and products that are under way end before the memory goes
+        const unsigned long long start = global_timer_ns();
+        while (global_timer_ns() - start < 200000ull) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (warp == 9) prefill::tmem_dealloc(tmem, kTmemColumns);
+}
+
+// The pieces of a unit that several CTAs share, in the order of its keys; a quarter warp or more has a row.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinRows = 16;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) prompt_join_kernel(const __grid_constant__ PromptArgs p) {
+    constexpr int kUnitRows = Config<D>::kTiles * kRows, kColumns = D / 4;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 raw = __ldcg(reinterpret_cast<const int4*>(p.splits + blockIdx.x));
+    const int request = raw.x, head = raw.y, unit = raw.z, pieces = raw.w;
+    if (pieces == 0) return;
+    const int group = p.a.heads / p.a.kv_heads, unit_tokens = p.tile_tokens * Config<D>::kTiles;
+    const int first = min(max(p.a.index[request], 0), p.a.tokens);
+    const int tokens = min(max(p.a.index[request + 1], first), p.a.tokens) - first;
+    auto slot_of = [&](int i) { return (static_cast<size_t>(blockIdx.x) + i) * 2 + (i == 0 ? 1 : 0); };
+    for (int i = threadIdx.x; i < kJoinRows * kColumns; i += kJoinThreads) {
+        const int r = blockIdx.y * kJoinRows + i / kColumns, c = i % kColumns * 4;
+        const int tile = r / kRows, in_tile = r % kRows, token = in_tile / group;
+        const int mine = unit * unit_tokens + tile * p.tile_tokens + token;
+        if (token >= p.tile_tokens || mine >= tokens) continue;
+        float highest = -INFINITY;
+        for (int q = 0; q < pieces; ++q) highest = fmaxf(highest, __ldcg(p.stats + (slot_of(q) * kUnitRows + r) * 2));
+        float total = 0.f;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int q = 0; q < pieces; ++q) {
+            const float2 s = __ldcg(reinterpret_cast<const float2*>(p.stats + (slot_of(q) * kUnitRows + r) * 2));
+            if (s.x == -INFINITY) continue;   // nothing of it was written
+            const float w = prefill::exp2_approx(s.x - highest);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.partial + (slot_of(q) * kUnitRows + r) * D + c));
+            total = fmaf(w, s.y, total);
+            sum.x = fmaf(w, v.x, sum.x);
+            sum.y = fmaf(w, v.y, sum.y);
+            sum.z = fmaf(w, v.z, sum.z);
+            sum.w = fmaf(w, v.w, sum.w);
+        }
+        store_output<T>(p.a.out + (static_cast<size_t>(first + mine) * p.a.heads + head * group + in_tile % group) * D + c,
+                        sum, total);
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------
+struct Shape {
+    int tiles, tile_tokens, ctas, ring, smem;
+    size_t stats, splits, bytes;   // workspace: partial sums, then from `stats` on the statistics, then the splits
+    bool joined;
+};
+
+template <int D>
+Shape shape_of(const AttentionArgs& a, int sms) {
+    using C = Config<D>;
+    Shape s;
+    const int group = a.heads / a.kv_heads;
+    s.tiles = C::kTiles;
+    s.tile_tokens = kRows / group;
+    // at most so many units, none longer than a row of the table
+    const long long units = (a.tokens / (s.tile_tokens * s.tiles) + std::min(a.requests, a.tokens)) * static_cast<long long>(a.kv_heads);
+    const long long capacity = static_cast<long long>(a.width) << a.page_shift;
+    const long long most = (units * (capacity + kTileCost) + kLeastKeys - 1) / kLeastKeys;
+    s.ctas = static_cast<int>(std::min<long long>(most, sms));
+    s.joined = capacity > kWholeKeys;
+    const int rest = C::kTiles * C::kQueryBytes + static_cast<int>(sizeof(PromptControl)) + 8 * (a.requests + 1) +
+                     static_cast<int>(sizeof(Request)) * a.requests;
+    s.ring = (kSmemLimit - rest) / C::kTileBytes;
+    if (s.ring > kMaxTiles) s.ring = kMaxTiles;
+    s.smem = rest + s.ring * C::kTileBytes;
+    const size_t rows = static_cast<size_t>(s.ctas) * 2 * C::kTiles * kRows;
+    s.stats = rows * D * 4;
+    s.splits = s.stats + rows * 8;
+    s.bytes = s.joined ? s.splits + s.ctas * sizeof(Split) : 0;
+    return s;
+}
+
+Shape shape_of(const AttentionArgs& a, int sms) {
+    return a.head_dim == 64 ? shape_of<64>(a, sms) : a.head_dim == 128 ? shape_of<128>(a, sms) : shape_of<256>(a, sms);
+}
+
+template <typename T, int D>
+cudaError_t launch_prompt(const CUtensorMap& queries, const CUtensorMap& keys, const CUtensorMap& values,
+                          const PromptArgs& args, const Shape& s, int device, cudaStream_t stream) {
+    static std::atomic<unsigned long long> configured{0};   // devices, by their bits
+    if (device >= 64 || !(configured.load(std::memory_order_relaxed) >> device & 1)) {
+        const cudaError_t err = cudaFuncSetAttribute(prompt_attention_kernel<T, D>,
+                                                     cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+        if (err != cudaSuccess) return err;
+        if (device < 64) configured.fetch_or(1ull << device, std::memory_order_relaxed);
+    }
+    cudaError_t err = launch_early(prompt_attention_kernel<T, D>, dim3(s.ctas), kThreads, s.smem, 1, stream, queries, keys,
+                                   values, args);
+    if (err == cudaSuccess && s.joined)
+        err = launch_early(prompt_join_kernel<T, D>, dim3(s.ctas, Config<D>::kTiles * kRows / kJoinRows), kJoinThreads, 0,
+                           1, stream, args);
+    return err;
+}
+
+template <typename T>
+cudaError_t launch_prompt(const CUtensorMap& queries, const CUtensorMap& keys, const CUtensorMap& values,
+                          const PromptArgs& args, const Shape& s, int device, cudaStream_t stream) {
+    if (args.a.head_dim == 64) return launch_prompt<T, 64>(queries, keys, values, args, s, device, stream);
+    if (args.a.head_dim == 128) return launch_prompt<T, 128>(queries, keys, values, args, s, device, stream);
+    return launch_prompt<T, 256>(queries, keys, values, args, s, device, stream);
+}
+
+CUtensorMapDataType data_type(int element) {
+    return element == MB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
+// Boxes of one 128-byte column of up to a block of tokens of a page and head.
+bool make_column_map(CUtensorMap* map, const AttentionArgs& a, const void* base, const Strides3& s, int element,
+                     int block) {
+    prefill::EncodeTiledFn fn = prefill::encode_tiled();
+    if (fn == nullptr) return false;
+    const int page = 1 << a.page_shift;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(page),
+                                static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.pages)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(s.token) * 2, static_cast<cuuint64_t>(s.head) * 2,
+                                   static_cast<cuuint64_t>(s.page) * 2};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(page < block ? page : block), 1, 1};
+    const cuuint32_t steps[4] = {1, 1, 1, 1};
+    return fn(map, data_type(element), 4, const_cast<void*>(base), dims, strides, box, steps,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Boxes of one 128-byte column of the query heads of a key head, for the tokens of a tile.
+bool make_query_map(CUtensorMap* map, const AttentionArgs& a, int element, int tile_tokens) {
+    prefill::EncodeTiledFn fn = prefill::encode_tiled();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(a.heads),
+                                static_cast<cuuint64_t>(a.tokens)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(a.q.head) * 2, static_cast<cuuint64_t>(a.q.token) * 2};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.heads / a.kv_heads), static_cast<cuuint32_t>(tile_tokens)};
+    const cuuint32_t steps[3] = {1, 1, 1};
+    return fn(map, data_type(element), 3, const_cast<unsigned short*>(a.query), dims, strides, box, steps,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
+int prompt_admitted(const AttentionArgs& a) { return a.heads / a.kv_heads <= kRows ? MB_OK : MB_ERR_UNSUPPORTED; }
+
+int64_t prompt_workspace(const AttentionArgs& a) {
+    int device;
+    cudaError_t err;
+    const int sms = multiprocessors(&device, &err);
+    if (err != cudaSuccess) return -cuda_error(err, "mb_paged_prefill_workspace");
+    return static_cast<int64_t>(shape_of(a, sms).bytes);
+}
+
+int prompt_attention(const AttentionArgs& a, int element, void* workspace, cudaStream_t stream) {
+    int device;
+    cudaError_t err;
+    const int sms = multiprocessors(&device, &err);
+    if (err != cudaSuccess) return cuda_error(err, "mb_paged_prefill");
+    const Shape s = shape_of(a, sms);
+    if (s.ring < 3) return MB_ERR_RESOURCE;
+    if (s.bytes != 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256)) return MB_ERR_INVALID;
+    CUtensorMap queries, keys, values;
+    const int block = a.head_dim == 256 ? Config<256>::kBlock : Config<128>::kBlock;
+    if (!make_query_map(&queries, a, element, s.tile_tokens) ||
+        !make_column_map(&keys, a, a.key_pages, a.kpool, element, block) ||
+        !make_column_map(&values, a, a.value_pages, a.vpool, element, block))
+        return MB_ERR_UNSUPPORTED;
+    PromptArgs args;
+    args.a = a;
+    args.tile_tokens = s.tile_tokens;
+    args.ring = s.ring;
+    args.scale_log2 = a.scale * kLog2e;
+    char* base = static_cast<char*>(workspace);
+    args.partial = reinterpret_cast<float*>(base);
+    args.stats = reinterpret_cast<float*>(base + s.stats);
+    args.splits = s.joined ? reinterpret_cast<Split*>(base + s.splits) : nullptr;
+    err = element == MB_BF16 ? launch_prompt<__nv_bfloat16>(queries, keys, values, args, s, device, stream)
+                             : launch_prompt<__half>(queries, keys, values, args, s, device, stream);
+    return err == cudaSuccess ? MB_OK : cuda_error(err, "mb_paged_prefill");
+}
+
+}  // namespace paged
+}  // namespace mb
