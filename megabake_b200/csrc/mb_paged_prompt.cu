@@ -21,7 +21,12 @@ namespace paged {
 namespace {
 
 constexpr int kRows = 128;             // of a query tile: tokens times the query heads of a key head
-constexpr int kThreads = 384;          // 4 + 4 softmax warps, one that copies, one that issues products, two idle
+// 4 + 4 softmax warps, one that copies, one that issues products, and two that fill their warpgroup: the softmax warps
+// take registers from it (a row's 128 scores stay in registers; read twice from tensor memory instead, a block took
+// 5,500 cycles, not 4,400).
+constexpr int kThreads = 384;
+constexpr int kLaunchRegisters = 168, kSoftmaxRegisters = 200, kOtherRegisters = 104;
+static_assert(2 * kSoftmaxRegisters + kOtherRegisters == 3 * kLaunchRegisters, "no more than the block was launched with");
 constexpr int kMaxTiles = 12;          // of the ring: keys and values in turn
 constexpr int kInfos = 8;              // blocks whose masks are kept
 constexpr int kSmemLimit = 227 * 1024;
@@ -67,6 +72,7 @@ struct PromptControl {
     unsigned long long half_ready, half_taken;
     float half[kRows][2];        // maximum and sum of the second half of a lone query tile's keys
     unsigned int mask[kInfos][4];
+    int partial[kInfos];         // not every key of the block counts
     long long warp_sums[kThreads / 32];
     unsigned int tmem;
     int abort_flag;
@@ -226,6 +232,37 @@ __device__ __forceinline__ void tmem_store16(unsigned int taddr, const unsigned 
         : "memory");
 }
 
+// Where every warp of a warpgroup passes; 256-wide heads get by with what they were launched with.
+template <bool kUsed>
+__device__ __forceinline__ void take_registers() {
+    if constexpr (kUsed) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
+}
+template <bool kUsed>
+__device__ __forceinline__ void give_registers() {
+    if constexpr (kUsed) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
+}
+
+// Two floats in a 64-bit register, for instructions that work on both.
+__device__ __forceinline__ unsigned long long pair_of(float x, float y) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float pair_low(unsigned long long v) { return __uint_as_float(static_cast<unsigned int>(v)); }
+__device__ __forceinline__ float pair_high(unsigned long long v) {
+    return __uint_as_float(static_cast<unsigned int>(v >> 32));
+}
+__device__ __forceinline__ unsigned long long fma_pair(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add_pair(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 template <typename T>
 __device__ __forceinline__ unsigned int pack_pair(float x, float y) {
     if constexpr (std::is_same_v<T, __half>) {
@@ -338,12 +375,10 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         if (t == 1 || lone(u)) return u.end;
         return min(max((u.position + p.tile_tokens + kBlock - 1) / kBlock, 1), u.end);
     };
-    auto takes = [&](const Piece<kBlock>& u, int t, int b) {
-        return kTiles == 1 ? t == 0 : lone(u) ? ((b - u.begin) & 1) == t : b < tile_end(u, t);
-    };
 
     if (warp == 8) {
         // ---- copies
+        give_registers<kTiles == 2>();
         int stage = 0, info = 0;
         unsigned int round = 0, units = 0;
         const int rows = min(page, kBlock);
@@ -396,6 +431,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                             ctl->mask[info][lane] = word;
                         }
                         __syncwarp();
+                        if (kind == 0 && lane == 0)
+                            ctl->partial[info] = boxes != per_block || n - b * kBlock < kBlock;
+                        __syncwarp();
                         if (elect_one())
                             mbar_arrive_expect_tx(&ctl->full[stage], boxes * kChunks * rows * 128);
                         __syncwarp();
@@ -421,15 +459,20 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             }
         }
     } else if (warp == 9) {
-        // ---- products: the scores of a step are issued before the weights of the step before are waited for
+        // ---- products: the scores of a step are issued before the weights of the step before are waited for.  The warp is
+        // busy with little else than issuing, and what it does between two products is time the tensor core waits: phases
+        // are bits of registers (arrays with an index would be memory), what a block needs is read a step ahead.
         constexpr unsigned int kFormat = std::is_same_v<T, __half> ? 0u : (1u << 7) | (1u << 10);
         constexpr unsigned int kIdescS = (1u << 4) | kFormat | (static_cast<unsigned int>(kBlock >> 3) << 17) |
                                          (static_cast<unsigned int>(kRows >> 4) << 24);
         constexpr unsigned int kIdescO = (1u << 4) | kFormat | (1u << 16) | (static_cast<unsigned int>(D >> 3) << 17) |
                                          (static_cast<unsigned int>(kRows >> 4) << 24);
+        give_registers<kTiles == 2>();
+        const unsigned int ring_at = smem_u32(ring), queries_at = smem_u32(queries);
         int stage = 0, info = 0;
         unsigned int round = 0, units = 0;
-        unsigned int p_phase[2] = {0, 0}, opened[2] = {0, 0};
+        unsigned int p_phase = 0;                // bit: slot
+        unsigned int o_phase = 0, o_used = 0;    // bit: query tile
         for (long long at = run_begin; ok && at < run_end;) {
             const Piece<kBlock> u(deal, at, run_end);
             at = u.next;
@@ -437,24 +480,25 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             ok = prefill::mbar_wait_warp(&ctl->q_full, units & 1, abort_flag);
             if (!ok) break;
             ++units;
-            int key_stage = 0, value_stage = 0;          // of the block whose scores were issued last
-            unsigned int key_round = 0, value_round = 0;
-            bool first[2] = {true, true};                // no product into the outputs of the tile yet
+            const bool alone = lone(u);
+            const int end0 = tile_end(u, 0), begin = u.begin, end = u.end;
+            unsigned int fresh = 3;              // bit: no product into the outputs of the tile yet
+            // the step whose scores were issued last
             int pending_tile = -1, pending_slot = 0, pending_stage = 0, pending_info = 0;
-            unsigned int pending_round = 0;
-            bool pending_last = false;                   // of its block
+            unsigned int pending_parity = 0;
+            bool pending_last = false, pending_partial = false;
 
             auto weights_times_values = [&]() {
-                if (first[pending_tile] && opened[pending_tile] > 0)   // the outputs before have been taken
-                    ok = prefill::mbar_wait_warp(&ctl->o_empty[pending_tile], (opened[pending_tile] - 1) & 1, abort_flag);
-                ok = ok && prefill::mbar_wait_warp(&ctl->full[pending_stage], pending_round & 1, abort_flag);
-                if (!ok) return;
-                unsigned char* values = ring + static_cast<size_t>(pending_stage) * C::kTileBytes;
-                // values of keys that do not count may be anything: 0 * NaN is NaN
-                bool partial = false;
-#pragma unroll
-                for (int w = 0; w < kBlock / 32; ++w) partial |= ctl->mask[pending_info][w] != 0xffffffffu;
-                if (partial) {
+                const unsigned int tile_bit = 1u << pending_tile;
+                const bool first = (fresh & tile_bit) != 0;
+                if (first && (o_used & tile_bit)) {   // the outputs before have been taken
+                    ok = prefill::mbar_wait_warp(&ctl->o_empty[pending_tile], (o_phase >> pending_tile) & 1, abort_flag);
+                    o_phase ^= tile_bit;
+                }
+                ok = ok && prefill::mbar_wait_warp(&ctl->full[pending_stage], pending_parity, abort_flag);
+                if (ok && pending_partial) {
+                    // values of keys that do not count may be anything: 0 * NaN is NaN
+                    unsigned char* values = ring + static_cast<size_t>(pending_stage) * C::kTileBytes;
                     for (int i = lane; i < kBlock * kChunks * 8; i += 32) {
                         const int row = i >> 3 & (kBlock - 1);
                         if (!((ctl->mask[pending_info][row >> 5] >> (row & 31)) & 1u))
@@ -463,67 +507,69 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
-                ok = prefill::mbar_wait_warp(&ctl->p_full[pending_slot], p_phase[pending_slot] & 1, abort_flag);
+                ok = ok && prefill::mbar_wait_warp(&ctl->p_full[pending_slot], (p_phase >> pending_slot) & 1, abort_flag);
                 if (!ok) return;
-                ++p_phase[pending_slot];
+                p_phase ^= 1u << pending_slot;
+                fresh &= ~tile_bit;
+                o_used |= tile_bit;
                 prefill::tc_fence_after();
-                const bool fresh = first[pending_tile];
-                if (fresh) {
-                    first[pending_tile] = false;
-                    ++opened[pending_tile];
-                }
                 if (elect_one()) {
-                    const unsigned int base = smem_u32(values);
+                    const unsigned long long v = umma_desc_rows(ring_at + pending_stage * C::kTileBytes, kBlock * 128);
+                    const unsigned int to = tmem + C::kColumnO + pending_tile * D, from = tmem + pending_slot * kBlock;
 #pragma unroll
                     for (int k = 0; k < kBlock / 16; ++k)
-                        umma_from_tmem(tmem + C::kColumnO + pending_tile * D, tmem + pending_slot * kBlock + k * 8,
-                                       umma_desc_rows(base + k * 16 * 128, kBlock * 128), kIdescO,
-                                       fresh && k == 0 ? 0u : 1u);
+                        umma_from_tmem(to, from + k * 8, v + (k * 16 * 128 >> 4), kIdescO, first && k == 0 ? 0u : 1u);
                     prefill::umma_commit(&ctl->pv_done[pending_slot]);
                     if (pending_last) prefill::umma_commit(&ctl->empty[pending_stage]);
                 }
                 __syncwarp();
             };
 
-            for (int b = u.begin; ok && b < u.end; ++b) {
-                key_stage = stage;
-                key_round = round;
+            for (int b = begin; ok && b < end; ++b) {
+                const int key_stage = stage;
+                const unsigned int key_parity = round & 1;
                 if (++stage == p.ring) {
                     stage = 0;
                     ++round;
                 }
-                value_stage = stage;
-                value_round = round;
+                const int value_stage = stage;
+                const unsigned int value_parity = round & 1;
                 if (++stage == p.ring) {
                     stage = 0;
                     ++round;
                 }
-                ok = prefill::mbar_wait_warp(&ctl->full[key_stage], key_round & 1, abort_flag);
+                ok = prefill::mbar_wait_warp(&ctl->full[key_stage], key_parity, abort_flag);
                 if (!ok) break;
-                const int last_tile = takes(u, 1, b) ? 1 : 0;
-                for (int t = 0; ok && t < kTiles; ++t) {
-                    if (!takes(u, t, b)) continue;
+                const bool partial = ctl->partial[info] != 0;
+                const bool takes0 = kTiles == 1 || (alone ? ((b - begin) & 1) == 0 : b < end0);
+                const bool takes1 = kTiles == 2 && (alone ? !takes0 : true);
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) {
+                    if (!ok || !(t == 0 ? takes0 : takes1)) continue;
                     const int slot = kTiles == 2 ? t : b & 1;
                     if (pending_tile >= 0 && pending_slot == slot) {   // its weights lie where these scores go
                         weights_times_values();
                         pending_tile = -1;
-                        if (!ok) break;
+                        if (!ok) continue;
                     }
+                    const bool last = t == 1 || !takes1;
                     prefill::tc_fence_after();
                     if (elect_one()) {
-                        const unsigned int q = smem_u32(queries + (lone(u) ? 0 : t * C::kQueryBytes));
-                        const unsigned int k0 = smem_u32(ring + static_cast<size_t>(key_stage) * C::kTileBytes);
+                        const unsigned long long q =
+                            prefill::umma_desc(queries_at + (alone ? 0 : t * C::kQueryBytes));
+                        const unsigned long long k0 = prefill::umma_desc(ring_at + key_stage * C::kTileBytes);
+                        const unsigned int to = tmem + slot * kBlock;
 #pragma unroll
                         for (int c = 0; c < kChunks; ++c)
 #pragma unroll
                             for (int k = 0; k < 4; ++k)
-                                prefill::umma_bf16(tmem + slot * kBlock, prefill::umma_desc(q + c * kRows * 128) + 2 * k,
-                                                   prefill::umma_desc(k0 + c * kBlock * 128) + 2 * k, kIdescS,
+                                prefill::umma_bf16(to, q + ((c * kRows * 128 >> 4) + 2 * k),
+                                                   k0 + ((c * kBlock * 128 >> 4) + 2 * k), kIdescS,
                                                    (c | k) != 0 ? 1u : 0u);
                         prefill::umma_commit(&ctl->s_full[slot]);
-                        if (t == last_tile) {
+                        if (last) {
                             prefill::umma_commit(&ctl->empty[key_stage]);
-                            if (b == u.end - 1) prefill::umma_commit(&ctl->q_empty);
+                            if (b == end - 1) prefill::umma_commit(&ctl->q_empty);
                         }
                     }
                     __syncwarp();
@@ -531,9 +577,10 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     pending_tile = t;
                     pending_slot = slot;
                     pending_stage = value_stage;
-                    pending_round = value_round;
+                    pending_parity = value_parity;
                     pending_info = info;
-                    pending_last = t == last_tile;
+                    pending_last = last;
+                    pending_partial = partial;
                 }
                 info = (info + 1) % kInfos;
             }
@@ -541,12 +588,13 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         }
     } else if (warp < 4 * kTiles) {
         // ---- softmax and outputs of one query tile: a thread has a row
+        take_registers<kTiles == 2>();
         const int tile = warp >> 2, r = (warp & 3) * 32 + lane;
         const int token = r / group, query = r % group;          // of the tile
         const unsigned int lanes = tmem + (static_cast<unsigned int>((warp & 3) * 32) << 16);
         const unsigned int outputs = lanes + C::kColumnO + tile * D;
         int info = 0;
-        unsigned int steps[2] = {0, 0};                 // of every slot so far
+        unsigned int phase = 0;                         // bit: slot
         unsigned int halves = 0;                        // lone tiles so far
         Split split = {0, 0, 0, 0};
         const bool premultiply = p.scale_log2 <= 0.f;   // the largest score is not that of the largest product
@@ -568,40 +616,36 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             float m = -INFINITY, l = 0.f;
             for (int b = first_block; b < blocks; b += alone ? 2 : 1) {
                 const int slot = kTiles == 2 ? tile : b & 1;
-                ok = ok && prefill::mbar_wait_warp(&ctl->s_full[slot], steps[slot] & 1, abort_flag);
+                ok = ok && prefill::mbar_wait_warp(&ctl->s_full[slot], (phase >> slot) & 1, abort_flag);
                 if (!ok) break;
-                ++steps[slot];
+                phase ^= 1u << slot;
                 prefill::tc_fence_after();
                 const unsigned int scores = lanes + slot * kBlock;
+                const int block_info = (info + b - u.begin) % kInfos;
+                const bool partial = ctl->partial[block_info] != 0 || b * kBlock + kBlock - 1 > first_position;
                 float s[kBlock];
 #pragma unroll
                 for (int c = 0; c < kBlock; c += 32) tmem_load32_async(scores + c, s + c);
-                unsigned int word[kBlock / 32];
-                bool partial = b * kBlock + kBlock - 1 > first_position;
-#pragma unroll
-                for (int w = 0; w < kBlock / 32; ++w) {
-                    word[w] = ctl->mask[(info + b - u.begin) % kInfos][w];
-                    partial |= word[w] != 0xffffffffu;
-                }
                 tmem_wait_load();
                 if (premultiply) {
 #pragma unroll
                     for (int c = 0; c < kBlock; ++c) s[c] *= p.scale_log2;
                 }
-                if (partial) {
+                if (partial) {   // scores that do not count are minus infinity
 #pragma unroll
                     for (int w = 0; w < kBlock / 32; ++w) {
-                        const int seen = position - b * kBlock - w * 32;   // the last key of the word that counts
-                        const unsigned int keep = word[w] & (seen < 0 ? 0u : seen >= 31 ? ~0u : (2u << seen) - 1);
+                        const int last = position - b * kBlock - w * 32;   // the last key of the word that counts
+                        const unsigned int keep =
+                            ctl->mask[block_info][w] & (last < 0 ? 0u : last >= 31 ? ~0u : (2u << last) - 1);
 #pragma unroll
                         for (int c = 0; c < 32; ++c) s[w * 32 + c] = (keep >> c) & 1u ? s[w * 32 + c] : -INFINITY;
                     }
                 }
-                float highest[4] = {s[0], s[1], s[2], s[3]};
+                float highest[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 4; c < kBlock; c += 4)
+                for (int c = 0; c < kBlock; c += 8)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) highest[i] = fmaxf(highest[i], s[c + i]);
+                    for (int i = 0; i < 4; ++i) highest[i] = fmaxf(fmaxf(highest[i], s[c + i]), s[c + 4 + i]);
                 const float now = fmaxf(fmaxf(highest[0], highest[1]), fmaxf(highest[2], highest[3])) * multiplier;
                 if (b == first_block) {
                     m = now;
@@ -614,7 +658,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     // the product before is in the outputs; the one before that is, since these scores are there
                     const int slot_before = kTiles == 2 ? slot : slot ^ 1;
                     ok = prefill::mbar_wait_warp(&ctl->pv_done[slot_before],
-                                                 (steps[slot_before] - (kTiles == 2 ? 2 : 1)) & 1, abort_flag);
+                                                 ((phase >> slot_before) & 1) ^ (kTiles == 2 ? 0 : 1), abort_flag);
                     if (!ok) break;
                     prefill::tc_fence_after();
 #pragma unroll 1
@@ -629,32 +673,38 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     tmem_wait_store();
                 }
                 const float base = (m == -INFINITY ? 0.f : m) - kPromptShift<T>;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const unsigned long long multiplier2 = pair_of(multiplier, multiplier), base2 = pair_of(-base, -base);
+                unsigned long long sum0 = pair_of(0.f, 0.f), sum1 = sum0;
 #pragma unroll
                 for (int c = 0; c < kBlock; c += 32) {
                     unsigned int packed[16];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float x = prefill::exp2_approx(fmaf(s[c + i], multiplier, -base));
-                        const float y = prefill::exp2_approx(fmaf(s[c + i + 1], multiplier, -base));
-                        sum[i & 2] += x;
-                        sum[(i & 2) + 1] += y;
-                        packed[i / 2] = pack_pair<T>(x, y);
+                    for (int i = 0; i < 32; i += 4) {
+                        const unsigned long long e0 = fma_pair(pair_of(s[c + i], s[c + i + 1]), multiplier2, base2);
+                        const unsigned long long e1 = fma_pair(pair_of(s[c + i + 2], s[c + i + 3]), multiplier2, base2);
+                        const float x0 = prefill::exp2_approx(pair_low(e0)), y0 = prefill::exp2_approx(pair_high(e0));
+                        const float x1 = prefill::exp2_approx(pair_low(e1)), y1 = prefill::exp2_approx(pair_high(e1));
+                        sum0 = add_pair(sum0, pair_of(x0, y0));
+                        sum1 = add_pair(sum1, pair_of(x1, y1));
+                        packed[i / 2] = pack_pair<T>(x0, y0);
+                        packed[i / 2 + 1] = pack_pair<T>(x1, y1);
                     }
+                    // weights of 32 keys take 16 columns, of scores that have been read
                     tmem_store16(scores + c / 2, packed);
                 }
                 tmem_wait_store();
                 prefill::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctl->p_full[slot]);
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                sum0 = add_pair(sum0, sum1);
+                l += pair_low(sum0) + pair_high(sum0);
             }
             info = (info + u.end - u.begin) % kInfos;
             // the outputs of the piece
             const bool any = first_block < blocks;
             if (any) {
                 const int slot = kTiles == 2 ? tile : (blocks - 1) & 1;
-                ok = ok && prefill::mbar_wait_warp(&ctl->pv_done[slot], (steps[slot] - 1) & 1, abort_flag);
+                ok = ok && prefill::mbar_wait_warp(&ctl->pv_done[slot], ((phase >> slot) & 1) ^ 1, abort_flag);
                 prefill::tc_fence_after();
             }
             float keep = 1.f, other = 0.f;   // factors of these outputs and of the other half's
@@ -731,14 +781,17 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         }
         if (tid == 0 && p.splits != nullptr)
             *reinterpret_cast<int4*>(p.splits + blockIdx.x) = make_int4(split.request, split.head, split.tile, split.pieces);
-    } else if (p.a.zero_rest != 0 && warp >= 10) {
-        // queries of no request
-        const size_t row = static_cast<size_t>(p.a.heads) * D / 8;
-        int end = 0;
-        for (int r = 0; r < p.a.requests; ++r) end = max(end, requests[r].first + requests[r].tokens);
-        uint4* to = reinterpret_cast<uint4*>(p.a.out) + end * row;
-        const size_t all = (p.a.tokens - end) * row;
-        for (size_t i = blockIdx.x * 64 + (tid - 320); i < all; i += gridDim.x * 64) to[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (p.a.zero_rest != 0) {   // queries of no request
+            const size_t row = static_cast<size_t>(p.a.heads) * D / 8;
+            int end = 0;
+            for (int q = 0; q < p.a.requests; ++q) end = max(end, requests[q].first + requests[q].tokens);
+            uint4* rest = reinterpret_cast<uint4*>(p.a.out) + end * row;
+            const size_t all = (p.a.tokens - end) * row;
+            for (size_t i = blockIdx.x * kTiles * 128 + tid; i < all; i += gridDim.x * kTiles * 128)
+                rest[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+    } else if (warp >= 8) {
+        give_registers<kTiles == 2>();
     }
     if (!ok && lane == 0) {
         *abort_flag = 1;
@@ -840,6 +893,12 @@ cudaError_t launch_prompt(const CUtensorMap& queries, const CUtensorMap& keys, c
         const cudaError_t err = cudaFuncSetAttribute(prompt_attention_kernel<T, D>,
                                                      cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
         if (err != cudaSuccess) return err;
+        if (Config<D>::kTiles == 2) {   // the warps' shares add up to what this build was given, or it does not run
+            cudaFuncAttributes attributes;
+            const cudaError_t known = cudaFuncGetAttributes(&attributes, prompt_attention_kernel<T, D>);
+            if (known != cudaSuccess) return known;
+            if (attributes.numRegs != kLaunchRegisters) return cudaErrorInvalidKernelImage;
+        }
         if (device < 64) configured.fetch_or(1ull << device, std::memory_order_relaxed);
     }
     cudaError_t err = launch_early(prompt_attention_kernel<T, D>, dim3(s.ctas), kThreads, s.smem, 1, stream, queries, keys,
