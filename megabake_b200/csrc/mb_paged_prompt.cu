@@ -46,6 +46,7 @@ template <int D>
 struct Config {
     static constexpr int kBlock = D == 256 ? 64 : 128;       // keys of a block
     static constexpr int kTiles = D == 256 ? 1 : 2;          // query tiles that share it
+    static constexpr int kEarly = kBlock * 3 / 4;            // keys whose weights are handed over before the others'
     static constexpr int kChunks = D / 64;                   // 128-byte columns
     static constexpr int kQueryBytes = kRows * D * 2;        // of one query tile
     static constexpr int kTileBytes = kBlock * D * 2;        // of a block's keys, and of its values
@@ -67,8 +68,8 @@ struct PromptArgs {
 };
 
 struct PromptControl {
-    unsigned long long full[kMaxTiles], empty[kMaxTiles];
-    unsigned long long q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_empty[2];   // [slot], [tile] the last
+    unsigned long long full[kMaxTiles], empty[kMaxTiles], clean[kMaxTiles];
+    unsigned long long q_full, q_empty, s_full[2], p_full[2][2], pv_done[2], o_empty[2];   // [slot], [tile] the last
     unsigned long long half_ready, half_taken;
     float half[kRows][2];        // maximum and sum of the second half of a lone query tile's keys
     unsigned int mask[kInfos][4];
@@ -263,6 +264,19 @@ __device__ __forceinline__ unsigned long long add_pair(unsigned long long a, uns
     return r;
 }
 
+__device__ __forceinline__ void tmem_store8(unsigned int taddr, const unsigned int* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+// What the warp stored in tensor memory goes to the thread that issues products.
+__device__ __forceinline__ void hand_over(unsigned long long* bar, int lane) {
+    tmem_wait_store();
+    prefill::tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+}
+
 template <typename T>
 __device__ __forceinline__ unsigned int pack_pair(float x, float y) {
     if constexpr (std::is_same_v<T, __half>) {
@@ -300,13 +314,15 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
     if (tid == 0) {
         for (int s = 0; s < p.ring; ++s) {
             mbar_init(&ctl->full[s], 1);
-            mbar_init(&ctl->empty[s], 1);
+            mbar_init(&ctl->empty[s], 2);
+            mbar_init(&ctl->clean[s], 1);
         }
         mbar_init(&ctl->q_full, 1);
         mbar_init(&ctl->q_empty, 1);
         for (int s = 0; s < 2; ++s) {
             mbar_init(&ctl->s_full[s], 1);
-            mbar_init(&ctl->p_full[s], 4);
+            mbar_init(&ctl->p_full[s][0], 4);
+            mbar_init(&ctl->p_full[s][1], 4);
             mbar_init(&ctl->pv_done[s], 1);
             mbar_init(&ctl->o_empty[s], 4);
         }
@@ -459,132 +475,160 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             }
         }
     } else if (warp == 9) {
-        // ---- products: the scores of a step are issued before the weights of the step before are waited for.  The warp is
-        // busy with little else than issuing, and what it does between two products is time the tensor core waits: phases
-        // are bits of registers (arrays with an index would be memory), what a block needs is read a step ahead.
+        // ---- products: the scores of a step are issued before the weights of the step before are waited for.  One thread does
+        // it all: what it does between two products is time the tensor core waits (votes and elections of a whole warp
+        // around every wait took {MMA_BEFORE} cycles of a block).  Phases are bits of registers.
+        give_registers<kTiles == 2>();
         constexpr unsigned int kFormat = std::is_same_v<T, __half> ? 0u : (1u << 7) | (1u << 10);
         constexpr unsigned int kIdescS = (1u << 4) | kFormat | (static_cast<unsigned int>(kBlock >> 3) << 17) |
                                          (static_cast<unsigned int>(kRows >> 4) << 24);
         constexpr unsigned int kIdescO = (1u << 4) | kFormat | (1u << 16) | (static_cast<unsigned int>(D >> 3) << 17) |
                                          (static_cast<unsigned int>(kRows >> 4) << 24);
-        give_registers<kTiles == 2>();
-        const unsigned int ring_at = smem_u32(ring), queries_at = smem_u32(queries);
-        int stage = 0, info = 0;
-        unsigned int round = 0, units = 0;
-        unsigned int p_phase = 0;                // bit: slot
-        unsigned int o_phase = 0, o_used = 0;    // bit: query tile
-        for (long long at = run_begin; ok && at < run_end;) {
-            const Piece<kBlock> u(deal, at, run_end);
-            at = u.next;
-            if (u.begin >= u.end) continue;
-            ok = prefill::mbar_wait_warp(&ctl->q_full, units & 1, abort_flag);
-            if (!ok) break;
-            ++units;
-            const bool alone = lone(u);
-            const int end0 = tile_end(u, 0), begin = u.begin, end = u.end;
-            unsigned int fresh = 3;              // bit: no product into the outputs of the tile yet
-            // the step whose scores were issued last
-            int pending_tile = -1, pending_slot = 0, pending_stage = 0, pending_info = 0;
-            unsigned int pending_parity = 0;
-            bool pending_last = false, pending_partial = false;
+        if (elect_one()) {
+            const unsigned int ring_at = smem_u32(ring), queries_at = smem_u32(queries);
+            int stage = 0, info = 0;
+            unsigned int round = 0, units = 0;
+            unsigned int p_phase = 0;                // bit: slot
+            unsigned int o_phase = 0, o_used = 0;    // bit: query tile
+            unsigned int clean_phase = 0;            // bit: stage of the ring
+            for (long long at = run_begin; ok && at < run_end;) {
+                const Piece<kBlock> u(deal, at, run_end);
+                at = u.next;
+                if (u.begin >= u.end) continue;
+                ok = mbar_wait_bounded(&ctl->q_full, units & 1, abort_flag);
+                ++units;
+                const bool alone = lone(u);
+                const int end0 = tile_end(u, 0), begin = u.begin, end = u.end;
+                unsigned int fresh = 3;              // bit: no product into the outputs of the tile yet
+                // the step whose scores were issued last
+                int pending_tile = -1, pending_slot = 0, pending_stage = 0;
+                unsigned int pending_parity = 0;
+                bool pending_first = false, pending_last = false, pending_partial = false;   // first and last of its block
 
-            auto weights_times_values = [&]() {
-                const unsigned int tile_bit = 1u << pending_tile;
-                const bool first = (fresh & tile_bit) != 0;
-                if (first && (o_used & tile_bit)) {   // the outputs before have been taken
-                    ok = prefill::mbar_wait_warp(&ctl->o_empty[pending_tile], (o_phase >> pending_tile) & 1, abort_flag);
-                    o_phase ^= tile_bit;
-                }
-                ok = ok && prefill::mbar_wait_warp(&ctl->full[pending_stage], pending_parity, abort_flag);
-                if (ok && pending_partial) {
-                    // values of keys that do not count may be anything: 0 * NaN is NaN
-                    unsigned char* values = ring + static_cast<size_t>(pending_stage) * C::kTileBytes;
-                    for (int i = lane; i < kBlock * kChunks * 8; i += 32) {
-                        const int row = i >> 3 & (kBlock - 1);
-                        if (!((ctl->mask[pending_info][row >> 5] >> (row & 31)) & 1u))
-                            *reinterpret_cast<uint4*>(values + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                auto weights_times_values = [&]() {
+                    const unsigned int tile_bit = 1u << pending_tile;
+                    const bool first = (fresh & tile_bit) != 0;
+                    if (first && (o_used & tile_bit)) {   // the outputs before have been taken
+                        ok = ok && mbar_wait_bounded(&ctl->o_empty[pending_tile], (o_phase >> pending_tile) & 1, abort_flag);
+                        o_phase ^= tile_bit;
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                }
-                ok = ok && prefill::mbar_wait_warp(&ctl->p_full[pending_slot], (p_phase >> pending_slot) & 1, abort_flag);
-                if (!ok) return;
-                p_phase ^= 1u << pending_slot;
-                fresh &= ~tile_bit;
-                o_used |= tile_bit;
-                prefill::tc_fence_after();
-                if (elect_one()) {
+                    if (pending_first) {
+                        ok = ok && mbar_wait_bounded(&ctl->full[pending_stage], pending_parity, abort_flag);
+                        if (pending_partial) {
+                            ok = ok && mbar_wait_bounded(&ctl->clean[pending_stage], (clean_phase >> pending_stage) & 1,
+                                                         abort_flag);
+                            clean_phase ^= 1u << pending_stage;
+                        }
+                    }
+                    fresh &= ~tile_bit;
+                    o_used |= tile_bit;
                     const unsigned long long v = umma_desc_rows(ring_at + pending_stage * C::kTileBytes, kBlock * 128);
                     const unsigned int to = tmem + C::kColumnO + pending_tile * D, from = tmem + pending_slot * kBlock;
 #pragma unroll
-                    for (int k = 0; k < kBlock / 16; ++k)
-                        umma_from_tmem(to, from + k * 8, v + (k * 16 * 128 >> 4), kIdescO, first && k == 0 ? 0u : 1u);
+                    for (int part = 0; part < 2; ++part) {
+                        ok = ok && mbar_wait_bounded(&ctl->p_full[pending_slot][part], (p_phase >> pending_slot) & 1, abort_flag);
+                        if (!ok) return;
+                        prefill::tc_fence_after();
+#pragma unroll
+                        for (int k = part == 0 ? 0 : C::kEarly / 16; k < (part == 0 ? C::kEarly : kBlock) / 16; ++k)
+                            umma_from_tmem(to, from + k * 8, v + (k * 16 * 128 >> 4), kIdescO, first && k == 0 ? 0u : 1u);
+                    }
+                    p_phase ^= 1u << pending_slot;
                     prefill::umma_commit(&ctl->pv_done[pending_slot]);
                     if (pending_last) prefill::umma_commit(&ctl->empty[pending_stage]);
-                }
-                __syncwarp();
-            };
+                };
 
-            for (int b = begin; ok && b < end; ++b) {
-                const int key_stage = stage;
-                const unsigned int key_parity = round & 1;
-                if (++stage == p.ring) {
-                    stage = 0;
-                    ++round;
-                }
-                const int value_stage = stage;
-                const unsigned int value_parity = round & 1;
-                if (++stage == p.ring) {
-                    stage = 0;
-                    ++round;
-                }
-                ok = prefill::mbar_wait_warp(&ctl->full[key_stage], key_parity, abort_flag);
-                if (!ok) break;
-                const bool partial = ctl->partial[info] != 0;
-                const bool takes0 = kTiles == 1 || (alone ? ((b - begin) & 1) == 0 : b < end0);
-                const bool takes1 = kTiles == 2 && (alone ? !takes0 : true);
-#pragma unroll
-                for (int t = 0; t < kTiles; ++t) {
-                    if (!ok || !(t == 0 ? takes0 : takes1)) continue;
-                    const int slot = kTiles == 2 ? t : b & 1;
-                    if (pending_tile >= 0 && pending_slot == slot) {   // its weights lie where these scores go
-                        weights_times_values();
-                        pending_tile = -1;
-                        if (!ok) continue;
+                for (int b = begin; ok && b < end; ++b) {
+                    const int key_stage = stage;
+                    const unsigned int key_parity = round & 1;
+                    if (++stage == p.ring) {
+                        stage = 0;
+                        ++round;
                     }
-                    const bool last = t == 1 || !takes1;
-                    prefill::tc_fence_after();
-                    if (elect_one()) {
-                        const unsigned long long q =
-                            prefill::umma_desc(queries_at + (alone ? 0 : t * C::kQueryBytes));
+                    const int value_stage = stage;
+                    const unsigned int value_parity = round & 1;
+                    if (++stage == p.ring) {
+                        stage = 0;
+                        ++round;
+                    }
+                    ok = mbar_wait_bounded(&ctl->full[key_stage], key_parity, abort_flag);
+                    const bool partial = ctl->partial[info] != 0;
+                    const bool takes0 = kTiles == 1 || (alone ? ((b - begin) & 1) == 0 : b < end0);
+                    const bool takes1 = kTiles == 2 && (alone ? !takes0 : true);
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) {
+                        if (!ok || !(t == 0 ? takes0 : takes1)) continue;
+                        const int slot = kTiles == 2 ? t : b & 1;
+                        if (pending_tile >= 0 && pending_slot == slot) {   // its weights lie where these scores go
+                            weights_times_values();
+                            pending_tile = -1;
+                            if (!ok) continue;
+                        }
+                        const bool last = t == 1 || !takes1;
+                        const unsigned long long q = prefill::umma_desc(queries_at + (alone ? 0 : t * C::kQueryBytes));
                         const unsigned long long k0 = prefill::umma_desc(ring_at + key_stage * C::kTileBytes);
                         const unsigned int to = tmem + slot * kBlock;
+                        prefill::tc_fence_after();
 #pragma unroll
                         for (int c = 0; c < kChunks; ++c)
 #pragma unroll
                             for (int k = 0; k < 4; ++k)
                                 prefill::umma_bf16(to, q + ((c * kRows * 128 >> 4) + 2 * k),
-                                                   k0 + ((c * kBlock * 128 >> 4) + 2 * k), kIdescS,
-                                                   (c | k) != 0 ? 1u : 0u);
+                                                   k0 + ((c * kBlock * 128 >> 4) + 2 * k), kIdescS, (c | k) != 0 ? 1u : 0u);
                         prefill::umma_commit(&ctl->s_full[slot]);
                         if (last) {
                             prefill::umma_commit(&ctl->empty[key_stage]);
                             if (b == end - 1) prefill::umma_commit(&ctl->q_empty);
                         }
+                        if (pending_tile >= 0) weights_times_values();
+                        pending_tile = t;
+                        pending_slot = slot;
+                        pending_stage = value_stage;
+                        pending_parity = value_parity;
+                        pending_first = t == 0 || !takes0;
+                        pending_last = last;
+                        pending_partial = partial;
+                    }
+                    info = (info + 1) % kInfos;
+                }
+                if (ok && pending_tile >= 0) weights_times_values();
+            }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+    } else if (warp == 10) {
+        // ---- values of keys that do not count may be anything, and 0 * NaN is NaN: where a block has such keys their rows
+        // are zeroed before the product.  Every tile of the ring passes here, so that none is filled again unseen.
+        give_registers<kTiles == 2>();
+        int stage = 0, info = 0;
+        unsigned int round = 0;
+        for (long long at = run_begin; ok && at < run_end;) {
+            const Piece<kBlock> u(deal, at, run_end);
+            at = u.next;
+            for (int b = u.begin; ok && b < u.end; ++b) {
+#pragma unroll
+                for (int kind = 0; kind < 2; ++kind) {
+                    ok = ok && prefill::mbar_wait_warp(&ctl->full[stage], round & 1, abort_flag);
+                    if (!ok) break;
+                    if (kind == 1 && ctl->partial[info] != 0) {
+                        unsigned char* values = ring + static_cast<size_t>(stage) * C::kTileBytes;
+                        for (int i = lane; i < kBlock * kChunks * 8; i += 32) {
+                            const int row = i >> 3 & (kBlock - 1);
+                            if (!((ctl->mask[info][row >> 5] >> (row & 31)) & 1u))
+                                *reinterpret_cast<uint4*>(values + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&ctl->clean[stage]);
                     }
                     __syncwarp();
-                    if (pending_tile >= 0) weights_times_values();
-                    pending_tile = t;
-                    pending_slot = slot;
-                    pending_stage = value_stage;
-                    pending_parity = value_parity;
-                    pending_info = info;
-                    pending_last = last;
-                    pending_partial = partial;
+                    if (lane == 0) mbar_arrive(&ctl->empty[stage]);
+                    if (++stage == p.ring) {
+                        stage = 0;
+                        ++round;
+                    }
                 }
                 info = (info + 1) % kInfos;
             }
-            if (ok && pending_tile >= 0) weights_times_values();
         }
     } else if (warp < 4 * kTiles) {
         // ---- softmax and outputs of one query tile: a thread has a row
@@ -690,12 +734,19 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                         packed[i / 2 + 1] = pack_pair<T>(x1, y1);
                     }
                     // weights of 32 keys take 16 columns, of scores that have been read
-                    tmem_store16(scores + c / 2, packed);
+                    if constexpr (kBlock == 128) {
+                        tmem_store16(scores + c / 2, packed);
+                        if (c + 32 != C::kEarly && c + 32 != kBlock) continue;
+                    } else {   // 48 and 16 keys
+                        tmem_store8(scores + c / 2, packed);
+                        if (c + 32 == kBlock) {
+                            hand_over(&ctl->p_full[slot][0], lane);
+                        }
+                        tmem_store8(scores + c / 2 + 8, packed + 8);
+                        if (c + 32 != kBlock) continue;
+                    }
+                    hand_over(&ctl->p_full[slot][c + 32 == kBlock], lane);
                 }
-                tmem_wait_store();
-                prefill::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&ctl->p_full[slot]);
                 sum0 = add_pair(sum0, sum1);
                 l += pair_low(sum0) + pair_high(sum0);
             }
