@@ -486,6 +486,13 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                                          (static_cast<unsigned int>(kRows >> 4) << 24);
         if (elect_one()) {
             const unsigned int ring_at = smem_u32(ring), queries_at = smem_u32(queries);
+            // the high halves of operand descriptors, and the low ones without the address
+            const unsigned int high = static_cast<unsigned int>(prefill::umma_desc(0) >> 32);
+            const unsigned int low_rows = static_cast<unsigned int>(umma_desc_rows(0, kBlock * 128));
+            const unsigned int low = static_cast<unsigned int>(prefill::umma_desc(0));
+            auto descriptor = [&](unsigned int low_half) {
+                return static_cast<unsigned long long>(high) << 32 | low_half;
+            };
             int stage = 0, info = 0;
             unsigned int round = 0, units = 0;
             unsigned int p_phase = 0;                // bit: slot
@@ -500,98 +507,111 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                 const bool alone = lone(u);
                 const int end0 = tile_end(u, 0), begin = u.begin, end = u.end;
                 unsigned int fresh = 3;              // bit: no product into the outputs of the tile yet
-                // the step whose scores were issued last
-                int pending_tile = -1, pending_slot = 0, pending_stage = 0;
+                // a step is a query tile at a block; `pending` is the one whose scores were issued last
+                int b = begin, t = alone || kTiles == 1 || begin < end0 ? 0 : 1;
+                bool block_open = false;             // the block of the step is there
+                int key_stage = 0, value_stage = 0;
+                unsigned int value_parity = 0;
+                bool partial = false, first_of_block = true;
+                int pending = -1, pending_slot = 0, pending_stage = 0;
                 unsigned int pending_parity = 0;
-                bool pending_first = false, pending_last = false, pending_partial = false;   // first and last of its block
-
-                auto weights_times_values = [&]() {
-                    const unsigned int tile_bit = 1u << pending_tile;
-                    const bool first = (fresh & tile_bit) != 0;
-                    if (first && (o_used & tile_bit)) {   // the outputs before have been taken
-                        ok = ok && mbar_wait_bounded(&ctl->o_empty[pending_tile], (o_phase >> pending_tile) & 1, abort_flag);
-                        o_phase ^= tile_bit;
-                    }
-                    if (pending_first) {
-                        ok = ok && mbar_wait_bounded(&ctl->full[pending_stage], pending_parity, abort_flag);
-                        if (pending_partial) {
-                            ok = ok && mbar_wait_bounded(&ctl->clean[pending_stage], (clean_phase >> pending_stage) & 1,
-                                                         abort_flag);
-                            clean_phase ^= 1u << pending_stage;
+                bool pending_first = false, pending_last = false, pending_partial = false;
+                while (ok && (b < end || pending >= 0)) {
+                    const int slot = kTiles == 2 ? t : b & 1;
+                    // scores go where the weights of the step before lie: those first
+                    const bool scores = b < end && !(pending >= 0 && pending_slot == slot);
+                    const bool last = kTiles == 1 || alone || t == 1;   // of its block
+                    if (scores) {
+                        if (!block_open) {
+                            key_stage = stage;
+                            const unsigned int key_parity = round & 1;
+                            if (++stage == p.ring) {
+                                stage = 0;
+                                ++round;
+                            }
+                            value_stage = stage;
+                            value_parity = round & 1;
+                            if (++stage == p.ring) {
+                                stage = 0;
+                                ++round;
+                            }
+                            ok = mbar_wait_bounded(&ctl->full[key_stage], key_parity, abort_flag);
+                            if (!ok) break;
+                            partial = ctl->partial[info] != 0;
+                            info = (info + 1) % kInfos;
+                            block_open = first_of_block = true;
                         }
-                    }
-                    fresh &= ~tile_bit;
-                    o_used |= tile_bit;
-                    const unsigned long long v = umma_desc_rows(ring_at + pending_stage * C::kTileBytes, kBlock * 128);
-                    const unsigned int to = tmem + C::kColumnO + pending_tile * D, from = tmem + pending_slot * kBlock;
-#pragma unroll
-                    for (int part = 0; part < 2; ++part) {
-                        ok = ok && mbar_wait_bounded(&ctl->p_full[pending_slot][part], (p_phase >> pending_slot) & 1, abort_flag);
-                        if (!ok) return;
-                        prefill::tc_fence_after();
-#pragma unroll
-                        for (int k = part == 0 ? 0 : C::kEarly / 16; k < (part == 0 ? C::kEarly : kBlock) / 16; ++k)
-                            umma_from_tmem(to, from + k * 8, v + (k * 16 * 128 >> 4), kIdescO, first && k == 0 ? 0u : 1u);
-                    }
-                    p_phase ^= 1u << pending_slot;
-                    prefill::umma_commit(&ctl->pv_done[pending_slot]);
-                    if (pending_last) prefill::umma_commit(&ctl->empty[pending_stage]);
-                };
-
-                for (int b = begin; ok && b < end; ++b) {
-                    const int key_stage = stage;
-                    const unsigned int key_parity = round & 1;
-                    if (++stage == p.ring) {
-                        stage = 0;
-                        ++round;
-                    }
-                    const int value_stage = stage;
-                    const unsigned int value_parity = round & 1;
-                    if (++stage == p.ring) {
-                        stage = 0;
-                        ++round;
-                    }
-                    ok = mbar_wait_bounded(&ctl->full[key_stage], key_parity, abort_flag);
-                    const bool partial = ctl->partial[info] != 0;
-                    const bool takes0 = kTiles == 1 || (alone ? ((b - begin) & 1) == 0 : b < end0);
-                    const bool takes1 = kTiles == 2 && (alone ? !takes0 : true);
-#pragma unroll
-                    for (int t = 0; t < kTiles; ++t) {
-                        if (!ok || !(t == 0 ? takes0 : takes1)) continue;
-                        const int slot = kTiles == 2 ? t : b & 1;
-                        if (pending_tile >= 0 && pending_slot == slot) {   // its weights lie where these scores go
-                            weights_times_values();
-                            pending_tile = -1;
-                            if (!ok) continue;
-                        }
-                        const bool last = t == 1 || !takes1;
-                        const unsigned long long q = prefill::umma_desc(queries_at + (alone ? 0 : t * C::kQueryBytes));
-                        const unsigned long long k0 = prefill::umma_desc(ring_at + key_stage * C::kTileBytes);
+                        const unsigned int q = low + ((queries_at + (alone ? 0 : t * C::kQueryBytes)) >> 4);
+                        const unsigned int k0 = low + ((ring_at + key_stage * C::kTileBytes) >> 4);
                         const unsigned int to = tmem + slot * kBlock;
                         prefill::tc_fence_after();
 #pragma unroll
                         for (int c = 0; c < kChunks; ++c)
 #pragma unroll
                             for (int k = 0; k < 4; ++k)
-                                prefill::umma_bf16(to, q + ((c * kRows * 128 >> 4) + 2 * k),
-                                                   k0 + ((c * kBlock * 128 >> 4) + 2 * k), kIdescS, (c | k) != 0 ? 1u : 0u);
+                                prefill::umma_bf16(to, descriptor(q + (c * kRows * 128 >> 4) + 2 * k),
+                                                   descriptor(k0 + (c * kBlock * 128 >> 4) + 2 * k), kIdescS,
+                                                   (c | k) != 0 ? 1u : 0u);
                         prefill::umma_commit(&ctl->s_full[slot]);
                         if (last) {
                             prefill::umma_commit(&ctl->empty[key_stage]);
                             if (b == end - 1) prefill::umma_commit(&ctl->q_empty);
                         }
-                        if (pending_tile >= 0) weights_times_values();
-                        pending_tile = t;
+                    }
+                    if (pending >= 0) {   // weights times values
+                        const unsigned int tile_bit = 1u << pending;
+                        const bool first = (fresh & tile_bit) != 0;
+                        if (first && (o_used & tile_bit)) {   // the outputs before have been taken
+                            ok = mbar_wait_bounded(&ctl->o_empty[pending], (o_phase >> pending) & 1, abort_flag);
+                            o_phase ^= tile_bit;
+                        }
+                        if (pending_first) {
+                            ok = ok && mbar_wait_bounded(&ctl->full[pending_stage], pending_parity, abort_flag);
+                            if (pending_partial) {
+                                ok = ok && mbar_wait_bounded(&ctl->clean[pending_stage],
+                                                             (clean_phase >> pending_stage) & 1, abort_flag);
+                                clean_phase ^= 1u << pending_stage;
+                            }
+                        }
+                        fresh &= ~tile_bit;
+                        o_used |= tile_bit;
+                        const unsigned int v = low_rows + ((ring_at + pending_stage * C::kTileBytes) >> 4);
+                        const unsigned int to = tmem + C::kColumnO + pending * D, from = tmem + pending_slot * kBlock;
+#pragma unroll
+                        for (int part = 0; part < 2; ++part) {
+                            ok = ok &&
+                                 mbar_wait_bounded(&ctl->p_full[pending_slot][part], (p_phase >> pending_slot) & 1, abort_flag);
+                            if (!ok) break;
+                            prefill::tc_fence_after();
+#pragma unroll
+                            for (int k = part == 0 ? 0 : C::kEarly / 16; k < (part == 0 ? C::kEarly : kBlock) / 16; ++k)
+                                umma_from_tmem(to, from + k * 8, descriptor(v + (k * 16 * 128 >> 4)), kIdescO,
+                                               first && k == 0 ? 0u : 1u);
+                        }
+                        if (!ok) break;
+                        p_phase ^= 1u << pending_slot;
+                        prefill::umma_commit(&ctl->pv_done[pending_slot]);
+                        if (pending_last) prefill::umma_commit(&ctl->empty[pending_stage]);
+                        pending = -1;
+                    }
+                    if (scores) {
+                        pending = t;
                         pending_slot = slot;
                         pending_stage = value_stage;
                         pending_parity = value_parity;
-                        pending_first = t == 0 || !takes0;
+                        pending_first = first_of_block;
                         pending_last = last;
                         pending_partial = partial;
+                        first_of_block = false;
+                        if (last) {
+                            ++b;
+                            block_open = false;
+                            t = kTiles == 1 ? 0 : alone ? t ^ 1 : b < end0 ? 0 : 1;
+                        } else {
+                            t = 1;
+                        }
                     }
-                    info = (info + 1) % kInfos;
                 }
-                if (ok && pending_tile >= 0) weights_times_values();
             }
         }
         ok = __all_sync(0xffffffffu, ok);
