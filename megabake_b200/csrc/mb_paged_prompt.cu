@@ -21,14 +21,10 @@ namespace paged {
 namespace {
 
 constexpr int kRows = 128;             // of a query tile: tokens times the query heads of a key head
-// 4 + 4 softmax warps, one that copies, one that issues products, and two that fill their warpgroup: the softmax warps
-// take registers from it (a row's 128 scores stay in registers; read twice from tensor memory instead, a block took
-// 5,500 cycles, not 4,400).
-constexpr int kThreads = 384;
-constexpr int kLaunchRegisters = 168, kSoftmaxRegisters = 200, kOtherRegisters = 104;
-static_assert(2 * kSoftmaxRegisters + kOtherRegisters == 3 * kLaunchRegisters, "no more than the block was launched with");
+constexpr int kThreads = 384;          // 4 + 4 softmax warps, one that copies, two that issue products, one that cleans
+constexpr int kBlock = 64;             // keys of a block
 constexpr int kMaxTiles = 12;          // of the ring: keys and values in turn
-constexpr int kInfos = 8;              // blocks whose masks are kept
+constexpr int kInfos = 16;             // blocks whose masks are kept
 constexpr int kSmemLimit = 227 * 1024;
 constexpr int kTileCost = 128;         // what a unit costs besides its keys, in keys
 constexpr int kLeastKeys = 512;        // of a run
@@ -44,13 +40,11 @@ constexpr float kPromptShift<__nv_bfloat16> = -39.f;
 
 template <int D>
 struct Config {
-    static constexpr int kBlock = D == 256 ? 64 : 128;       // keys of a block
-    static constexpr int kTiles = D == 256 ? 1 : 2;          // query tiles that share it
-    static constexpr int kEarly = kBlock * 3 / 4;            // keys whose weights are handed over before the others'
+    static constexpr int kTiles = D == 256 ? 1 : 2;          // query tiles that share a block
     static constexpr int kChunks = D / 64;                   // 128-byte columns
     static constexpr int kQueryBytes = kRows * D * 2;        // of one query tile
     static constexpr int kTileBytes = kBlock * D * 2;        // of a block's keys, and of its values
-    static constexpr int kColumnO = 2 * kBlock;              // tensor memory: two score buffers, then the outputs
+    static constexpr int kColumnO = 2 * kTiles * kBlock;     // tensor memory: two slots of scores a tile, then the outputs
 };
 
 struct Split {
@@ -69,10 +63,10 @@ struct PromptArgs {
 
 struct PromptControl {
     unsigned long long full[kMaxTiles], empty[kMaxTiles], clean[kMaxTiles];
-    unsigned long long q_full, q_empty, s_full[2], p_full[2][2], pv_done[2], o_empty[2];   // [slot], [tile] the last
+    unsigned long long q_full, q_empty, s_full[4], p_full[4], pv_done[4], o_empty[2];   // [slot], [tile] the last
     unsigned long long half_ready, half_taken;
     float half[kRows][2];        // maximum and sum of the second half of a lone query tile's keys
-    unsigned int mask[kInfos][4];
+    unsigned int mask[kInfos][2];
     int partial[kInfos];         // not every key of the block counts
     long long warp_sums[kThreads / 32];
     unsigned int tmem;
@@ -108,7 +102,6 @@ __device__ __forceinline__ long long request_length(const Request& q, int unit_t
     return length_before(q, unit_tokens, units - 1) + max(q.length - q.tokens, 0) + q.tokens + kTileCost;
 }
 
-template <int kBlock>
 struct Piece {
     int request, head, tile;
     int begin, end, blocks;      // blocks of this piece, and of the unit
@@ -163,10 +156,9 @@ struct Piece {
 };
 
 // The first end or begin of a unit from `at` on.
-template <int kBlock>
 __device__ __forceinline__ long long unit_boundary(const Deal& d, long long at) {
     if (at >= d.total) return at;
-    const Piece<kBlock> u(d, at, d.total);
+    const Piece u(d, at, d.total);
     return u.at_start ? at : u.unit_end;
 }
 
@@ -233,16 +225,6 @@ __device__ __forceinline__ void tmem_store16(unsigned int taddr, const unsigned 
         : "memory");
 }
 
-// Where every warp of a warpgroup passes; 256-wide heads get by with what they were launched with.
-template <bool kUsed>
-__device__ __forceinline__ void take_registers() {
-    if constexpr (kUsed) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
-}
-template <bool kUsed>
-__device__ __forceinline__ void give_registers() {
-    if constexpr (kUsed) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
-}
-
 // Two floats in a 64-bit register, for instructions that work on both.
 __device__ __forceinline__ unsigned long long pair_of(float x, float y) {
     unsigned long long r;
@@ -264,19 +246,6 @@ __device__ __forceinline__ unsigned long long add_pair(unsigned long long a, uns
     return r;
 }
 
-__device__ __forceinline__ void tmem_store8(unsigned int taddr, const unsigned int* r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
-                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                 : "memory");
-}
-// What the warp stored in tensor memory goes to the thread that issues products.
-__device__ __forceinline__ void hand_over(unsigned long long* bar, int lane) {
-    tmem_wait_store();
-    prefill::tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bar);
-}
-
 template <typename T>
 __device__ __forceinline__ unsigned int pack_pair(float x, float y) {
     if constexpr (std::is_same_v<T, __half>) {
@@ -288,19 +257,20 @@ __device__ __forceinline__ unsigned int pack_pair(float x, float y) {
 }
 
 // ---------------------------------------------------------------------------------------
-// The kernel.  Two query tiles of 128 rows (tokens x the query heads of a key head) share every block of 128 keys:
-// while the softmax warps of one tile work on its scores, the tensor core multiplies for the other.  Scores come out in
-// tensor memory, weights go back there as 16-bit numbers over the scores they were made of and are the first
-// operand of the second product, values are taken as they lie in the pages (rows are the reduction).  A thread has a
-// row: no shuffles.  Outputs stay in tensor memory and are rescaled only when a row's maximum has grown by
-// more than 2^8 since the last time.  256-wide heads: one query tile, blocks of 64 keys, whose scores have two buffers.
+// The kernel.  Two query tiles of 128 rows (tokens x the query heads of a key head) share every block of 64 keys, and
+// every tile has two slots of scores in tensor memory: while its softmax warps work on one block, the scores of the
+// next are there or under way, and the tensor core multiplies for both tiles.  Weights go back to tensor memory as
+// 16-bit numbers over the scores they were made of and are the first operand of the second product, values are taken
+// as they lie in the pages (rows are the reduction).  A thread has a row: no shuffles.  Outputs stay in tensor
+// memory and are rescaled only when a row's maximum has grown by more than 2^8 since the last time.  256-wide
+// heads: one query tile.
 // ---------------------------------------------------------------------------------------
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __grid_constant__ CUtensorMap key_map,
                         const __grid_constant__ CUtensorMap value_map, const __grid_constant__ PromptArgs p) {
     using C = Config<D>;
-    constexpr int kBlock = C::kBlock, kTiles = C::kTiles, kChunks = C::kChunks;
+    constexpr int kTiles = C::kTiles, kChunks = C::kChunks;
     extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char* queries = smem;                                   // [tiles][chunks][128 rows][128 bytes]
     unsigned char* ring = queries + kTiles * C::kQueryBytes;         // [ring][chunks][block rows][128 bytes]
@@ -314,24 +284,24 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
     if (tid == 0) {
         for (int s = 0; s < p.ring; ++s) {
             mbar_init(&ctl->full[s], 1);
-            mbar_init(&ctl->empty[s], 2);
+            mbar_init(&ctl->empty[s], kTiles + 1);
             mbar_init(&ctl->clean[s], 1);
         }
         mbar_init(&ctl->q_full, 1);
-        mbar_init(&ctl->q_empty, 1);
-        for (int s = 0; s < 2; ++s) {
+        mbar_init(&ctl->q_empty, kTiles);
+        for (int s = 0; s < 4; ++s) {
             mbar_init(&ctl->s_full[s], 1);
-            mbar_init(&ctl->p_full[s][0], 4);
-            mbar_init(&ctl->p_full[s][1], 4);
+            mbar_init(&ctl->p_full[s], 4);
             mbar_init(&ctl->pv_done[s], 1);
-            mbar_init(&ctl->o_empty[s], 4);
         }
+        mbar_init(&ctl->o_empty[0], 4);
+        mbar_init(&ctl->o_empty[1], 4);
         mbar_init(&ctl->half_ready, 4);
         mbar_init(&ctl->half_taken, 4);
         ctl->abort_flag = 0;
         mbar_init_fence();
     }
-    if (warp == 9) prefill::tmem_alloc(&ctl->tmem, kTmemColumns);
+    if (warp == 11) prefill::tmem_alloc(&ctl->tmem, kTmemColumns);
     prefill::tc_fence_before();
     __syncthreads();
     prefill::tc_fence_after();
@@ -378,30 +348,29 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
     long long run_begin = min(blockIdx.x * deal.per, deal.total);
     long long run_end = min(run_begin + deal.per, deal.total);
     if (p.splits == nullptr) {   // no unit is cut: runs go from unit to unit
-        run_begin = unit_boundary<kBlock>(deal, run_begin);
-        run_end = unit_boundary<kBlock>(deal, run_end);
+        run_begin = unit_boundary(deal, run_begin);
+        run_end = unit_boundary(deal, run_end);
     }
     volatile int* abort_flag = &ctl->abort_flag;
     bool ok = true;
 
     // A unit of two query tiles: each takes the blocks up to the one its last query lies in.  A lone tile of a pair takes
     // the place of both, which share its blocks in turn and meet at the end.
-    auto lone = [&](const Piece<kBlock>& u) { return kTiles == 1 || u.tokens <= p.tile_tokens; };
-    auto tile_end = [&](const Piece<kBlock>& u, int t) {
+    auto lone = [&](const Piece& u) { return kTiles == 1 || u.tokens <= p.tile_tokens; };
+    auto tile_end = [&](const Piece& u, int t) {
         if (t == 1 || lone(u)) return u.end;
         return min(max((u.position + p.tile_tokens + kBlock - 1) / kBlock, 1), u.end);
     };
 
     if (warp == 8) {
         // ---- copies
-        give_registers<kTiles == 2>();
         int stage = 0, info = 0;
         unsigned int round = 0, units = 0;
         const int rows = min(page, kBlock);
         const int per_block = kBlock / rows;
         const int batch = 32 / per_block;
         for (long long at = run_begin; ok && at < run_end;) {
-            const Piece<kBlock> u(deal, at, run_end);
+            const Piece u(deal, at, run_end);
             at = u.next;
             if (u.begin >= u.end) continue;
             if (units > 0) ok = prefill::mbar_wait_warp(&ctl->q_empty, (units - 1) & 1, abort_flag);
@@ -474,155 +443,117 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                 }
             }
         }
-    } else if (warp == 9) {
-        // ---- products: the scores of a step are issued before the weights of the step before are waited for.  One thread does
-        // it all: what it does between two products is time the tensor core waits (votes and elections of a whole warp
-        // around every wait took {MMA_BEFORE} cycles of a block).  Phases are bits of registers.
-        give_registers<kTiles == 2>();
+    } else if (warp == 9 || (kTiles == 2 && warp == 10)) {
+        // ---- products of one query tile.  One thread issues them, in one place for the scores and one for the outputs: what
+        // it does between two products is time the tensor core waits, unless the other tile's thread has something for
+        // it ({MMA_NOTE}).
         constexpr unsigned int kFormat = std::is_same_v<T, __half> ? 0u : (1u << 7) | (1u << 10);
         constexpr unsigned int kIdescS = (1u << 4) | kFormat | (static_cast<unsigned int>(kBlock >> 3) << 17) |
                                          (static_cast<unsigned int>(kRows >> 4) << 24);
         constexpr unsigned int kIdescO = (1u << 4) | kFormat | (1u << 16) | (static_cast<unsigned int>(D >> 3) << 17) |
                                          (static_cast<unsigned int>(kRows >> 4) << 24);
         if (elect_one()) {
+            const int tile = warp - 9;
             const unsigned int ring_at = smem_u32(ring), queries_at = smem_u32(queries);
-            // the high halves of operand descriptors, and the low ones without the address
+            // the high half of operand descriptors, and the low ones without the address
             const unsigned int high = static_cast<unsigned int>(prefill::umma_desc(0) >> 32);
             const unsigned int low_rows = static_cast<unsigned int>(umma_desc_rows(0, kBlock * 128));
             const unsigned int low = static_cast<unsigned int>(prefill::umma_desc(0));
             auto descriptor = [&](unsigned int low_half) {
                 return static_cast<unsigned long long>(high) << 32 | low_half;
             };
-            int stage = 0, info = 0;
-            unsigned int round = 0, units = 0;
+            const unsigned int slots = tmem + tile * 2 * kBlock, outputs = tmem + C::kColumnO + tile * D;
+            int key_stage = 0, value_stage = 1, info = 0;    // of the next block
+            unsigned int key_round = 0, value_round = 0, units = 0, outputs_used = 0;
+            auto advance = [&](int& stage, unsigned int& round) {
+                stage += 2;
+                if (stage >= p.ring) {
+                    stage -= p.ring;
+                    ++round;
+                }
+            };
             unsigned int p_phase = 0;                // bit: slot
-            unsigned int o_phase = 0, o_used = 0;    // bit: query tile
             unsigned int clean_phase = 0;            // bit: stage of the ring
             for (long long at = run_begin; ok && at < run_end;) {
-                const Piece<kBlock> u(deal, at, run_end);
+                const Piece u(deal, at, run_end);
                 at = u.next;
                 if (u.begin >= u.end) continue;
                 ok = mbar_wait_bounded(&ctl->q_full, units & 1, abort_flag);
                 ++units;
-                const bool alone = lone(u);
-                const int end0 = tile_end(u, 0), begin = u.begin, end = u.end;
-                unsigned int fresh = 3;              // bit: no product into the outputs of the tile yet
-                // a step is a query tile at a block; `pending` is the one whose scores were issued last
-                int b = begin, t = alone || kTiles == 1 || begin < end0 ? 0 : 1;
-                bool block_open = false;             // the block of the step is there
-                int key_stage = 0, value_stage = 0;
-                unsigned int value_parity = 0;
-                bool partial = false, first_of_block = true;
-                int pending = -1, pending_slot = 0, pending_stage = 0;
-                unsigned int pending_parity = 0;
-                bool pending_first = false, pending_last = false, pending_partial = false;
-                while (ok && (b < end || pending >= 0)) {
-                    const int slot = kTiles == 2 ? t : b & 1;
-                    // scores go where the weights of the step before lie: those first
-                    const bool scores = b < end && !(pending >= 0 && pending_slot == slot);
-                    const bool last = kTiles == 1 || alone || t == 1;   // of its block
-                    if (scores) {
-                        if (!block_open) {
-                            key_stage = stage;
-                            const unsigned int key_parity = round & 1;
-                            if (++stage == p.ring) {
-                                stage = 0;
-                                ++round;
+                const bool alone = kTiles == 2 && lone(u);
+                const int begin = u.begin, end = u.end, tile_stop = tile_end(u, tile);
+                auto takes = [&](int b) { return alone ? ((b - begin) & 1) == tile : b < tile_stop; };
+                const unsigned int q = low + ((queries_at + (alone ? 0 : tile * C::kQueryBytes)) >> 4);
+                int bs = begin, bv = begin;          // blocks whose scores, and whose products with values, come next
+                unsigned int scored = 0, done = 0;   // steps
+                while (ok && bv < end) {
+                    if (bs < end && scored - done < 2) {
+                        // scores go where the weights of two steps ago were; not waited for while there is something to do
+                        const bool idle = bs == bv;
+                        if (idle ? ok = mbar_wait_bounded(&ctl->full[key_stage], key_round & 1, abort_flag)
+                                 : mbar_try_wait(&ctl->full[key_stage], key_round & 1)) {
+                            if (takes(bs)) {
+                                const int slot = scored & 1;
+                                const unsigned int k0 = low + ((ring_at + key_stage * C::kTileBytes) >> 4);
+                                prefill::tc_fence_after();
+#pragma unroll
+                                for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k)
+                                        prefill::umma_bf16(slots + slot * kBlock, descriptor(q + (c * kRows * 128 >> 4) + 2 * k),
+                                                           descriptor(k0 + (c * kBlock * 128 >> 4) + 2 * k), kIdescS,
+                                                           (c | k) != 0 ? 1u : 0u);
+                                prefill::umma_commit(&ctl->s_full[tile * 2 + slot]);
+                                prefill::umma_commit(&ctl->empty[key_stage]);
+                                ++scored;
+                            } else {
+                                mbar_arrive(&ctl->empty[key_stage]);
                             }
-                            value_stage = stage;
-                            value_parity = round & 1;
-                            if (++stage == p.ring) {
-                                stage = 0;
-                                ++round;
-                            }
-                            ok = mbar_wait_bounded(&ctl->full[key_stage], key_parity, abort_flag);
-                            if (!ok) break;
-                            partial = ctl->partial[info] != 0;
-                            info = (info + 1) % kInfos;
-                            block_open = first_of_block = true;
-                        }
-                        const unsigned int q = low + ((queries_at + (alone ? 0 : t * C::kQueryBytes)) >> 4);
-                        const unsigned int k0 = low + ((ring_at + key_stage * C::kTileBytes) >> 4);
-                        const unsigned int to = tmem + slot * kBlock;
-                        prefill::tc_fence_after();
-#pragma unroll
-                        for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                prefill::umma_bf16(to, descriptor(q + (c * kRows * 128 >> 4) + 2 * k),
-                                                   descriptor(k0 + (c * kBlock * 128 >> 4) + 2 * k), kIdescS,
-                                                   (c | k) != 0 ? 1u : 0u);
-                        prefill::umma_commit(&ctl->s_full[slot]);
-                        if (last) {
-                            prefill::umma_commit(&ctl->empty[key_stage]);
-                            if (b == end - 1) prefill::umma_commit(&ctl->q_empty);
-                        }
-                    }
-                    if (pending >= 0) {   // weights times values
-                        const unsigned int tile_bit = 1u << pending;
-                        const bool first = (fresh & tile_bit) != 0;
-                        if (first && (o_used & tile_bit)) {   // the outputs before have been taken
-                            ok = mbar_wait_bounded(&ctl->o_empty[pending], (o_phase >> pending) & 1, abort_flag);
-                            o_phase ^= tile_bit;
-                        }
-                        if (pending_first) {
-                            ok = ok && mbar_wait_bounded(&ctl->full[pending_stage], pending_parity, abort_flag);
-                            if (pending_partial) {
-                                ok = ok && mbar_wait_bounded(&ctl->clean[pending_stage],
-                                                             (clean_phase >> pending_stage) & 1, abort_flag);
-                                clean_phase ^= 1u << pending_stage;
-                            }
-                        }
-                        fresh &= ~tile_bit;
-                        o_used |= tile_bit;
-                        const unsigned int v = low_rows + ((ring_at + pending_stage * C::kTileBytes) >> 4);
-                        const unsigned int to = tmem + C::kColumnO + pending * D, from = tmem + pending_slot * kBlock;
-#pragma unroll
-                        for (int part = 0; part < 2; ++part) {
-                            ok = ok &&
-                                 mbar_wait_bounded(&ctl->p_full[pending_slot][part], (p_phase >> pending_slot) & 1, abort_flag);
-                            if (!ok) break;
-                            prefill::tc_fence_after();
-#pragma unroll
-                            for (int k = part == 0 ? 0 : C::kEarly / 16; k < (part == 0 ? C::kEarly : kBlock) / 16; ++k)
-                                umma_from_tmem(to, from + k * 8, descriptor(v + (k * 16 * 128 >> 4)), kIdescO,
-                                               first && k == 0 ? 0u : 1u);
+                            advance(key_stage, key_round);
+                            if (++bs == end) prefill::umma_commit(&ctl->q_empty);
+                            continue;
                         }
                         if (!ok) break;
-                        p_phase ^= 1u << pending_slot;
-                        prefill::umma_commit(&ctl->pv_done[pending_slot]);
-                        if (pending_last) prefill::umma_commit(&ctl->empty[pending_stage]);
-                        pending = -1;
                     }
-                    if (scores) {
-                        pending = t;
-                        pending_slot = slot;
-                        pending_stage = value_stage;
-                        pending_parity = value_parity;
-                        pending_first = first_of_block;
-                        pending_last = last;
-                        pending_partial = partial;
-                        first_of_block = false;
-                        if (last) {
-                            ++b;
-                            block_open = false;
-                            t = kTiles == 1 ? 0 : alone ? t ^ 1 : b < end0 ? 0 : 1;
-                        } else {
-                            t = 1;
+                    ok = mbar_wait_bounded(&ctl->full[value_stage], value_round & 1, abort_flag);
+                    if (ok && takes(bv)) {
+                        const int slot = done & 1;
+                        if (done == 0 && outputs_used++ > 0)   // the outputs before have been taken
+                            ok = mbar_wait_bounded(&ctl->o_empty[tile], outputs_used & 1, abort_flag);
+                        if (ok && ctl->partial[info] != 0) {
+                            ok = mbar_wait_bounded(&ctl->clean[value_stage], (clean_phase >> value_stage) & 1, abort_flag);
+                            clean_phase ^= 1u << value_stage;
                         }
+                        ok = ok && mbar_wait_bounded(&ctl->p_full[tile * 2 + slot], (p_phase >> slot) & 1, abort_flag);
+                        if (!ok) break;
+                        p_phase ^= 1u << slot;
+                        prefill::tc_fence_after();
+                        const unsigned int v = low_rows + ((ring_at + value_stage * C::kTileBytes) >> 4);
+#pragma unroll
+                        for (int k = 0; k < kBlock / 16; ++k)
+                            umma_from_tmem(outputs, slots + slot * kBlock + k * 8, descriptor(v + (k * 16 * 128 >> 4)), kIdescO,
+                                           done == 0 && k == 0 ? 0u : 1u);
+                        prefill::umma_commit(&ctl->pv_done[tile * 2 + slot]);
+                        prefill::umma_commit(&ctl->empty[value_stage]);
+                        ++done;
+                    } else if (ok) {
+                        if (ctl->partial[info] != 0) clean_phase ^= 1u << value_stage;
+                        mbar_arrive(&ctl->empty[value_stage]);
                     }
+                    advance(value_stage, value_round);
+                    info = (info + 1) % kInfos;
+                    ++bv;
                 }
             }
         }
         ok = __all_sync(0xffffffffu, ok);
-    } else if (warp == 10) {
+    } else if (warp == 11) {
         // ---- values of keys that do not count may be anything, and 0 * NaN is NaN: where a block has such keys their rows
         // are zeroed before the product.  Every tile of the ring passes here, so that none is filled again unseen.
-        give_registers<kTiles == 2>();
         int stage = 0, info = 0;
         unsigned int round = 0;
         for (long long at = run_begin; ok && at < run_end;) {
-            const Piece<kBlock> u(deal, at, run_end);
+            const Piece u(deal, at, run_end);
             at = u.next;
             for (int b = u.begin; ok && b < u.end; ++b) {
 #pragma unroll
@@ -652,7 +583,6 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         }
     } else if (warp < 4 * kTiles) {
         // ---- softmax and outputs of one query tile: a thread has a row
-        take_registers<kTiles == 2>();
         const int tile = warp >> 2, r = (warp & 3) * 32 + lane;
         const int token = r / group, query = r % group;          // of the tile
         const unsigned int lanes = tmem + (static_cast<unsigned int>((warp & 3) * 32) << 16);
@@ -664,7 +594,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         const bool premultiply = p.scale_log2 <= 0.f;   // the largest score is not that of the largest product
         const float multiplier = premultiply ? 1.f : p.scale_log2;
         for (long long at = run_begin; at < run_end;) {
-            const Piece<kBlock> u(deal, at, run_end);
+            const Piece u(deal, at, run_end);
             at = u.next;
             const int slot_out = (blockIdx.x * 2 + (u.begin == 0 && u.end > 0 ? 1 : 0)) * kTiles * kRows + tile * kRows + r;
             if (u.begin >= u.end) {
@@ -678,8 +608,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             const int mine = own * p.tile_tokens + token;        // token of the unit
             const int position = u.position + mine, first_position = u.position + own * p.tile_tokens;
             float m = -INFINITY, l = 0.f;
-            for (int b = first_block; b < blocks; b += alone ? 2 : 1) {
-                const int slot = kTiles == 2 ? tile : b & 1;
+            unsigned int step = 0;
+            for (int b = first_block; b < blocks; b += alone ? 2 : 1, ++step) {
+                const int slot = tile * 2 + (step & 1);
                 ok = ok && prefill::mbar_wait_warp(&ctl->s_full[slot], (phase >> slot) & 1, abort_flag);
                 if (!ok) break;
                 phase ^= 1u << slot;
@@ -720,9 +651,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     m = grown;
                     l *= factor;
                     // the product before is in the outputs; the one before that is, since these scores are there
-                    const int slot_before = kTiles == 2 ? slot : slot ^ 1;
-                    ok = prefill::mbar_wait_warp(&ctl->pv_done[slot_before],
-                                                 ((phase >> slot_before) & 1) ^ (kTiles == 2 ? 0 : 1), abort_flag);
+                    ok = prefill::mbar_wait_warp(&ctl->pv_done[slot ^ 1], ((phase >> (slot ^ 1)) & 1) ^ 1, abort_flag);
                     if (!ok) break;
                     prefill::tc_fence_after();
 #pragma unroll 1
@@ -754,19 +683,12 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                         packed[i / 2 + 1] = pack_pair<T>(x1, y1);
                     }
                     // weights of 32 keys take 16 columns, of scores that have been read
-                    if constexpr (kBlock == 128) {
-                        tmem_store16(scores + c / 2, packed);
-                        if (c + 32 != C::kEarly && c + 32 != kBlock) continue;
-                    } else {   // 48 and 16 keys
-                        tmem_store8(scores + c / 2, packed);
-                        if (c + 32 == kBlock) {
-                            hand_over(&ctl->p_full[slot][0], lane);
-                        }
-                        tmem_store8(scores + c / 2 + 8, packed + 8);
-                        if (c + 32 != kBlock) continue;
-                    }
-                    hand_over(&ctl->p_full[slot][c + 32 == kBlock], lane);
+                    tmem_store16(scores + c / 2, packed);
                 }
+                tmem_wait_store();
+                prefill::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl->p_full[slot]);
                 sum0 = add_pair(sum0, sum1);
                 l += pair_low(sum0) + pair_high(sum0);
             }
@@ -774,7 +696,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             // the outputs of the piece
             const bool any = first_block < blocks;
             if (any) {
-                const int slot = kTiles == 2 ? tile : (blocks - 1) & 1;
+                const int slot = tile * 2 + ((step - 1) & 1);
                 ok = ok && prefill::mbar_wait_warp(&ctl->pv_done[slot], ((phase >> slot) & 1) ^ 1, abort_flag);
                 prefill::tc_fence_after();
             }
@@ -861,8 +783,6 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             for (size_t i = blockIdx.x * kTiles * 128 + tid; i < all; i += gridDim.x * kTiles * 128)
                 rest[i] = make_uint4(0u, 0u, 0u, 0u);
         }
-    } else if (warp >= 8) {
-        give_registers<kTiles == 2>();
     }
     if (!ok && lane == 0) {
         *abort_flag = 1;
@@ -875,7 +795,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         while (global_timer_ns() - start < 200000ull) __nanosleep(1000);
         __syncthreads();
     }
-    if (warp == 9) prefill::tmem_dealloc(tmem, kTmemColumns);
+    if (warp == 11) prefill::tmem_dealloc(tmem, kTmemColumns);
 }
 
 // The pieces of a unit that several CTAs share, in the order of its keys; a quarter warp or more has a row.
@@ -964,12 +884,6 @@ cudaError_t launch_prompt(const CUtensorMap& queries, const CUtensorMap& keys, c
         const cudaError_t err = cudaFuncSetAttribute(prompt_attention_kernel<T, D>,
                                                      cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
         if (err != cudaSuccess) return err;
-        if (Config<D>::kTiles == 2) {   // the warps' shares add up to what this build was given, or it does not run
-            cudaFuncAttributes attributes;
-            const cudaError_t known = cudaFuncGetAttributes(&attributes, prompt_attention_kernel<T, D>);
-            if (known != cudaSuccess) return known;
-            if (attributes.numRegs != kLaunchRegisters) return cudaErrorInvalidKernelImage;
-        }
         if (device < 64) configured.fetch_or(1ull << device, std::memory_order_relaxed);
     }
     cudaError_t err = launch_early(prompt_attention_kernel<T, D>, dim3(s.ctas), kThreads, s.smem, 1, stream, queries, keys,
@@ -993,8 +907,7 @@ CUtensorMapDataType data_type(int element) {
 }
 
 // Boxes of one 128-byte column of up to a block of tokens of a page and head.
-bool make_column_map(CUtensorMap* map, const AttentionArgs& a, const void* base, const Strides3& s, int element,
-                     int block) {
+bool make_column_map(CUtensorMap* map, const AttentionArgs& a, const void* base, const Strides3& s, int element) {
     prefill::EncodeTiledFn fn = prefill::encode_tiled();
     if (fn == nullptr) return false;
     const int page = 1 << a.page_shift;
@@ -1002,7 +915,7 @@ bool make_column_map(CUtensorMap* map, const AttentionArgs& a, const void* base,
                                 static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.pages)};
     const cuuint64_t strides[3] = {static_cast<cuuint64_t>(s.token) * 2, static_cast<cuuint64_t>(s.head) * 2,
                                    static_cast<cuuint64_t>(s.page) * 2};
-    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(page < block ? page : block), 1, 1};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(page < kBlock ? page : kBlock), 1, 1};
     const cuuint32_t steps[4] = {1, 1, 1, 1};
     return fn(map, data_type(element), 4, const_cast<void*>(base), dims, strides, box, steps,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -1044,10 +957,9 @@ int prompt_attention(const AttentionArgs& a, int element, void* workspace, cudaS
     if (s.ring < 3) return MB_ERR_RESOURCE;
     if (s.bytes != 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256)) return MB_ERR_INVALID;
     CUtensorMap queries, keys, values;
-    const int block = a.head_dim == 256 ? Config<256>::kBlock : Config<128>::kBlock;
     if (!make_query_map(&queries, a, element, s.tile_tokens) ||
-        !make_column_map(&keys, a, a.key_pages, a.kpool, element, block) ||
-        !make_column_map(&values, a, a.value_pages, a.vpool, element, block))
+        !make_column_map(&keys, a, a.key_pages, a.kpool, element) ||
+        !make_column_map(&values, a, a.value_pages, a.vpool, element))
         return MB_ERR_UNSUPPORTED;
     PromptArgs args;
     args.a = a;

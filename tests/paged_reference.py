@@ -75,15 +75,15 @@ def tolerance(result, keys: int, dtype: torch.dtype, weight_rounding: float):
 
     A score is a sum of D products in 32 bits, every partial sum off by at most 2^-23 of the sum of magnitudes M (an
     addition inside the matrix unit may cut instead of round): D 2^-23 M; the factors of scale and log2 e add
-    2^-22 |s| <= 2^-22 M.  A weight is then off by that, relatively, by 2^-21 for the exponential, and by 31 2^-24 for
-    the rounding of a maximum that is moved by up to 31, together less than 2^-18, in the numerator and in the
+    2^-22 |s| <= 2^-22 M.  A weight is then off by that, relatively, by 2.7e-6 at most for the exponential, and by
+    39 2^-24 for the rounding of a maximum that is moved by up to 39, together less than 2^-17, in the numerator and in the
     denominator; sums over n keys add n 2^-23 each; ``weight_rounding`` is the relative error of a weight as
     the second product takes it.  All of it multiplies the sum of weights times magnitudes of values; the rounding of
     the output, half a step of its type, comes on top."""
     out, magnitude, score = result
     half = torch.finfo(dtype).eps / 2
     dim = out.shape[-1]
-    relative = 2 * ((dim + 2) * 2.0 ** -23 * score + 2.0 ** -18 + keys * 2.0 ** -23) + weight_rounding
+    relative = 2 * ((dim + 2) * 2.0 ** -23 * score + 2.0 ** -17 + keys * 2.0 ** -23) + weight_rounding
     before = relative * magnitude
     return before + half * (out.abs() + before) + torch.finfo(dtype).tiny * half
 
