@@ -58,13 +58,29 @@ struct PromptArgs {
     float scale_log2;
     Split* splits;         // [ctas]
     float* stats;          // [ctas][2][tiles * 128][2]
-    float* partial;        // [ctas][2][tiles * 128][D]
+    float* partial;        // [ctas][2][D / 4][tiles * 128][4]
 };
 
+// A piece of a unit, as the warp that copies tells the others.
+struct Work {
+    int request, head, tile;
+    int begin, end, blocks;      // blocks of this piece, and of the unit; end < 0: nothing more
+    int first, tokens;           // queries of the unit
+    int position;                // of its first query
+    int stop0;                   // end of the blocks that its first query tile takes part in
+    int alone;                   // one query tile of two
+    int pieces;                  // CTAs that the unit's keys are shared out to, from this one on
+    int counted;                 // an empty piece that is one of another CTA's `pieces`
+};
+constexpr int kQueue = 4;
+
 struct PromptControl {
+    Work work[kQueue];
+    unsigned long long work_full[kQueue], work_empty[kQueue];
     unsigned long long full[kMaxTiles], empty[kMaxTiles], clean[kMaxTiles];
     unsigned long long q_full, q_empty, s_full[4], p_full[4], pv_done[4], o_empty[2];   // [slot], [tile] the last
     unsigned long long half_ready, half_taken;
+    unsigned long long turn[2][4];   // [query tile][warp]: its exponentials
     float half[kRows][2];        // maximum and sum of the second half of a lone query tile's keys
     unsigned int mask[kInfos][2];
     int partial[kInfos];         // not every key of the block counts
@@ -274,7 +290,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
     extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char* queries = smem;                                   // [tiles][chunks][128 rows][128 bytes]
     unsigned char* ring = queries + kTiles * C::kQueryBytes;         // [ring][chunks][block rows][128 bytes]
-    PromptControl* ctl = reinterpret_cast<PromptControl*>(ring + static_cast<size_t>(p.ring) * C::kTileBytes);
+    unsigned char* stagings = ring + static_cast<size_t>(p.ring) * C::kTileBytes;   // [softmax warps][32 rows][64 bytes]
+    PromptControl* ctl = reinterpret_cast<PromptControl*>(stagings + kTiles * 4 * 2048);
     long long* before = reinterpret_cast<long long*>(ctl + 1);       // [requests + 1]
     Request* requests = reinterpret_cast<Request*>(before + p.a.requests + 1);
 
@@ -296,6 +313,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         }
         mbar_init(&ctl->o_empty[0], 4);
         mbar_init(&ctl->o_empty[1], 4);
+        for (int q = 0; q < kQueue; ++q) {
+            mbar_init(&ctl->work_full[q], 1);
+            mbar_init(&ctl->work_empty[q], 5 * kTiles + 1);   // warps of softmax, of products, and the one that cleans
+        }
+        for (int w = 0; w < 8; ++w) mbar_init(&ctl->turn[w >> 2][w & 3], 1);
         mbar_init(&ctl->half_ready, 4);
         mbar_init(&ctl->half_taken, 4);
         ctl->abort_flag = 0;
@@ -354,12 +376,20 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
     volatile int* abort_flag = &ctl->abort_flag;
     bool ok = true;
 
-    // A unit of two query tiles: each takes the blocks up to the one its last query lies in.  A lone tile of a pair takes
-    // the place of both, which share its blocks in turn and meet at the end.
-    auto lone = [&](const Piece& u) { return kTiles == 1 || u.tokens <= p.tile_tokens; };
-    auto tile_end = [&](const Piece& u, int t) {
-        if (t == 1 || lone(u)) return u.end;
-        return min(max((u.position + p.tile_tokens + kBlock - 1) / kBlock, 1), u.end);
+    // The next piece, for a warp that all comes to; it keeps what it needs of it, or lets go of it later.
+    int queue = 0;
+    unsigned int queue_round = 0;
+    auto next_work = [&]() -> const Work* {
+        ok = ok && prefill::mbar_wait_warp(&ctl->work_full[queue], queue_round & 1, abort_flag);
+        return ok && ctl->work[queue].end >= 0 ? &ctl->work[queue] : nullptr;
+    };
+    auto release_work = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->work_empty[queue]);
+        if (++queue == kQueue) {
+            queue = 0;
+            ++queue_round;
+        }
     };
 
     if (warp == 8) {
@@ -369,14 +399,56 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         const int rows = min(page, kBlock);
         const int per_block = kBlock / rows;
         const int batch = 32 / per_block;
-        for (long long at = run_begin; ok && at < run_end;) {
-            const Piece u(deal, at, run_end);
-            at = u.next;
+        long long at = run_begin;
+        // a piece ahead of the copies, so that nobody waits for the arithmetic
+        auto publish = [&]() {
+            if (queue_round > 0)
+                ok = prefill::mbar_wait_warp(&ctl->work_empty[queue], (queue_round - 1) & 1, abort_flag);
+            if (!ok) return;
+            Work w = {};
+            w.end = -1;
+            if (at < run_end) {
+                // A unit of two query tiles: each takes the blocks up to the one its last query lies in.  A lone tile of a pair
+                // takes the place of both, which share its blocks in turn and meet at the end.
+                const Piece u(deal, at, run_end);
+                at = u.next;
+                w.request = u.request;
+                w.head = u.head;
+                w.tile = u.tile;
+                w.begin = u.begin;
+                w.end = u.end;
+                w.blocks = u.blocks;
+                w.first = u.first;
+                w.tokens = u.tokens;
+                w.position = u.position;
+                w.alone = kTiles == 2 && u.tokens <= p.tile_tokens;
+                w.stop0 = kTiles == 1 || w.alone
+                              ? u.end
+                              : min(max((u.position + p.tile_tokens + kBlock - 1) / kBlock, 1), u.end);
+                w.pieces = static_cast<int>((u.unit_end - 1) / deal.per - blockIdx.x) + 1;
+                w.counted = !u.at_start;
+            }
+            if (lane == 0) {
+                ctl->work[queue] = w;
+                mbar_arrive(&ctl->work_full[queue]);
+            }
+            __syncwarp();
+            if (++queue == kQueue) {
+                queue = 0;
+                ++queue_round;
+            }
+        };
+        publish();
+        for (int mine_at = 0; ok; mine_at = (mine_at + 1) % kQueue) {
+            const Work u = ctl->work[mine_at];
+            if (u.end < 0) break;
+            publish();
+            if (!ok) break;
             if (u.begin >= u.end) continue;
             if (units > 0) ok = prefill::mbar_wait_warp(&ctl->q_empty, (units - 1) & 1, abort_flag);
             if (!ok) break;
             ++units;
-            const int tiles = u.tokens > p.tile_tokens ? 2 : 1;
+            const int tiles = kTiles == 2 && !u.alone ? 2 : 1;
             if (elect_one()) {
                 mbar_arrive_expect_tx(&ctl->q_full, tiles * kChunks * p.tile_tokens * group * 128);
                 for (int t = 0; t < tiles; ++t)
@@ -474,14 +546,21 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             };
             unsigned int p_phase = 0;                // bit: slot
             unsigned int clean_phase = 0;            // bit: stage of the ring
-            for (long long at = run_begin; ok && at < run_end;) {
-                const Piece u(deal, at, run_end);
-                at = u.next;
-                if (u.begin >= u.end) continue;
+            while (ok) {
+                ok = mbar_wait_bounded(&ctl->work_full[queue], queue_round & 1, abort_flag);
+                if (!ok) break;
+                const int begin = ctl->work[queue].begin, end = ctl->work[queue].end;
+                if (end < 0) break;
+                const bool alone = ctl->work[queue].alone != 0;
+                const int tile_stop = tile == 0 ? ctl->work[queue].stop0 : end;
+                mbar_arrive(&ctl->work_empty[queue]);
+                if (++queue == kQueue) {
+                    queue = 0;
+                    ++queue_round;
+                }
+                if (begin >= end) continue;
                 ok = mbar_wait_bounded(&ctl->q_full, units & 1, abort_flag);
                 ++units;
-                const bool alone = kTiles == 2 && lone(u);
-                const int begin = u.begin, end = u.end, tile_stop = tile_end(u, tile);
                 auto takes = [&](int b) { return alone ? ((b - begin) & 1) == tile : b < tile_stop; };
                 const unsigned int q = low + ((queries_at + (alone ? 0 : tile * C::kQueryBytes)) >> 4);
                 int bs = begin, bv = begin;          // blocks whose scores, and whose products with values, come next
@@ -552,10 +631,10 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         // are zeroed before the product.  Every tile of the ring passes here, so that none is filled again unseen.
         int stage = 0, info = 0;
         unsigned int round = 0;
-        for (long long at = run_begin; ok && at < run_end;) {
-            const Piece u(deal, at, run_end);
-            at = u.next;
-            for (int b = u.begin; ok && b < u.end; ++b) {
+        while (const Work* u = next_work()) {
+            const int blocks = u->end - u->begin;
+            release_work();
+            for (int b = 0; ok && b < blocks; ++b) {
 #pragma unroll
                 for (int kind = 0; kind < 2; ++kind) {
                     ok = ok && prefill::mbar_wait_warp(&ctl->full[stage], round & 1, abort_flag);
@@ -584,31 +663,36 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
     } else if (warp < 4 * kTiles) {
         // ---- softmax and outputs of one query tile: a thread has a row
         const int tile = warp >> 2, r = (warp & 3) * 32 + lane;
-        const int token = r / group, query = r % group;          // of the tile
+        const int token = r / group;                             // of the tile
         const unsigned int lanes = tmem + (static_cast<unsigned int>((warp & 3) * 32) << 16);
         const unsigned int outputs = lanes + C::kColumnO + tile * D;
         int info = 0;
         unsigned int phase = 0;                         // bit: slot
         unsigned int halves = 0;                        // lone tiles so far
+        unsigned int turn = 0;                          // turns taken so far
         Split split = {0, 0, 0, 0};
         const bool premultiply = p.scale_log2 <= 0.f;   // the largest score is not that of the largest product
         const float multiplier = premultiply ? 1.f : p.scale_log2;
-        for (long long at = run_begin; at < run_end;) {
-            const Piece u(deal, at, run_end);
-            at = u.next;
-            const int slot_out = (blockIdx.x * 2 + (u.begin == 0 && u.end > 0 ? 1 : 0)) * kTiles * kRows + tile * kRows + r;
-            if (u.begin >= u.end) {
-                if (!u.at_start && p.splits != nullptr)   // counted as a piece
-                    *reinterpret_cast<float2*>(p.stats + static_cast<size_t>(slot_out) * 2) = make_float2(-INFINITY, 0.f);
+        while (const Work* u = next_work()) {
+            const int begin = u->begin, end = u->end;
+            if (begin >= end) {
+                if (u->counted != 0 && p.splits != nullptr)
+                    *reinterpret_cast<float2*>(p.stats + (static_cast<size_t>(blockIdx.x) * 2 * kTiles * kRows +
+                                                          tile * kRows + r) * 2) = make_float2(-INFINITY, 0.f);
+                release_work();
                 continue;
             }
-            const bool alone = kTiles == 2 && lone(u);
+            const bool alone = u->alone != 0;
             const int own = alone ? 0 : tile;                    // query tile
-            const int first_block = alone ? u.begin + tile : u.begin, blocks = tile_end(u, tile);
-            const int mine = own * p.tile_tokens + token;        // token of the unit
-            const int position = u.position + mine, first_position = u.position + own * p.tile_tokens;
+            const int first_block = alone ? begin + tile : begin, blocks = tile == 0 ? u->stop0 : end;
+            const int first_position = u->position + own * p.tile_tokens, position = first_position + token;
             float m = -INFINITY, l = 0.f;
-            unsigned int step = 0;
+            // turns are taken for as many steps as both tiles have
+            unsigned int step = 0, turns = 0;
+            if constexpr (kTiles == 2) {
+                turns = alone ? (end - begin) / 2 : max(u->stop0 - begin, 0);
+                if (tile == 1 && turns > 0 && lane == 0) mbar_arrive(&ctl->turn[0][warp & 3]);
+            }
             for (int b = first_block; b < blocks; b += alone ? 2 : 1, ++step) {
                 const int slot = tile * 2 + (step & 1);
                 ok = ok && prefill::mbar_wait_warp(&ctl->s_full[slot], (phase >> slot) & 1, abort_flag);
@@ -616,7 +700,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                 phase ^= 1u << slot;
                 prefill::tc_fence_after();
                 const unsigned int scores = lanes + slot * kBlock;
-                const int block_info = (info + b - u.begin) % kInfos;
+                const int block_info = (info + b - begin) % kInfos;
                 const bool partial = ctl->partial[block_info] != 0 || b * kBlock + kBlock - 1 > first_position;
                 float s[kBlock];
 #pragma unroll
@@ -665,6 +749,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     }
                     tmem_wait_store();
                 }
+                if (step < turns) {
+                    ok = prefill::mbar_wait_warp(&ctl->turn[tile][warp & 3], turn & 1, abort_flag);
+                    if (!ok) break;
+                    ++turn;
+                }
                 const float base = (m == -INFINITY ? 0.f : m) - kPromptShift<T>;
                 const unsigned long long multiplier2 = pair_of(multiplier, multiplier), base2 = pair_of(-base, -base);
                 unsigned long long sum0 = pair_of(0.f, 0.f), sum1 = sum0;
@@ -685,6 +774,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     // weights of 32 keys take 16 columns, of scores that have been read
                     tmem_store16(scores + c / 2, packed);
                 }
+                if (step + tile < turns && lane == 0) mbar_arrive(&ctl->turn[tile ^ 1][warp & 3]);
                 tmem_wait_store();
                 prefill::tc_fence_before();
                 __syncwarp();
@@ -692,7 +782,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                 sum0 = add_pair(sum0, sum1);
                 l += pair_low(sum0) + pair_high(sum0);
             }
-            info = (info + u.end - u.begin) % kInfos;
+            info = (info + end - begin) % kInfos;
             // the outputs of the piece
             const bool any = first_block < blocks;
             if (any) {
@@ -711,28 +801,39 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     prefill::tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&ctl->half_ready);
+                    release_work();
                     continue;
                 }
                 ok = ok && prefill::mbar_wait_warp(&ctl->half_ready, halves & 1, abort_flag);
                 ++halves;
                 prefill::tc_fence_after();
-                other_any = u.end - u.begin > 1;
+                other_any = end - begin > 1;
                 const float m1 = ctl->half[r][0], grown = fmaxf(m, m1), base = grown == -INFINITY ? 0.f : grown;
                 keep = prefill::exp2_approx(m - base);
                 other = prefill::exp2_approx(m1 - base);
                 l = l * keep + ctl->half[r][1] * other;
                 m = grown;
             }
-            const bool whole = u.begin == 0 && u.end == u.blocks;
-            const bool stored = ok && any && mine < u.tokens && token < p.tile_tokens;
+            const bool whole = begin == 0 && end == u->blocks;
+            const int unit_tokens = u->tokens;
             const float inverse = l == 0.f ? 0.f : 1.f / l;
             if (whole) keep *= inverse, other *= inverse;
-            if (!whole)
-                *reinterpret_cast<float2*>(p.stats + static_cast<size_t>(slot_out) * 2) =
-                    make_float2(any && l != 0.f ? m : -INFINITY, l);
-            unsigned short* to = p.a.out + (static_cast<size_t>(u.first + mine) * p.a.heads + u.head * group + query) * D;
-            float* partial = p.partial + static_cast<size_t>(slot_out) * D;
             if (ok && any) {
+                // a warp's 32 rows go through shared memory, 32 columns at a time, so that neighbouring lanes store
+                // neighbouring 16 bytes of a row; the partial sums of a cut unit have an order of their own, rows first
+                unsigned char* staging = stagings + warp * 2048;
+                float* partial = p.partial + static_cast<size_t>(blockIdx.x * 2 + (begin == 0 ? 1 : 0)) * kTiles * kRows * D +
+                                 (tile * kRows + r) * 4;
+                unsigned short* to[4];   // where this lane's rows go
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = r - lane + i * 8 + (lane >> 2), row_token = row / group;
+                    const int row_mine = own * p.tile_tokens + row_token;
+                    to[i] = row_token < p.tile_tokens && row_mine < unit_tokens
+                                ? p.a.out + (static_cast<size_t>(u->first + row_mine) * p.a.heads + u->head * group +
+                                             row % group) * D + (lane & 3) * 8
+                                : nullptr;
+                }
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
                     float o[32];
@@ -747,23 +848,36 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] = fmaf(o1[i], other, o[i]);
                     }
-                    if (!stored) continue;
                     if (whole) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8)
-                            *reinterpret_cast<uint4*>(to + c + i) =
+                        for (int i = 0; i < 32; i += 8)   // 64 bytes a row, 16-byte pieces swizzled over two rows
+                            *reinterpret_cast<uint4*>(staging + lane * 64 + (((i >> 3) ^ ((lane >> 1) & 3)) << 4)) =
                                 l == 0.f ? make_uint4(0u, 0u, 0u, 0u)
                                          : make_uint4(pack_pair<T>(o[i], o[i + 1]), pack_pair<T>(o[i + 2], o[i + 3]),
                                                       pack_pair<T>(o[i + 4], o[i + 5]), pack_pair<T>(o[i + 6], o[i + 7]));
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int at_row = i * 8 + (lane >> 2);
+                            const uint4 v = *reinterpret_cast<const uint4*>(staging + at_row * 64 +
+                                                                            (((lane & 3) ^ ((at_row >> 1) & 3)) << 4));
+                            if (to[i] != nullptr) *reinterpret_cast<uint4*>(to[i] + c) = v;
+                        }
+                        __syncwarp();
                     } else {
 #pragma unroll
                         for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<float4*>(partial + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                            *reinterpret_cast<float4*>(partial + static_cast<size_t>((c + i) / 4) * kTiles * kRows * 4) =
+                                make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                     }
                 }
             }
-            if (!whole && u.begin == 0)
-                split = {u.request, u.head, u.tile, static_cast<int>((u.unit_end - 1) / deal.per - blockIdx.x) + 1};
+            if (!whole) {
+                *reinterpret_cast<float2*>(
+                    p.stats + (static_cast<size_t>(blockIdx.x * 2 + (begin == 0 ? 1 : 0)) * kTiles * kRows + tile * kRows + r) * 2) =
+                    make_float2(any && l != 0.f ? m : -INFINITY, l);
+                if (begin == 0) split = {u->request, u->head, u->tile, u->pieces};
+            }
             prefill::tc_fence_before();
             __syncwarp();
             if (lane == 0) {
@@ -771,6 +885,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                 if (other_any) mbar_arrive(&ctl->o_empty[1]);
                 if (alone) mbar_arrive(&ctl->half_taken);
             }
+            release_work();
         }
         if (tid == 0 && p.splits != nullptr)
             *reinterpret_cast<int4*>(p.splits + blockIdx.x) = make_int4(split.request, split.head, split.tile, split.pieces);
@@ -798,7 +913,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
     if (warp == 11) prefill::tmem_dealloc(tmem, kTmemColumns);
 }
 
-// The pieces of a unit that several CTAs share, in the order of its keys; a quarter warp or more has a row.
+// The pieces of a unit that several CTAs share, in the order of its keys.
 constexpr int kJoinThreads = 256;
 constexpr int kJoinRows = 16;
 
@@ -814,7 +929,7 @@ __global__ void __launch_bounds__(kJoinThreads) prompt_join_kernel(const __grid_
     const int tokens = min(max(p.a.index[request + 1], first), p.a.tokens) - first;
     auto slot_of = [&](int i) { return (static_cast<size_t>(blockIdx.x) + i) * 2 + (i == 0 ? 1 : 0); };
     for (int i = threadIdx.x; i < kJoinRows * kColumns; i += kJoinThreads) {
-        const int r = blockIdx.y * kJoinRows + i / kColumns, c = i % kColumns * 4;
+        const int r = blockIdx.y * kJoinRows + i % kJoinRows, c = i / kJoinRows * 4;
         const int tile = r / kRows, in_tile = r % kRows, token = in_tile / group;
         const int mine = unit * unit_tokens + tile * p.tile_tokens + token;
         if (token >= p.tile_tokens || mine >= tokens) continue;
@@ -826,7 +941,8 @@ __global__ void __launch_bounds__(kJoinThreads) prompt_join_kernel(const __grid_
             const float2 s = __ldcg(reinterpret_cast<const float2*>(p.stats + (slot_of(q) * kUnitRows + r) * 2));
             if (s.x == -INFINITY) continue;   // nothing of it was written
             const float w = prefill::exp2_approx(s.x - highest);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.partial + (slot_of(q) * kUnitRows + r) * D + c));
+            const float4 v =
+                __ldcg(reinterpret_cast<const float4*>(p.partial + slot_of(q) * kUnitRows * D + (c / 4 * kUnitRows + r) * 4));
             total = fmaf(w, s.y, total);
             sum.x = fmaf(w, v.x, sum.x);
             sum.y = fmaf(w, v.y, sum.y);
@@ -860,7 +976,7 @@ Shape shape_of(const AttentionArgs& a, int sms) {
     const long long most = (units * (capacity + kTileCost) + kLeastKeys - 1) / kLeastKeys;
     s.ctas = static_cast<int>(std::min<long long>(most, sms));
     s.joined = capacity > kWholeKeys;
-    const int rest = C::kTiles * C::kQueryBytes + static_cast<int>(sizeof(PromptControl)) + 8 * (a.requests + 1) +
+    const int rest = C::kTiles * (C::kQueryBytes + 4 * 2048) + static_cast<int>(sizeof(PromptControl)) + 8 * (a.requests + 1) +
                      static_cast<int>(sizeof(Request)) * a.requests;
     s.ring = (kSmemLimit - rest) / C::kTileBytes;
     if (s.ring > kMaxTiles) s.ring = kMaxTiles;
