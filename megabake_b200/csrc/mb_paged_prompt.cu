@@ -32,6 +32,7 @@ constexpr int kWholeKeys = 1024;       // rows of the table that hold no more ar
 constexpr unsigned int kTmemColumns = 512;
 // A row's maximum may lag behind by this many powers of two before its sums are rescaled.
 constexpr float kLag = 8.f;
+constexpr int kPassAt = 48;            // keys of a block whose exponentials are done when the turn passes
 // As kWeightShift, with room for the lag.
 template <typename T>
 constexpr float kPromptShift = 7.f;
@@ -73,6 +74,7 @@ struct Work {
     int counted;                 // an empty piece that is one of another CTA's `pieces`
 };
 constexpr int kQueue = 4;
+constexpr int kStaging = 32 * 64;    // of a softmax warp's outputs
 
 struct PromptControl {
     Work work[kQueue];
@@ -127,7 +129,9 @@ struct Piece {
     long long next;              // where this piece ends in the deal
     bool at_start;               // of the unit
 
-    __device__ __forceinline__ Piece(const Deal& d, long long at, long long run_end) {
+    // Not inlined: the arithmetic of one piece is as much code as a softmax warp's loop, which it would drive out of the
+    // instruction cache.
+    __device__ __noinline__ Piece(const Deal& d, long long at, long long run_end) {
         int low = 0, high = d.count;   // before[low] * heads <= at < before[high] * heads
         while (high - low > 1) {
             const int middle = (low + high) >> 1;
@@ -272,6 +276,19 @@ __device__ __forceinline__ unsigned int pack_pair(float x, float y) {
     }
 }
 
+// Bounded waits.  What a wait that does not succeed at once does is one function for all of them: inlined into every one
+// it is a good part of the code that has to stay in the instruction cache.
+__device__ __noinline__ bool wait_on(unsigned long long* bar, unsigned int parity, volatile int* abort_flag) {
+    return mbar_wait_bounded(bar, parity, abort_flag);
+}
+__device__ __forceinline__ bool wait_thread(unsigned long long* bar, unsigned int parity, volatile int* abort_flag) {
+    return mbar_try_wait(bar, parity) || wait_on(bar, parity, abort_flag);
+}
+// Of a whole warp.
+__device__ __forceinline__ bool wait_warp(unsigned long long* bar, unsigned int parity, volatile int* abort_flag) {
+    return __all_sync(0xffffffffu, wait_thread(bar, parity, abort_flag)) != 0;
+}
+
 // ---------------------------------------------------------------------------------------
 // The kernel.  Two query tiles of 128 rows (tokens x the query heads of a key head) share every block of 64 keys, and
 // every tile has two slots of scores in tensor memory: while its softmax warps work on one block, the scores of the
@@ -291,7 +308,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
     unsigned char* queries = smem;                                   // [tiles][chunks][128 rows][128 bytes]
     unsigned char* ring = queries + kTiles * C::kQueryBytes;         // [ring][chunks][block rows][128 bytes]
     unsigned char* stagings = ring + static_cast<size_t>(p.ring) * C::kTileBytes;   // [softmax warps][32 rows][64 bytes]
-    PromptControl* ctl = reinterpret_cast<PromptControl*>(stagings + kTiles * 4 * 2048);
+    PromptControl* ctl = reinterpret_cast<PromptControl*>(stagings + kTiles * 4 * kStaging);
     long long* before = reinterpret_cast<long long*>(ctl + 1);       // [requests + 1]
     Request* requests = reinterpret_cast<Request*>(before + p.a.requests + 1);
 
@@ -380,7 +397,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
     int queue = 0;
     unsigned int queue_round = 0;
     auto next_work = [&]() -> const Work* {
-        ok = ok && prefill::mbar_wait_warp(&ctl->work_full[queue], queue_round & 1, abort_flag);
+        ok = ok && wait_warp(&ctl->work_full[queue], queue_round & 1, abort_flag);
         return ok && ctl->work[queue].end >= 0 ? &ctl->work[queue] : nullptr;
     };
     auto release_work = [&]() {
@@ -396,14 +413,15 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         // ---- copies
         int stage = 0, info = 0;
         unsigned int round = 0, units = 0;
-        const int rows = min(page, kBlock);
-        const int per_block = kBlock / rows;
-        const int batch = 32 / per_block;
+        constexpr int kBlockShift = kBlock == 128 ? 7 : 6;
+        const int rows_shift = min(shift, kBlockShift), rows = 1 << rows_shift;
+        const int per_shift = kBlockShift - rows_shift, per_block = 1 << per_shift;   // table entries of a block
+        const int batch = 32 >> per_shift;                                            // blocks whose entries the lanes hold
         long long at = run_begin;
         // a piece ahead of the copies, so that nobody waits for the arithmetic
         auto publish = [&]() {
             if (queue_round > 0)
-                ok = prefill::mbar_wait_warp(&ctl->work_empty[queue], (queue_round - 1) & 1, abort_flag);
+                ok = wait_warp(&ctl->work_empty[queue], (queue_round - 1) & 1, abort_flag);
             if (!ok) return;
             Work w = {};
             w.end = -1;
@@ -445,13 +463,15 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             publish();
             if (!ok) break;
             if (u.begin >= u.end) continue;
-            if (units > 0) ok = prefill::mbar_wait_warp(&ctl->q_empty, (units - 1) & 1, abort_flag);
+            if (units > 0) ok = wait_warp(&ctl->q_empty, (units - 1) & 1, abort_flag);
             if (!ok) break;
             ++units;
             const int tiles = kTiles == 2 && !u.alone ? 2 : 1;
             if (elect_one()) {
                 mbar_arrive_expect_tx(&ctl->q_full, tiles * kChunks * p.tile_tokens * group * 128);
+#pragma unroll 1
                 for (int t = 0; t < tiles; ++t)
+#pragma unroll 1
                     for (int c = 0; c < kChunks; ++c)
                         tma_load_3d(queries + t * C::kQueryBytes + c * kRows * 128, &query_map, c * 64, u.head * group,
                                     u.first + t * p.tile_tokens, &ctl->q_full);
@@ -461,8 +481,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             const int* entries = p.a.table + static_cast<size_t>(u.request) * p.a.width;
             const int entries_end = (n + page - 1) >> shift;
             auto entry_of = [&](int block) {
-                const int b = block + lane / per_block;
-                const int e = (b * kBlock + lane % per_block * rows) >> shift;
+                const int b = block + (lane >> per_shift);
+                const int e = (b * kBlock + ((lane & (per_block - 1)) << rows_shift)) >> shift;
                 const int id = b < u.end && e < entries_end ? entries[e] : -1;
                 return id >= 0 && id < p.a.pages ? id : -1;
             };
@@ -472,17 +492,18 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                 next = entry_of(b + batch);
                 for (int j = 0; ok && j < batch && b < u.end; ++j, ++b) {
                     const int place = page > kBlock ? (b * kBlock) & (page - 1) : 0;
-                    const unsigned int valid = __ballot_sync(0xffffffffu, mine >= 0) >> (j * per_block);
-                    int boxes = 0;
-                    for (int i = 0; i < per_block; ++i) boxes += (valid >> i) & 1u;
+                    const unsigned int valid = __ballot_sync(0xffffffffu, mine >= 0) >> (j << per_shift);
+                    const int boxes = __popc(valid & ((2u << (per_block - 1)) - 1));
+#pragma unroll 1
                     for (int kind = 0; kind < 2; ++kind) {   // keys, then values
-                        if (round > 0) ok = prefill::mbar_wait_warp(&ctl->empty[stage], (round - 1) & 1, abort_flag);
+                        if (round > 0) ok = wait_warp(&ctl->empty[stage], (round - 1) & 1, abort_flag);
                         if (!ok) break;
                         if (kind == 0 && lane < kBlock / 32) {
                             // which keys of the block count: on a page, and seen by any query of the unit
                             unsigned int word = 0;
+#pragma unroll 1
                             for (int i = 0; i < 32; i += 8)
-                                if ((valid >> ((lane * 32 + i) / rows)) & 1u) word |= 0xffu << i;
+                                if ((valid >> ((lane * 32 + i) >> rows_shift)) & 1u) word |= 0xffu << i;
                             const int left = n - b * kBlock - lane * 32;
                             if (left < 32) word &= left <= 0 ? 0u : (1u << left) - 1;
                             ctl->mask[info][lane] = word;
@@ -495,8 +516,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                             mbar_arrive_expect_tx(&ctl->full[stage], boxes * kChunks * rows * 128);
                         __syncwarp();
                         unsigned char* to = ring + static_cast<size_t>(stage) * C::kTileBytes;
+#pragma unroll 1
                         for (int i = 0; i < per_block; ++i) {
-                            const int id = __shfl_sync(0xffffffffu, mine, j * per_block + i);
+                            const int id = __shfl_sync(0xffffffffu, mine, (j << per_shift) + i);
                             if (id >= 0 && elect_one()) {
 #pragma unroll
                                 for (int c = 0; c < kChunks; ++c)
@@ -547,7 +569,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             unsigned int p_phase = 0;                // bit: slot
             unsigned int clean_phase = 0;            // bit: stage of the ring
             while (ok) {
-                ok = mbar_wait_bounded(&ctl->work_full[queue], queue_round & 1, abort_flag);
+                ok = wait_thread(&ctl->work_full[queue], queue_round & 1, abort_flag);
                 if (!ok) break;
                 const int begin = ctl->work[queue].begin, end = ctl->work[queue].end;
                 if (end < 0) break;
@@ -559,7 +581,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     ++queue_round;
                 }
                 if (begin >= end) continue;
-                ok = mbar_wait_bounded(&ctl->q_full, units & 1, abort_flag);
+                ok = wait_thread(&ctl->q_full, units & 1, abort_flag);
                 ++units;
                 auto takes = [&](int b) { return alone ? ((b - begin) & 1) == tile : b < tile_stop; };
                 const unsigned int q = low + ((queries_at + (alone ? 0 : tile * C::kQueryBytes)) >> 4);
@@ -569,7 +591,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     if (bs < end && scored - done < 2) {
                         // scores go where the weights of two steps ago were; not waited for while there is something to do
                         const bool idle = bs == bv;
-                        if (idle ? ok = mbar_wait_bounded(&ctl->full[key_stage], key_round & 1, abort_flag)
+                        if (idle ? ok = wait_thread(&ctl->full[key_stage], key_round & 1, abort_flag)
                                  : mbar_try_wait(&ctl->full[key_stage], key_round & 1)) {
                             if (takes(bs)) {
                                 const int slot = scored & 1;
@@ -594,16 +616,16 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                         }
                         if (!ok) break;
                     }
-                    ok = mbar_wait_bounded(&ctl->full[value_stage], value_round & 1, abort_flag);
+                    ok = wait_thread(&ctl->full[value_stage], value_round & 1, abort_flag);
                     if (ok && takes(bv)) {
                         const int slot = done & 1;
                         if (done == 0 && outputs_used++ > 0)   // the outputs before have been taken
-                            ok = mbar_wait_bounded(&ctl->o_empty[tile], outputs_used & 1, abort_flag);
+                            ok = wait_thread(&ctl->o_empty[tile], outputs_used & 1, abort_flag);
                         if (ok && ctl->partial[info] != 0) {
-                            ok = mbar_wait_bounded(&ctl->clean[value_stage], (clean_phase >> value_stage) & 1, abort_flag);
+                            ok = wait_thread(&ctl->clean[value_stage], (clean_phase >> value_stage) & 1, abort_flag);
                             clean_phase ^= 1u << value_stage;
                         }
-                        ok = ok && mbar_wait_bounded(&ctl->p_full[tile * 2 + slot], (p_phase >> slot) & 1, abort_flag);
+                        ok = ok && wait_thread(&ctl->p_full[tile * 2 + slot], (p_phase >> slot) & 1, abort_flag);
                         if (!ok) break;
                         p_phase ^= 1u << slot;
                         prefill::tc_fence_after();
@@ -635,12 +657,13 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             const int blocks = u->end - u->begin;
             release_work();
             for (int b = 0; ok && b < blocks; ++b) {
-#pragma unroll
+#pragma unroll 1
                 for (int kind = 0; kind < 2; ++kind) {
-                    ok = ok && prefill::mbar_wait_warp(&ctl->full[stage], round & 1, abort_flag);
+                    ok = ok && wait_warp(&ctl->full[stage], round & 1, abort_flag);
                     if (!ok) break;
                     if (kind == 1 && ctl->partial[info] != 0) {
                         unsigned char* values = ring + static_cast<size_t>(stage) * C::kTileBytes;
+#pragma unroll 2
                         for (int i = lane; i < kBlock * kChunks * 8; i += 32) {
                             const int row = i >> 3 & (kBlock - 1);
                             if (!((ctl->mask[info][row >> 5] >> (row & 31)) & 1u))
@@ -663,7 +686,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
     } else if (warp < 4 * kTiles) {
         // ---- softmax and outputs of one query tile: a thread has a row
         const int tile = warp >> 2, r = (warp & 3) * 32 + lane;
-        const int token = r / group;                             // of the tile
+        const int group_inverse = (65536 + group - 1) / group;   // r / group = r * this >> 16, for r below 128
+        const int token = r * group_inverse >> 16;               // of the tile
         const unsigned int lanes = tmem + (static_cast<unsigned int>((warp & 3) * 32) << 16);
         const unsigned int outputs = lanes + C::kColumnO + tile * D;
         int info = 0;
@@ -695,7 +719,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             }
             for (int b = first_block; b < blocks; b += alone ? 2 : 1, ++step) {
                 const int slot = tile * 2 + (step & 1);
-                ok = ok && prefill::mbar_wait_warp(&ctl->s_full[slot], (phase >> slot) & 1, abort_flag);
+                ok = ok && wait_warp(&ctl->s_full[slot], (phase >> slot) & 1, abort_flag);
                 if (!ok) break;
                 phase ^= 1u << slot;
                 prefill::tc_fence_after();
@@ -735,7 +759,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     m = grown;
                     l *= factor;
                     // the product before is in the outputs; the one before that is, since these scores are there
-                    ok = prefill::mbar_wait_warp(&ctl->pv_done[slot ^ 1], ((phase >> (slot ^ 1)) & 1) ^ 1, abort_flag);
+                    ok = wait_warp(&ctl->pv_done[slot ^ 1], ((phase >> (slot ^ 1)) & 1) ^ 1, abort_flag);
                     if (!ok) break;
                     prefill::tc_fence_after();
 #pragma unroll 1
@@ -750,7 +774,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     tmem_wait_store();
                 }
                 if (step < turns) {
-                    ok = prefill::mbar_wait_warp(&ctl->turn[tile][warp & 3], turn & 1, abort_flag);
+                    ok = wait_warp(&ctl->turn[tile][warp & 3], turn & 1, abort_flag);
                     if (!ok) break;
                     ++turn;
                 }
@@ -762,6 +786,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     unsigned int packed[16];
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
+                        // the other tile's begin while the last of these are under way
+                        if (c + i == kPassAt && step + tile < turns && lane == 0) mbar_arrive(&ctl->turn[tile ^ 1][warp & 3]);
                         const unsigned long long e0 = fma_pair(pair_of(s[c + i], s[c + i + 1]), multiplier2, base2);
                         const unsigned long long e1 = fma_pair(pair_of(s[c + i + 2], s[c + i + 3]), multiplier2, base2);
                         const float x0 = prefill::exp2_approx(pair_low(e0)), y0 = prefill::exp2_approx(pair_high(e0));
@@ -774,7 +800,6 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     // weights of 32 keys take 16 columns, of scores that have been read
                     tmem_store16(scores + c / 2, packed);
                 }
-                if (step + tile < turns && lane == 0) mbar_arrive(&ctl->turn[tile ^ 1][warp & 3]);
                 tmem_wait_store();
                 prefill::tc_fence_before();
                 __syncwarp();
@@ -787,14 +812,14 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             const bool any = first_block < blocks;
             if (any) {
                 const int slot = tile * 2 + ((step - 1) & 1);
-                ok = ok && prefill::mbar_wait_warp(&ctl->pv_done[slot], ((phase >> slot) & 1) ^ 1, abort_flag);
+                ok = ok && wait_warp(&ctl->pv_done[slot], ((phase >> slot) & 1) ^ 1, abort_flag);
                 prefill::tc_fence_after();
             }
             float keep = 1.f, other = 0.f;   // factors of these outputs and of the other half's
             bool other_any = false;
             if (alone) {
                 if (tile == 1) {
-                    if (halves > 0) ok = ok && prefill::mbar_wait_warp(&ctl->half_taken, (halves - 1) & 1, abort_flag);
+                    if (halves > 0) ok = ok && wait_warp(&ctl->half_taken, (halves - 1) & 1, abort_flag);
                     ++halves;
                     ctl->half[r][0] = m;
                     ctl->half[r][1] = l;
@@ -804,7 +829,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     release_work();
                     continue;
                 }
-                ok = ok && prefill::mbar_wait_warp(&ctl->half_ready, halves & 1, abort_flag);
+                ok = ok && wait_warp(&ctl->half_ready, halves & 1, abort_flag);
                 ++halves;
                 prefill::tc_fence_after();
                 other_any = end - begin > 1;
@@ -821,19 +846,12 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             if (ok && any) {
                 // a warp's 32 rows go through shared memory, 32 columns at a time, so that neighbouring lanes store
                 // neighbouring 16 bytes of a row; the partial sums of a cut unit have an order of their own, rows first
-                unsigned char* staging = stagings + warp * 2048;
+                unsigned char* staging = stagings + warp * kStaging;
                 float* partial = p.partial + static_cast<size_t>(blockIdx.x * 2 + (begin == 0 ? 1 : 0)) * kTiles * kRows * D +
                                  (tile * kRows + r) * 4;
-                unsigned short* to[4];   // where this lane's rows go
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = r - lane + i * 8 + (lane >> 2), row_token = row / group;
-                    const int row_mine = own * p.tile_tokens + row_token;
-                    to[i] = row_token < p.tile_tokens && row_mine < unit_tokens
-                                ? p.a.out + (static_cast<size_t>(u->first + row_mine) * p.a.heads + u->head * group +
-                                             row % group) * D + (lane & 3) * 8
-                                : nullptr;
-                }
+                const size_t first_row = (static_cast<size_t>(u->first) + own * p.tile_tokens) * p.a.heads + u->head * group;
+                const int tokens = min(unit_tokens - own * p.tile_tokens, p.tile_tokens);
+                unsigned short* to = p.a.out + first_row * D + (lane & 3) * 8;
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
                     float o[32];
@@ -850,7 +868,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     }
                     if (whole) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8)   // 64 bytes a row, 16-byte pieces swizzled over two rows
+                        for (int i = 0; i < 32; i += 8)   // 64 bytes a row, 16-byte pieces swizzled over eight rows
                             *reinterpret_cast<uint4*>(staging + lane * 64 + (((i >> 3) ^ ((lane >> 1) & 3)) << 4)) =
                                 l == 0.f ? make_uint4(0u, 0u, 0u, 0u)
                                          : make_uint4(pack_pair<T>(o[i], o[i + 1]), pack_pair<T>(o[i + 2], o[i + 3]),
@@ -858,10 +876,13 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                         __syncwarp();
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int at_row = i * 8 + (lane >> 2);
+                            const int at_row = i * 8 + (lane >> 2), row = r - lane + at_row;
+                            const int row_token = row * group_inverse >> 16, in_group = row - row_token * group;
                             const uint4 v = *reinterpret_cast<const uint4*>(staging + at_row * 64 +
                                                                             (((lane & 3) ^ ((at_row >> 1) & 3)) << 4));
-                            if (to[i] != nullptr) *reinterpret_cast<uint4*>(to[i] + c) = v;
+                            if (row_token < tokens)
+                                *reinterpret_cast<uint4*>(to + (static_cast<size_t>(row_token) * p.a.heads + in_group) * D + c) =
+                                    v;
                         }
                         __syncwarp();
                     } else {
@@ -976,7 +997,7 @@ Shape shape_of(const AttentionArgs& a, int sms) {
     const long long most = (units * (capacity + kTileCost) + kLeastKeys - 1) / kLeastKeys;
     s.ctas = static_cast<int>(std::min<long long>(most, sms));
     s.joined = capacity > kWholeKeys;
-    const int rest = C::kTiles * (C::kQueryBytes + 4 * 2048) + static_cast<int>(sizeof(PromptControl)) + 8 * (a.requests + 1) +
+    const int rest = C::kTiles * (C::kQueryBytes + 4 * kStaging) + static_cast<int>(sizeof(PromptControl)) + 8 * (a.requests + 1) +
                      static_cast<int>(sizeof(Request)) * a.requests;
     s.ring = (kSmemLimit - rest) / C::kTileBytes;
     if (s.ring > kMaxTiles) s.ring = kMaxTiles;
