@@ -26,8 +26,10 @@ constexpr int kBlock = 64;             // keys of a block
 constexpr int kMaxTiles = 12;          // of the ring: keys and values in turn
 constexpr int kInfos = 16;             // blocks whose masks are kept
 constexpr int kSmemLimit = 227 * 1024;
-constexpr int kTileCost = 128;         // what a unit costs besides its keys, in keys
-constexpr int kLeastKeys = 512;        // of a run
+// What a unit costs besides its keys, in keys: its outputs, and the way from one to the next.  With 128 and 256, 8,192
+// tokens of 128-wide heads took 510 and 481 us (192: 492, 320: 484), seven prompts of 64-wide ones 72 and 78.
+__host__ __device__ constexpr int tile_cost(int head_dim) { return head_dim == 64 ? 128 : 256; }
+constexpr int kLeastKeys = 512;        // of a run, where units are cut
 constexpr int kWholeKeys = 1024;       // rows of the table that hold no more are not cut
 constexpr unsigned int kTmemColumns = 512;
 // A row's maximum may lag behind by this many powers of two before its sums are rescaled.
@@ -103,7 +105,7 @@ struct Request {
 struct Deal {
     const long long* before;     // [requests + 1] lengths of the requests before, for one head
     const Request* requests;
-    int count, heads, unit_tokens;
+    int count, heads, unit_tokens, cost;
     long long total, per;
 };
 
@@ -111,13 +113,13 @@ __device__ __forceinline__ int units_of(const Request& q, int unit_tokens) {
     return (q.tokens + unit_tokens - 1) / unit_tokens;
 }
 // Lengths of the first `j` of the request's units, all of them full.
-__device__ __forceinline__ long long length_before(const Request& q, int unit_tokens, long long j) {
-    return j * (max(q.length - q.tokens, 0) + kTileCost) + j * (j + 1) / 2 * unit_tokens;
+__device__ __forceinline__ long long length_before(const Request& q, int unit_tokens, int cost, long long j) {
+    return j * (max(q.length - q.tokens, 0) + cost) + j * (j + 1) / 2 * unit_tokens;
 }
-__device__ __forceinline__ long long request_length(const Request& q, int unit_tokens) {
+__device__ __forceinline__ long long request_length(const Request& q, int unit_tokens, int cost) {
     const int units = units_of(q, unit_tokens);
     if (units == 0) return 0;
-    return length_before(q, unit_tokens, units - 1) + max(q.length - q.tokens, 0) + q.tokens + kTileCost;
+    return length_before(q, unit_tokens, cost, units - 1) + max(q.length - q.tokens, 0) + q.tokens + cost;
 }
 
 struct Piece {
@@ -150,14 +152,14 @@ struct Piece {
         int lower = 0, upper = units;
         while (upper - lower > 1) {
             const int middle = (lower + upper) >> 1;
-            if (length_before(q, d.unit_tokens, middle) <= rest)
+            if (length_before(q, d.unit_tokens, d.cost, middle) <= rest)
                 lower = middle;
             else
                 upper = middle;
         }
         tile = lower;
-        const long long start = length_before(q, d.unit_tokens, tile);
-        const long long end_of = tile + 1 == units ? length : length_before(q, d.unit_tokens, tile + 1);
+        const long long start = length_before(q, d.unit_tokens, d.cost, tile);
+        const long long end_of = tile + 1 == units ? length : length_before(q, d.unit_tokens, d.cost, tile + 1);
         const long long unit_begin = at - (rest - start);
         unit_end = unit_begin + (end_of - start);
         next = min(unit_end, run_end);
@@ -354,6 +356,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
     deal.count = p.a.requests;
     deal.heads = p.a.kv_heads;
     deal.unit_tokens = p.tile_tokens * kTiles;
+    deal.cost = tile_cost(D);
     {
         const int each = (p.a.requests + kThreads - 1) / kThreads;
         const int r0 = min(tid * each, p.a.requests), r1 = min(r0 + each, p.a.requests);
@@ -363,7 +366,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             const int first = min(max(p.a.index[r], 0), p.a.tokens), end = min(max(p.a.index[r + 1], first), p.a.tokens);
             const Request q = {first, end - first, min(max(p.a.lengths[r], 0), capacity)};
             requests[r] = q;
-            sum += request_length(q, deal.unit_tokens);
+            sum += request_length(q, deal.unit_tokens, deal.cost);
         }
         long long inclusive = sum;
 #pragma unroll
@@ -377,13 +380,13 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         for (int w = 0; w < warp; ++w) mine += ctl->warp_sums[w];
         for (int r = r0; r < r1; ++r) {
             before[r] = mine;
-            mine += request_length(requests[r], deal.unit_tokens);
+            mine += request_length(requests[r], deal.unit_tokens, deal.cost);
         }
         if (r0 < p.a.requests && r1 == p.a.requests) before[p.a.requests] = mine;
         __syncthreads();
     }
     deal.total = before[p.a.requests] * deal.heads;
-    deal.per = max((deal.total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kLeastKeys));
+    deal.per = max((deal.total + gridDim.x - 1) / gridDim.x, p.splits != nullptr ? static_cast<long long>(kLeastKeys) : 1);
     long long run_begin = min(blockIdx.x * deal.per, deal.total);
     long long run_end = min(run_begin + deal.per, deal.total);
     if (p.splits == nullptr) {   // no unit is cut: runs go from unit to unit
@@ -994,9 +997,9 @@ Shape shape_of(const AttentionArgs& a, int sms) {
     // at most so many units, none longer than a row of the table
     const long long units = (a.tokens / (s.tile_tokens * s.tiles) + std::min(a.requests, a.tokens)) * static_cast<long long>(a.kv_heads);
     const long long capacity = static_cast<long long>(a.width) << a.page_shift;
-    const long long most = (units * (capacity + kTileCost) + kLeastKeys - 1) / kLeastKeys;
-    s.ctas = static_cast<int>(std::min<long long>(most, sms));
     s.joined = capacity > kWholeKeys;
+    const long long most = s.joined ? (units * (capacity + tile_cost(D)) + kLeastKeys - 1) / kLeastKeys : units;
+    s.ctas = static_cast<int>(std::min<long long>(most, sms));
     const int rest = C::kTiles * (C::kQueryBytes + 4 * kStaging) + static_cast<int>(sizeof(PromptControl)) + 8 * (a.requests + 1) +
                      static_cast<int>(sizeof(Request)) * a.requests;
     s.ring = (kSmemLimit - rest) / C::kTileBytes;
