@@ -76,6 +76,8 @@ struct Work {
     int counted;                 // an empty piece that is one of another CTA's `pieces`
 };
 constexpr int kQueue = 4;
+// What is special about a block: keys of it do not count, or some queries of the unit come before keys of it.
+constexpr int kMasked = 1, kDiagonal = 2;
 constexpr int kStaging = 32 * 64;    // of a softmax warp's outputs
 
 struct PromptControl {
@@ -87,7 +89,8 @@ struct PromptControl {
     unsigned long long turn[2][4];   // [query tile][warp]: its exponentials
     float half[kRows][2];        // maximum and sum of the second half of a lone query tile's keys
     unsigned int mask[kInfos][2];
-    int partial[kInfos];         // not every key of the block counts
+    int special[kInfos];         // of a block: kMasked, kDiagonal
+    int odd[kInfos];             // values that are no numbers were taken out of it
     long long warp_sums[kThreads / 32];
     unsigned int tmem;
     int abort_flag;
@@ -275,6 +278,46 @@ __device__ __forceinline__ unsigned int pack_pair(float x, float y) {
         return *reinterpret_cast<const unsigned int*>(&h);
     } else {
         return prefill::pack_bf16_pair(x, y);
+    }
+}
+
+// Whether one of two 16-bit values is infinite or NaN: all bits of its exponent set, which one more carries out of it.
+template <typename T>
+__device__ __forceinline__ bool not_finite(unsigned int v) {
+    constexpr unsigned int kExponents = std::is_same_v<T, __half> ? 0x7c007c00u : 0x7f807f80u;
+    constexpr unsigned int kOnes = std::is_same_v<T, __half> ? 0x04000400u : 0x00800080u;
+    return ((v & kExponents) + kOnes & 0x80008000u) != 0u;
+}
+template <typename T>
+__device__ __forceinline__ unsigned int without_odd(unsigned int v) {
+    return (not_finite<T>(v & 0xffffu) ? 0u : v & 0xffffu) | (not_finite<T>(v & 0xffff0000u) ? 0u : v & 0xffff0000u);
+}
+// The infinities and NaN that were taken out of blocks `from` .. `end` - 1 of a unit, 32 columns of them from `column` on,
+// added to the outputs of a query at `position`.  `info` is that of block `end`.
+template <typename T, int kBlock>
+__device__ __noinline__ void give_back(float* o, const AttentionArgs& a, const PromptControl* ctl, const Work* u, int info,
+                                       int from, int end, int column, int position) {
+#pragma unroll 1
+    for (int b = from; b < end; ++b) {
+        const int block_info = (info + 2 * kInfos - (end - b)) % kInfos;
+        if (ctl->odd[block_info] == 0) continue;
+#pragma unroll 1
+        for (int k = 0; k < kBlock; ++k) {
+            const int key = b * kBlock + k;
+            if (!((ctl->mask[block_info][k >> 5] >> (k & 31)) & 1u) || key > position) continue;
+            const long long entry = a.table[static_cast<size_t>(u->request) * a.width + (key >> a.page_shift)];
+            const unsigned short* values = a.value_pages + entry * a.vpool.page +
+                                           (key & ((1 << a.page_shift) - 1)) * a.vpool.token + u->head * a.vpool.head + column;
+#pragma unroll 1
+            for (int i = 0; i < 32; ++i) {
+                const unsigned short bits = values[i];
+                if (!not_finite<T>(bits)) continue;
+                if constexpr (std::is_same_v<T, __half>)
+                    o[i] += __half2float(*reinterpret_cast<const __half*>(&bits));
+                else
+                    o[i] += bf16_bits_to_float(bits);
+            }
+        }
     }
 }
 
@@ -513,7 +556,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                         }
                         __syncwarp();
                         if (kind == 0 && lane == 0)
-                            ctl->partial[info] = boxes != per_block || n - b * kBlock < kBlock;
+                            ctl->odd[info] = 0, ctl->special[info] = (boxes != per_block || n - b * kBlock < kBlock ? kMasked : 0) |
+                                                 (b * kBlock + kBlock - 1 > u.position ? kDiagonal : 0);
                         __syncwarp();
                         if (elect_one())
                             mbar_arrive_expect_tx(&ctl->full[stage], boxes * kChunks * rows * 128);
@@ -624,7 +668,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                         const int slot = done & 1;
                         if (done == 0 && outputs_used++ > 0)   // the outputs before have been taken
                             ok = wait_thread(&ctl->o_empty[tile], outputs_used & 1, abort_flag);
-                        if (ok && ctl->partial[info] != 0) {
+                        if (ok && ctl->special[info] != 0) {
                             ok = wait_thread(&ctl->clean[value_stage], (clean_phase >> value_stage) & 1, abort_flag);
                             clean_phase ^= 1u << value_stage;
                         }
@@ -641,7 +685,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                         prefill::umma_commit(&ctl->empty[value_stage]);
                         ++done;
                     } else if (ok) {
-                        if (ctl->partial[info] != 0) clean_phase ^= 1u << value_stage;
+                        if (ctl->special[info] != 0) clean_phase ^= 1u << value_stage;
                         mbar_arrive(&ctl->empty[value_stage]);
                     }
                     advance(value_stage, value_round);
@@ -653,7 +697,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         ok = __all_sync(0xffffffffu, ok);
     } else if (warp == 11) {
         // ---- values of keys that do not count may be anything, and 0 * NaN is NaN: where a block has such keys their rows
-        // are zeroed before the product.  Every tile of the ring passes here, so that none is filled again unseen.
+        // are zeroed before the product.  Where some queries see a key and some do not, infinities and NaN are taken out and
+        // given back to those who see them with the outputs.  Every tile of the ring passes here, so that none is
+        // filled again unseen.
         int stage = 0, info = 0;
         unsigned int round = 0;
         while (const Work* u = next_work()) {
@@ -664,14 +710,30 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                 for (int kind = 0; kind < 2; ++kind) {
                     ok = ok && wait_warp(&ctl->full[stage], round & 1, abort_flag);
                     if (!ok) break;
-                    if (kind == 1 && ctl->partial[info] != 0) {
+                    const int special = kind == 1 ? ctl->special[info] : 0;
+                    if (special != 0) {
                         unsigned char* values = ring + static_cast<size_t>(stage) * C::kTileBytes;
+                        bool odd = false;
 #pragma unroll 2
                         for (int i = lane; i < kBlock * kChunks * 8; i += 32) {
                             const int row = i >> 3 & (kBlock - 1);
-                            if (!((ctl->mask[info][row >> 5] >> (row & 31)) & 1u))
-                                *reinterpret_cast<uint4*>(values + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                            uint4* at = reinterpret_cast<uint4*>(values + i * 16);
+                            if (!((ctl->mask[info][row >> 5] >> (row & 31)) & 1u)) {
+                                *at = make_uint4(0u, 0u, 0u, 0u);
+                            } else if (special & kDiagonal) {
+                                uint4 v = *at;
+                                if (not_finite<T>(v.x) | not_finite<T>(v.y) | not_finite<T>(v.z) | not_finite<T>(v.w)) {
+                                    odd = true;
+                                    v.x = without_odd<T>(v.x);
+                                    v.y = without_odd<T>(v.y);
+                                    v.z = without_odd<T>(v.z);
+                                    v.w = without_odd<T>(v.w);
+                                    *at = v;
+                                }
+                            }
                         }
+                        odd = __any_sync(0xffffffffu, odd);
+                        if (lane == 0) ctl->odd[info] = odd;
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&ctl->clean[stage]);
@@ -728,7 +790,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                 prefill::tc_fence_after();
                 const unsigned int scores = lanes + slot * kBlock;
                 const int block_info = (info + b - begin) % kInfos;
-                const bool partial = ctl->partial[block_info] != 0 || b * kBlock + kBlock - 1 > first_position;
+                const bool partial = (ctl->special[block_info] & kMasked) != 0 || b * kBlock + kBlock - 1 > first_position;
                 float s[kBlock];
 #pragma unroll
                 for (int c = 0; c < kBlock; c += 32) tmem_load32_async(scores + c, s + c);
@@ -844,6 +906,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             }
             const bool whole = begin == 0 && end == u->blocks;
             const int unit_tokens = u->tokens;
+            const int diagonal = max(begin, max(u->position, 0) / kBlock);   // the first block that a query may not see whole
+            bool any_odd = false;
+            for (int b = diagonal; b < end; ++b) any_odd |= ctl->odd[(info + 2 * kInfos - (end - b)) % kInfos] != 0;
             const float inverse = l == 0.f ? 0.f : 1.f / l;
             if (whole) keep *= inverse, other *= inverse;
             if (ok && any) {
@@ -868,6 +933,14 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                         tmem_wait_load();
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] = fmaf(o1[i], other, o[i]);
+                    }
+                    if (any_odd) {
+                        float given[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) given[i] = o[i];
+                        if (l != 0.f) give_back<T, kBlock>(given, p.a, ctl, u, info, diagonal, end, c, position);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = given[i];
                     }
                     if (whole) {
 #pragma unroll

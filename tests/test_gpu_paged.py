@@ -428,6 +428,41 @@ def test_prompt_infinities_and_nan():
     assert out[:50].isfinite().all() and out[100:].isfinite().all()
 
 
+@pytest.mark.parametrize("heads,new,cached", [((4, 2, 64), 200, 0), ((2, 1, 128), 40, 500), ((8, 1, 256), 50, 3),
+                                              ((1, 1, 64), 300, 5000), ((4, 4, 128), 20, 0)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_prompt_values_that_are_no_numbers(heads, new, cached, dtype):
+    """Infinities and NaN among the values reach the queries that see them, in their columns, and no others."""
+    count, kv_heads, dim = heads
+    cache = Cache([new + cached], kv_heads, dim, 16, dtype, new)
+    query = _normal((new, count, dim), cache.g, dtype)
+    odd = {cached + new // 2: {0: float("inf"), 33: float("nan")}, cached + new // 2 + 3: {0: -float("inf"), dim - 1: -float("inf")},
+           cached + new - 1: {7: float("nan")}}
+    if cached:
+        odd[cached // 2] = {40: float("inf")}
+    for position, columns in odd.items():
+        slot = cache.slots[0][position]
+        for column, value in columns.items():
+            cache.pools[1][slot // 16, slot % 16, kv_heads - 1, column] = value
+    out = paged_prefill_attention(query, *cache.pools, cache.table, cache.lengths, _int32([0, new]))
+    finite = [p.clone() for p in cache.pools]
+    finite[1].nan_to_num_(0.0, 0.0, 0.0)
+    group = count // kv_heads
+    mine = torch.arange(count, device="cuda") // group == kv_heads - 1
+    for t in _some(new):
+        seen = {}
+        for position, columns in odd.items():
+            if position <= cached + t:
+                for column, value in columns.items():
+                    seen[column] = seen.get(column, 0.0) + value
+        got, expected = out[t].clone(), reference.attend(query[t], *finite, cache.table[0], cached + t + 1, dim ** -0.5)
+        for column, value in seen.items():
+            there = got[mine, column]
+            assert bool(there.isnan().all() if value != value else there.eq(value).all()), (t, column)
+            got[mine, column] = expected[0][mine, column].to(dtype)
+        _check(got, expected, cached + t + 1, dtype, reference.prompt_rounding(dtype))
+
+
 # ---------------------------------------------------------------------------------------
 # Streams, graphs, devices, refusals
 # ---------------------------------------------------------------------------------------
