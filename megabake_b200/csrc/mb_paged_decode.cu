@@ -82,7 +82,9 @@ __device__ __forceinline__ Piece piece_at(const Deal& d, long long at, long long
     p.token = low;
     p.blocks = d.first_block[low + 1] - d.first_block[low];
     const long long rest = at - static_cast<long long>(d.first_block[low]) * d.units;
-    p.unit = static_cast<int>(rest / p.blocks);
+    // (a division of 64-bit numbers takes several hundred cycles)
+    p.unit = rest >> 32 == 0 ? static_cast<int>(static_cast<unsigned int>(rest) / static_cast<unsigned int>(p.blocks))
+                             : static_cast<int>(rest / p.blocks);
     p.begin = static_cast<int>(rest - static_cast<long long>(p.unit) * p.blocks);
     p.end = static_cast<int>(min(static_cast<long long>(p.blocks), p.begin + (run_end - at)));
     return p;
@@ -246,9 +248,9 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
         int stage = 0;
         unsigned int round = 0;
         bool ok = true;
-        const int per_block = page < kBlock ? kBlock >> shift : 1;     // table entries of a block
-        const int batch = 32 / per_block;                              // blocks whose entries the lanes hold
-        const int rows = min(page, kBlock);
+        const int rows_shift = min(shift, 6), rows = 1 << rows_shift;
+        const int per_shift = 6 - rows_shift, per_block = 1 << per_shift;   // table entries of a block
+        const int batch = 32 >> per_shift;                                  // blocks whose entries the lanes hold
         for (long long at = run_begin; ok && at < run_end;) {
             const Piece piece = piece_at(deal, at, run_end);
             at += piece.end - piece.begin;
@@ -256,8 +258,8 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
             const int* entries = p.a.table + static_cast<size_t>(table_rows[piece.token]) * p.a.width;
             const int entries_end = (n + page - 1) >> shift;
             auto entry_of = [&](int block) {   // this lane's entry of the batch that starts at `block`
-                const int b = block + lane / per_block;
-                const int e = page < kBlock ? b * per_block + lane % per_block : b >> (shift - 6);
+                const int b = block + (lane >> per_shift);
+                const int e = shift < 6 ? (b << per_shift) + (lane & (per_block - 1)) : b >> (shift - 6);
                 int id = b < piece.end && e < entries_end ? entries[e] : -1;
                 return id >= 0 && id < p.a.pages ? id : -1;
             };
@@ -272,29 +274,34 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
                     }
                     unsigned char* keys = ring + static_cast<size_t>(stage) * 2 * kTile;
                     const int left = n - b * kBlock;
-                    unsigned long long mask = 0;
-                    int boxes = 0;
-                    for (int i = 0; i < per_block; ++i) {
-                        if (__shfl_sync(0xffffffffu, mine, j * per_block + i) < 0) continue;
-                        mask |= (rows == kBlock ? ~0ull : (1ull << rows) - 1) << (i * rows);
-                        ++boxes;
-                    }
-                    if (left < kBlock) mask &= (1ull << left) - 1;
+                    const int id = __shfl_sync(0xffffffffu, mine, (j << per_shift) + (lane & (per_block - 1)));
+                    const unsigned int valid = __ballot_sync(0xffffffffu, id >= 0) & ((2u << (per_block - 1)) - 1);
+                    // lanes 0 .. 7: of which eight keys are on a page
+                    const unsigned int eights =
+                        __ballot_sync(0xffffffffu, lane < 8 && ((valid >> (lane >> (rows_shift - 3))) & 1u));
                     if (elect_one()) {
+                        unsigned long long mask = 0;   // a byte for every bit of `eights`
+                        if (eights == 0xffu)
+                            mask = ~0ull;
+                        else
+                            for (int i = 0; i < 8; ++i) mask |= ((eights >> i) & 1u) ? 0xffull << (8 * i) : 0ull;
+                        if (left < kBlock) mask &= (1ull << left) - 1;
                         ctl->mask[stage] = mask;
-                        mbar_arrive_expect_tx(&ctl->full[stage], boxes * 2 * rows * D * 2);
+                        mbar_arrive_expect_tx(&ctl->full[stage], __popc(valid) * 2 * rows * D * 2);
                     }
                     __syncwarp();
                     const int place = page > kBlock ? (b * kBlock) & (page - 1) : 0;
-                    for (int i = 0; i < per_block; ++i) {
-                        const int id = __shfl_sync(0xffffffffu, mine, j * per_block + i);
+                    if (per_block == 1) {
                         if (id >= 0 && elect_one()) {
-                            tma_load_page(keys + i * rows * D * 2, &key_map, place, head, id, &ctl->full[stage]);
-                            tma_load_page(keys + kTile + i * rows * D * 2, &value_map, place, head, id,
-                                          &ctl->full[stage]);
+                            tma_load_page(keys, &key_map, place, head, id, &ctl->full[stage]);
+                            tma_load_page(keys + kTile, &value_map, place, head, id, &ctl->full[stage]);
                         }
-                        __syncwarp();
+                    } else if (lane < 2 * per_block && id >= 0) {   // a box a lane: keys, then values
+                        const bool second = lane >= per_block;
+                        tma_load_page(keys + (second ? kTile : 0) + (lane & (per_block - 1)) * rows * D * 2,
+                                      second ? &value_map : &key_map, place, head, id, &ctl->full[stage]);
                     }
+                    __syncwarp();
                     if (++stage == p.stages) {
                         stage = 0;
                         ++round;
