@@ -23,8 +23,16 @@ namespace paged {
 namespace {
 
 constexpr int kBlock = 64;          // keys of a ring stage
-constexpr int kWarps = 4;           // that compute, 16 keys of a stage each
-constexpr int kThreads = 32 * (kWarps + 1);
+// Warps that compute, 16 keys of a stage each: two teams of four on stages in turn for 64-wide heads, whose stages are
+// half as many bytes and take a team nearly as long (37 ragged contexts of up to 4,099 keys in pages of 16, 2 key heads:
+// 22.0 -> 20.5 us).  The ring then has an even number of stages, so that a stage always belongs to one team, which sees
+// every phase of its barrier: one that saw every other phase could not tell them apart by their parity.
+template <int D>
+constexpr int kTeams = D == 64 ? 2 : 1;
+template <int D>
+constexpr int kWarps = 4 * kTeams<D>;
+template <int D>
+constexpr int kThreads = 32 * (kWarps<D> + 1);
 constexpr int kMaxStages = 16;
 constexpr int kSmemLimit = 227 * 1024;
 constexpr int kConsumerBarrier = 1;
@@ -48,8 +56,8 @@ struct DecodeArgs {
 
 struct Control4 {
     unsigned long long full[kMaxStages], empty[kMaxStages], mask[kMaxStages];
-    float stats[kWarps][16][2];
-    int warp_sums[kWarps + 1];
+    float stats[8][16][2];
+    int warp_sums[9];
     int abort_flag;
 };
 
@@ -88,6 +96,18 @@ __device__ __forceinline__ Piece piece_at(const Deal& d, long long at, long long
     p.begin = static_cast<int>(rest - static_cast<long long>(p.unit) * p.blocks);
     p.end = static_cast<int>(min(static_cast<long long>(p.blocks), p.begin + (run_end - at)));
     return p;
+}
+
+// The piece after `p`, which ended with its unit at `at`.
+__device__ __forceinline__ void next_piece(const Deal& d, Piece& p, long long at, long long run_end) {
+    if (++p.unit == d.units) {
+        p.unit = 0;
+        do ++p.token;
+        while (d.first_block[p.token + 1] == d.first_block[p.token]);   // there is one with keys: `at` is before the end
+        p.blocks = d.first_block[p.token + 1] - d.first_block[p.token];
+    }
+    p.begin = 0;
+    p.end = static_cast<int>(min(static_cast<long long>(p.blocks), run_end - at));
 }
 
 // The first end or begin of a unit from `at` on.
@@ -163,16 +183,17 @@ __device__ __forceinline__ float shuffled_sum(float v) {
 __device__ __forceinline__ float finite_base(float m) { return m == -INFINITY ? 0.f : m; }
 
 // ---------------------------------------------------------------------------------------
-// The kernel: one CTA per SM.  A warp copies pages into a ring of stages of 64 keys and their values; four warps take 16
-// keys of a stage each.  Keys are the 16 rows of m16n8k16 products and queries its 8 columns, so that 8
+// The kernel: one CTA per SM.  A warp copies pages into a ring of stages of 64 keys and their values; teams of four warps
+// take stages in turn, a warp 16 of its keys.  Keys are the 16 rows of m16n8k16 products and queries its 8 columns, so that 8
 // query heads of a key head cost what one costs; the scores come out with a query's keys spread over lanes, a transpose
 // of 8 x 8 (movmatrix) makes them the second product's columns, and values are read transposed (ldmatrix.trans) as its
 // rows: o^T = v^T p^T, whose columns are queries again, so that rescaling is by the lane's own two queries.
 // ---------------------------------------------------------------------------------------
 template <typename T, int D, int N>   // N: 8-query columns of a unit
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads<D>, 1)
 decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
                         const __grid_constant__ DecodeArgs p) {
+    constexpr int kTeams = paged::kTeams<D>, kWarps = paged::kWarps<D>, kThreads = paged::kThreads<D>;
     constexpr int kTile = kBlock * D * 2;           // bytes of a stage's keys, and of its values
     constexpr int kQueries = 8 * N;
     constexpr int kMergeRow = D + 4;                // floats; the padding keeps a warp's stores off each other's banks
@@ -189,7 +210,7 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
     if (tid == 0) {
         for (int s = 0; s < p.stages; ++s) {
             mbar_init(&ctl->full[s], 1);
-            mbar_init(&ctl->empty[s], kWarps);
+            mbar_init(&ctl->empty[s], 4);
         }
         ctl->abort_flag = 0;
         mbar_init_fence();
@@ -251,10 +272,14 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
         const int rows_shift = min(shift, 6), rows = 1 << rows_shift;
         const int per_shift = 6 - rows_shift, per_block = 1 << per_shift;   // table entries of a block
         const int batch = 32 >> per_shift;                                  // blocks whose entries the lanes hold
+        Piece piece = {};
         for (long long at = run_begin; ok && at < run_end;) {
-            const Piece piece = piece_at(deal, at, run_end);
+            if (at == run_begin)
+                piece = piece_at(deal, at, run_end);
+            else
+                next_piece(deal, piece, at, run_end);
             at += piece.end - piece.begin;
-            const int n = lengths[piece.token], head = piece.unit / p.subgroups;
+            const int n = lengths[piece.token], head = p.subgroups == 1 ? piece.unit : piece.unit / p.subgroups;
             const int* entries = p.a.table + static_cast<size_t>(table_rows[piece.token]) * p.a.width;
             const int entries_end = (n + page - 1) >> shift;
             auto entry_of = [&](int block) {   // this lane's entry of the batch that starts at `block`
@@ -320,7 +345,7 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
         bool ok = true;
         Split split = {0, 0, 0, 0};
         const int rows = min(page, kBlock);
-        const int key0 = warp * 16;
+        const int key0 = (warp & 3) * 16, team = warp >> 2;
         // where this lane's rows of the 16 x 16 fragments lie: keys (not transposed) and values (transposed)
         const int k_row = key0 + (lane & 7) + ((lane >> 3) & 1) * 8, k_half = lane >> 4;
         const int v_row = key0 + (lane & 7) + (lane >> 4) * 8, v_half = (lane >> 3) & 1;
@@ -328,10 +353,16 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
         const int k_base = (k_row / rows) * rows * D * 2 + (k_row % rows) * 128;
         const int v_base = (v_row / rows) * rows * D * 2 + (v_row % rows) * 128;
         const int column = rows * 128;
+        int turn = 0;   // of the teams
+        Piece piece = {};
         for (long long at = run_begin; at < run_end;) {
-            const Piece piece = piece_at(deal, at, run_end);
+            if (at == run_begin)
+                piece = piece_at(deal, at, run_end);
+            else
+                next_piece(deal, piece, at, run_end);
             at += piece.end - piece.begin;
-            const int n = lengths[piece.token], head = piece.unit / p.subgroups, sub = piece.unit % p.subgroups;
+            const int n = lengths[piece.token], head = p.subgroups == 1 ? piece.unit : piece.unit / p.subgroups;
+            const int sub = piece.unit - head * p.subgroups;
             const int first_query = head * group + sub * kQueries;
             const int queries = min(group - sub * kQueries, kQueries);
             // queries as columns of the first product: two neighbouring values and those 8 further on a 16-wide step
@@ -347,7 +378,7 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
                     q[c][k][1] = mine < queries ? *reinterpret_cast<const unsigned int*>(source + k * 16 + 8) : 0u;
                 }
             }
-            const bool mine_is_last = p.a.key != nullptr && piece.end == piece.blocks && (((n - 1) & 63) >> 4) == warp;
+            const bool mine_is_last = p.a.key != nullptr && piece.end == piece.blocks && (((n - 1) & 63) >> 4) == (warp & 3);
             uint4 new_key, new_value;
             if (mine_is_last && lane < D / 8) {
                 new_key = *reinterpret_cast<const uint4*>(p.a.key + piece.token * p.a.k.token + head * p.a.k.head + lane * 8);
@@ -363,8 +394,17 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
                 for (int i = 0; i < D / 16; ++i) o[c][i][0] = o[c][i][1] = o[c][i][2] = o[c][i][3] = 0.f;
             }
             for (int b = piece.begin; b < piece.end; ++b) {
+                const bool mine = turn == team;
+                if (++turn == kTeams) turn = 0;
+                if (!mine) {
+                    if (++stage == p.stages) {
+                        stage = 0;
+                        ++round;
+                    }
+                    continue;
+                }
                 ok = ok && prefill::mbar_wait_warp(&ctl->full[stage], round & 1, &ctl->abort_flag);
-                if (!ok) continue;   // the barriers below are for all four warps
+                if (!ok) continue;   // the barriers below are for all warps
                 unsigned char* keys = ring + static_cast<size_t>(stage) * 2 * kTile;
                 unsigned char* values = keys + kTile;
                 const unsigned int mask = static_cast<unsigned int>(ctl->mask[stage] >> key0) & 0xffffu;
@@ -472,7 +512,7 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
                     ++round;
                 }
             }
-            // the four warps' shares of the piece
+            // the warps' shares of the piece
 #pragma unroll
             for (int c = 0; c < N; ++c)
 #pragma unroll
@@ -637,9 +677,11 @@ Shape shape_of(const AttentionArgs& a, int sms) {
     s.ctas = static_cast<int>(most < sms ? most : sms);
     s.joined = blocks > kWholeBlocks;
     const int tile = 2 * kBlock * a.head_dim * 2;
-    const int rest = kWarps * s.rows * (a.head_dim + 4) * 4 + static_cast<int>(sizeof(Control4)) + (3 * a.tokens + 1) * 4;
+    const int teams = a.head_dim == 64 ? kTeams<64> : kTeams<128>, warps = 4 * teams;
+    const int rest = warps * s.rows * (a.head_dim + 4) * 4 + static_cast<int>(sizeof(Control4)) + (3 * a.tokens + 1) * 4;
     s.stages = (kSmemLimit - rest) / tile;
     if (s.stages > kMaxStages) s.stages = kMaxStages;
+    s.stages -= s.stages % teams;
     s.smem = s.stages * tile + rest;
     const size_t pieces = static_cast<size_t>(s.ctas) * 2 * s.rows;
     s.stats = pieces * a.head_dim * 4;
@@ -665,7 +707,7 @@ cudaError_t launch_decode(const CUtensorMap& keys, const CUtensorMap& values, co
         if (err != cudaSuccess) return err;
         if (device < 64) configured.fetch_or(1ull << device, std::memory_order_relaxed);
     }
-    cudaError_t err = launch_early(decode_attention_kernel<T, D, N>, dim3(s.ctas), kThreads, s.smem, 1, stream, keys, values,
+    cudaError_t err = launch_early(decode_attention_kernel<T, D, N>, dim3(s.ctas), kThreads<D>, s.smem, 1, stream, keys, values,
                                    args);
     if (err == cudaSuccess && s.joined) err = launch_join<T, D>(args, s, stream);
     return err;
