@@ -56,7 +56,7 @@ struct DecodeArgs {
 
 struct Control4 {
     unsigned long long full[kMaxStages], empty[kMaxStages], mask[kMaxStages];
-    float stats[8][16][2];
+    float2 stats[8][16];   // of every warp and query: maximum, sum
     int warp_sums[9];
     int abort_flag;
 };
@@ -256,7 +256,9 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
     deal.tokens = p.a.tokens;
     deal.units = p.a.kv_heads * p.subgroups;
     deal.total = static_cast<long long>(first_block[p.a.tokens]) * deal.units;
-    deal.per = max((deal.total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kLeastBlocks));
+    deal.per = deal.total >> 31 == 0 ? (static_cast<unsigned int>(deal.total) + gridDim.x - 1) / gridDim.x
+                                     : (deal.total + gridDim.x - 1) / gridDim.x;
+    deal.per = max(deal.per, static_cast<long long>(kLeastBlocks));
     long long run_begin = min(blockIdx.x * deal.per, deal.total);
     long long run_end = min(run_begin + deal.per, deal.total);
     if (p.splits == nullptr) {   // no unit is cut: runs go from unit to unit
@@ -512,32 +514,20 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
                     ++round;
                 }
             }
-            // the warps' shares of the piece
-#pragma unroll
-            for (int c = 0; c < N; ++c)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    l[c][i] = shuffled_sum(l[c][i]);
-                    if (lane < 4) {
-                        ctl->stats[warp][c * 8 + lane * 2 + i][0] = m[c][i];
-                        ctl->stats[warp][c * 8 + lane * 2 + i][1] = l[c][i];
-                    }
-                }
-            named_barrier(kConsumerBarrier, kWarps * 32);
+            // the warps' shares of the piece, every one relative to its own maximum
 #pragma unroll
             for (int c = 0; c < N; ++c)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int mine = c * 8 + (lane & 3) * 2 + i;
-                    float highest = -INFINITY;
-                    for (int other = 0; other < kWarps; ++other) highest = fmaxf(highest, ctl->stats[other][mine][0]);
-                    const float factor = prefill::exp2_approx(m[c][i] - finite_base(highest));
+                    l[c][i] = shuffled_sum(l[c][i]);
+                    if (lane < 4) ctl->stats[warp][mine] = make_float2(m[c][i], l[c][i]);
                     if (mine < queries) {
                         float* to = merge + (warp * kQueries + mine) * kMergeRow + (lane >> 2);
 #pragma unroll
                         for (int t = 0; t < D / 16; ++t) {
-                            to[t * 16] = o[c][t][i] * factor;
-                            to[t * 16 + 8] = o[c][t][i + 2] * factor;
+                            to[t * 16] = o[c][t][i];
+                            to[t * 16 + 8] = o[c][t][i + 2];
                         }
                     }
                 }
@@ -548,16 +538,21 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
                 const int mine = i / (D / 4), c = i % (D / 4) * 4;
                 float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
                 float highest = -INFINITY, total = 0.f;
-                for (int other = 0; other < kWarps; ++other) highest = fmaxf(highest, ctl->stats[other][mine][0]);
+                float2 share[kWarps];
+#pragma unroll
                 for (int other = 0; other < kWarps; ++other) {
-                    total += ctl->stats[other][mine][1] *
-                             prefill::exp2_approx(ctl->stats[other][mine][0] - finite_base(highest));
-                    const float4 v =
-                        *reinterpret_cast<const float4*>(merge + (other * kQueries + mine) * kMergeRow + c);
-                    sum.x += v.x;
-                    sum.y += v.y;
-                    sum.z += v.z;
-                    sum.w += v.w;
+                    share[other] = ctl->stats[other][mine];
+                    highest = fmaxf(highest, share[other].x);
+                }
+#pragma unroll
+                for (int other = 0; other < kWarps; ++other) {
+                    const float4 v = *reinterpret_cast<const float4*>(merge + (other * kQueries + mine) * kMergeRow + c);
+                    const float factor = prefill::exp2_approx(share[other].x - finite_base(highest));
+                    total = fmaf(factor, share[other].y, total);
+                    sum.x = fmaf(factor, v.x, sum.x);
+                    sum.y = fmaf(factor, v.y, sum.y);
+                    sum.z = fmaf(factor, v.z, sum.z);
+                    sum.w = fmaf(factor, v.w, sum.w);
                 }
                 if (whole) {
                     store_output<T>(p.a.out + (static_cast<size_t>(piece.token) * p.a.heads + first_query + mine) * D + c,
