@@ -14,6 +14,8 @@ parts of it this backend keeps):
 ``GreedyGenerator``                 compiled prefill + decode loop over one KV state
 ``PagedState``                      the tensors of a paged key-value cache, and its operators:
 ``paged_reserve``, ``paged_append``, ``paged_kv_attention``, ``paged_prefill_attention``
+``PagedDecoder``                    any tokens of many requests through a model over a ``PagedState``
+``PagedGenerator``                  prompts of any lengths, admitted and ended over one paged cache
 ``bucketed`` / ``PaddingDependence`` prompts of any length through a few fixed-shape compiles
 ``register_transformers_attention`` the ``"megabake"`` attention implementation for HF models
 ``CompilerError``                   every refusal, with a staged diagnostic
@@ -24,7 +26,7 @@ from .ops import attention, kv_attention
 
 __all__ = [
     "CompilerDiagnostic", "CompilerError", "DecodeStep", "GreedyGenerator", "GroupedStateDecoder",
-    "PaddingDependence", "PagedBatch", "PagedState",
+    "PaddingDependence", "PagedBatch", "PagedDecoder", "PagedGenerator", "PagedState",
     "PrefillLogits", "StatefulDecoder", "StatefulPrefill", "attention", "bucketed",
     "graphed", "kv_attention", "make_backend", "paged_append", "paged_kv_attention",
     "paged_prefill_attention", "paged_reserve", "register_transformers_attention",
@@ -39,8 +41,8 @@ def __getattr__(name):
     if name in ("graphed", "GraphedCall", "BoundDecoder"):
         from . import engine
         return getattr(engine, name)
-    if name in ("DecodeStep", "GroupedStateDecoder", "PrefillLogits", "StatefulDecoder",
-                "StatefulPrefill", "register_transformers_attention"):
+    if name in ("DecodeStep", "GroupedStateDecoder", "PagedDecoder", "PrefillLogits",
+                "StatefulDecoder", "StatefulPrefill", "register_transformers_attention"):
         from . import hf
         return getattr(hf, name)
     if name in ("bucketed", "PaddingDependence"):
@@ -50,7 +52,7 @@ def __getattr__(name):
                 "paged_reserve"):
         from . import paged
         return getattr(paged, name)
-    if name == "GreedyGenerator":
-        from .generate import GreedyGenerator
-        return GreedyGenerator
+    if name in ("GreedyGenerator", "PagedGenerator"):
+        from . import generate
+        return getattr(generate, name)
     raise AttributeError(name)

@@ -15,7 +15,7 @@ import torch
 from . import runtime as rt
 from .engine import graphed
 from .frontend import make_backend
-from .hf import StatefulDecoder, StatefulPrefill
+from .hf import PagedDecoder, StatefulDecoder, StatefulPrefill
 
 
 class GreedyGenerator:
@@ -136,3 +136,125 @@ class GreedyGenerator:
         if int(self._cursor.max()) != new_tokens or int(self._cursor.min()) != new_tokens:
             raise RuntimeError("the device-side loop produced an unexpected number of tokens")
         return self._picked[:, :new_tokens].clone()
+
+
+class PagedGenerator:
+    """Greedy generation of many prompts of any lengths over one paged cache: requests take a row of the table as one
+    becomes free and pages of the pool as they grow, and give both back when they end.
+
+    ``requests`` rows run at once; ``pages`` pages of ``page_size`` tokens are shared by them (default: enough for all
+    of them to grow to ``capacity``).  A prompt is admitted when its row and the pages for all of its tokens are there, so
+    no request is refused later.  Decode steps are one CUDA graph: pages, attention, projections and the greedy
+    pick, without the host; ids are read once at the end."""
+
+    def __init__(self, model: torch.nn.Module, requests: int, capacity: int, *, page_size: int = 64,
+                 pages: int | None = None):
+        self.decoder = PagedDecoder(model).eval()
+        self.state = self.decoder.make_paged_state(requests, capacity, page_size=page_size, pages=pages)
+        self.requests, self.pages = requests, self.state.free_pages.numel()
+        self.device = self.state.lengths.device
+        int32 = torch.int32
+        # the row behind the last one takes what belongs to no request
+        self._picked = torch.zeros(requests + 1, dtype=torch.int64, device=self.device)
+        self._produced = torch.zeros(requests + 1, dtype=torch.int64, device=self.device)
+        self._log = torch.zeros(requests + 1, self.state.capacity, dtype=torch.int64, device=self.device)
+        self._counts = torch.zeros(requests, dtype=int32, device=self.device)
+        self._graph = None
+
+    def _pages_of(self, tokens: int) -> int:
+        return -(-tokens // self.state.page_size)
+
+    def _pick(self, logits: torch.Tensor, rows: torch.Tensor) -> None:
+        """The greedy pick of every row of ``logits`` becomes the next id of request ``rows`` and is logged."""
+        picked = torch.empty(logits.shape[0], dtype=torch.int64, device=self.device)
+        rt.greedy_advance(logits, picked)
+        rows = torch.where(rows < 0, self.requests, rows).long()
+        self._picked.index_copy_(0, rows, picked)
+        self._log.index_put_((rows, self._produced[rows]), picked)
+        self._produced.index_add_(0, rows, (rows < self.requests).long())
+
+    def _decode(self) -> None:
+        batch = self.state.reserve(self._counts, self.requests)
+        rows = torch.where(batch.rows < 0, self.requests, batch.rows).long()
+        logits = self.decoder(self._picked[rows], batch, self.state, one_token=True)
+        self._pick(logits, batch.rows)
+
+    def _decode_step(self) -> None:
+        if self._graph is None:
+            self._decode()          # once without a graph: what is set up lazily is set up here
+            torch.cuda.synchronize(self.device)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                self._decode()
+            self._graph = graph
+        else:
+            self._graph.replay()
+
+    def _prefill(self, prompts: dict[int, torch.Tensor]) -> None:
+        """Admit ``prompts`` (by row) and pick their first new ids."""
+        total = sum(p.numel() for p in prompts.values())
+        counts = torch.zeros(self.requests, dtype=torch.int32)
+        last, rows, at = [], sorted(prompts), 0
+        for row in rows:
+            counts[row] = prompts[row].numel()
+            at += prompts[row].numel()
+            last.append(at - 1)
+        batch = self.state.reserve(counts.to(self.device), total)
+        ids = torch.cat([prompts[row].flatten() for row in rows]).to(self.device, torch.int64)
+        logits = self.decoder(ids, batch, self.state, tokens=torch.tensor(last, device=self.device))
+        self._pick(logits, torch.tensor(rows, device=self.device))
+
+    @torch.no_grad()
+    def __call__(self, prompts: list[torch.Tensor], new_tokens: int | list[int]) -> list[torch.Tensor]:
+        """``new_tokens`` ids (one number, or one per prompt) after each of ``prompts`` (1-d, any lengths)."""
+        wanted = [new_tokens] * len(prompts) if isinstance(new_tokens, int) else list(new_tokens)
+        if len(wanted) != len(prompts):
+            raise ValueError("new_tokens must be one number, or one per prompt")
+        for prompt, count in zip(prompts, wanted):
+            # the last id is picked and never fed back
+            if prompt.numel() < 1 or count < 1 or prompt.numel() + count - 1 > self.state.capacity or \
+                    self._pages_of(prompt.numel() + count - 1) > self.pages:
+                raise ValueError("every prompt needs a token, a new one, and room for them in a row and in the pool")
+        with torch.cuda.device(self.device):
+            return self._run(prompts, wanted)
+
+    def _run(self, prompts: list[torch.Tensor], wanted: list[int]) -> list[torch.Tensor]:
+        self.state.reset()
+        self._produced.zero_()
+        waiting, running, done = list(range(len(prompts))), {}, {}   # running: row -> [prompt, ids produced]
+        free_pages, active = self.pages, None
+        while waiting or running:
+            admitted = {}
+            for row in range(self.requests):
+                if not waiting or row in running:
+                    continue
+                need = self._pages_of(prompts[waiting[0]].numel() + wanted[waiting[0]] - 1)
+                if need > free_pages:
+                    break
+                free_pages -= need
+                index = waiting.pop(0)
+                running[row] = [index, 1]
+                admitted[row] = prompts[index]
+            if admitted:
+                self._prefill(admitted)
+            else:
+                now = sorted(running)
+                if now != active:
+                    counts = torch.zeros(self.requests, dtype=torch.int32)
+                    counts[now] = 1
+                    self._counts.copy_(counts)
+                    active = now
+                self._decode_step()
+                for entry in running.values():
+                    entry[1] += 1
+            ended = [row for row, (index, count) in running.items() if count == wanted[index]]
+            if ended:
+                counts = torch.zeros(self.requests, dtype=torch.int32)
+                counts[ended] = -self.state.capacity
+                for row in ended:
+                    index, count = running.pop(row)
+                    done[index] = self._log[row, :count].clone()
+                    free_pages += self._pages_of(prompts[index].numel() + count - 1)
+                    self._produced[row] = 0
+                self.state.reserve(counts.to(self.device), 0)
+        return [done[index] for index in range(len(prompts))]

@@ -23,6 +23,8 @@ Two wrappers produce that convention:
                      wrapper (``tests/fixtures.py:236-238``): all key caches, then all value
                      caches, then all valid lengths.
 
+``PagedDecoder`` the same loop over a paged cache (``paged.PagedState``), for packed tokens of requests of any lengths.
+
 ``megabake_attention_forward``, ``megabake_decode_attention``,
 ``register_transformers_attention`` and ``_PassThroughLayer`` below restate the reference's
 ``src/megabake/fx_handler/hf_attention.py:28-162`` closely -- same branches, same error texts:
@@ -40,6 +42,7 @@ from transformers.cache_utils import Cache, CacheLayerMixin
 
 from . import ops as _ops  # noqa: F401  (registers torch.ops.megabake.*)
 from .ops import attention as _attention_op
+from .paged import PagedBatch, PagedState, paged_append, paged_kv_attention, paged_prefill_attention
 
 ATTENTION_IMPLEMENTATION = "megabake"
 
@@ -341,3 +344,50 @@ class StatefulPrefill(StatefulDecoder):
         batch, tokens = input_ids.shape
         positions = torch.arange(tokens, device=input_ids.device)[None].expand(batch, -1)
         return super().forward(input_ids, positions, *state)
+
+
+class PagedDecoder(StatefulDecoder):
+    """The loop of ``StatefulDecoder`` over a paged cache: ``forward(input_ids[tokens], batch, state) -> logits``.
+
+    ``batch`` is what ``state.reserve`` returned for these tokens: packed, one request after the other, each at its own
+    length.  With ``one_token`` every request has one at most (a decode step): its key and value are appended on the
+    way; otherwise requests may have any number (prompts, chunks of them, decoding requests among them).
+    ``tokens`` (int64) selects the places whose logits are wanted.  Not compiled: projections, norms and the MLP are the
+    model's own modules, attention and the cache are the native operators; places behind the last token are computed like
+    the others and mean nothing, so that a step of fixed size can be captured in a CUDA graph."""
+
+    def make_paged_state(self, requests: int, capacity: int, **options) -> PagedState:
+        """A ``PagedState`` of this model's layers and heads."""
+        weight = self.model.embed_tokens.weight
+        options = {"dtype": weight.dtype, "device": weight.device, **options}
+        return PagedState(self.layer_count, requests, capacity, self.kv_heads, self.head_dim, **options)
+
+    @torch.no_grad()
+    def forward(self, input_ids: torch.Tensor, batch: PagedBatch, state: PagedState, *, one_token: bool = False,
+                tokens: torch.Tensor | None = None) -> torch.Tensor:
+        if input_ids.shape != batch.positions.shape:
+            raise ValueError(f"{tuple(input_ids.shape)} ids for {batch.positions.numel()} places")
+        if len(state.key_pages) != self.layer_count:
+            raise ValueError(f"a state of {len(state.key_pages)} layers for {self.layer_count}")
+        hidden = self.model.embed_tokens(input_ids[None])
+        rotary = self.model.rotary_emb(hidden, batch.positions[None])
+        dim, count = self.head_dim, input_ids.shape[0]
+        for index, layer in enumerate(self.model.layers):
+            module, normalized = layer.self_attn, layer.input_layernorm(hidden)
+            query = module.q_proj(normalized).view(1, count, -1, dim)
+            key = module.k_proj(normalized).view(1, count, -1, dim)
+            value = module.v_proj(normalized).view(count, -1, dim)
+            rotate = sys.modules[type(module).__module__].apply_rotary_pos_emb
+            query, key = rotate(query, key, rotary[0], rotary[1], unsqueeze_dim=2)
+            pools = (state.key_pages[index], state.value_pages[index])
+            if one_token:
+                mixed = paged_kv_attention(query[0], key[0], value, *pools, state.block_table, state.lengths,
+                                           batch.rows, scale=module.scaling)
+            else:
+                paged_append(key[0], value, *pools, batch.slots)
+                mixed = paged_prefill_attention(query[0], *pools, state.block_table, state.lengths, batch.offsets,
+                                                scale=module.scaling)
+            hidden = hidden + module.o_proj(mixed.view(1, count, -1))
+            hidden = hidden + layer.mlp(layer.post_attention_layernorm(hidden))
+        hidden = self.model.norm(hidden)[0]
+        return self.lm_head(hidden if tokens is None else hidden[tokens])
