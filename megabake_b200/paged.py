@@ -14,7 +14,7 @@ are the first ``free_count`` (int32 ``[1]``) entries of the stack ``free_pages``
 
 Each is one call into the native library on torch's current stream: nothing is synchronised, all of them can be
 captured in a CUDA graph, and a scratch buffer is the call's own.  bf16 and fp16; heads of 64, 128 or 256;
-any number of query heads per key head; pages of 8 to 1,024 tokens (a power of two); pools and rows may have any
+any number of query heads per key head (128 for prompts); pages of 8 to 1,024 tokens (a power of two); pools and rows may have any
 strides that are multiples of 16 bytes.  Scores, softmax statistics and sums are fp32 and outputs are rounded
 once -- unlike ``kv_attention``, whose rounding points are the reference's eager ones.  Inference only.
 

@@ -638,6 +638,87 @@ def test_status_stays_when_nothing_went_wrong():
     assert status.item() == 0
 
 
+@pytest.mark.parametrize("heads", [(3, 1, 64), (9, 1, 256)])
+def test_the_most_requests(heads):
+    """2,048 rows, of which every 50th is compared: the tables of the kernels take shared memory from their rings."""
+    count, kv_heads, dim = heads
+    new = [(i * 7) % 5 for i in range(2048)]
+    lengths = [n + (i * 31) % 150 for i, n in enumerate(new)]
+    cache = Cache(lengths, kv_heads, dim, 16, BF16, 1)
+    query = _normal((2048, count, dim), cache.g, BF16)
+    out = paged_kv_attention(query, None, None, *cache.pools, cache.table, cache.lengths)
+    for r in range(0, 2048, 50):
+        expected = reference.attend(query[r], *cache.pools, cache.table[r], lengths[r], dim ** -0.5)
+        _check(out[r], expected, lengths[r], BF16, reference.decode_rounding(BF16))
+    offsets = [0]
+    for n in new:
+        offsets.append(offsets[-1] + n)
+    query = _normal((offsets[-1], count, dim), cache.g, BF16)
+    out = paged_prefill_attention(query, *cache.pools, cache.table, cache.lengths, _int32(offsets))
+    for r in range(0, 2048, 50):
+        for j in range(new[r]):
+            keys = lengths[r] - new[r] + j + 1
+            expected = reference.attend(query[offsets[r] + j], *cache.pools, cache.table[r], keys, dim ** -0.5)
+            _check(out[offsets[r] + j], expected, keys, BF16, reference.prompt_rounding(BF16))
+    rows = torch.zeros(2049, dtype=torch.int32, device="cuda")
+    with pytest.raises(CompilerError, match="2048"):
+        paged_kv_attention(_normal((2049, count, dim), cache.g, BF16), None, None, *cache.pools, cache.table, cache.lengths, rows)
+
+
+def test_query_heads_per_key_head():
+    """Up to 128 for prompts; single tokens take any number."""
+    cache = Cache([70], 1, 64, 16, BF16, 2)
+    for count in (128, 130):
+        query = _normal((1, count, 64), cache.g, BF16)
+        expected = reference.attend(query[0], *cache.pools, cache.table[0], 70, 0.125)
+        out = paged_kv_attention(query, None, None, *cache.pools, cache.table, cache.lengths)
+        _check(out[0], expected, 70, BF16, reference.decode_rounding(BF16))
+        if count == 128:
+            out = paged_prefill_attention(query, *cache.pools, cache.table, cache.lengths, _int32([0, 1]))
+            _check(out[0], expected, 70, BF16, reference.prompt_rounding(BF16))
+        else:
+            with pytest.raises(CompilerError):
+                paged_prefill_attention(query, *cache.pools, cache.table, cache.lengths, _int32([0, 1]))
+
+
+def test_output_in_the_place_of_the_queries():
+    cache, query = _step_inputs(8, lengths=(5000, 77, 131, 20000))
+    offsets = _int32([0, 1, 2, 2, 4])
+    for call in (lambda q, out: paged_kv_attention(q, None, None, *cache.pools, cache.table, cache.lengths, out=out),
+                 lambda q, out: paged_prefill_attention(q, *cache.pools, cache.table, cache.lengths, offsets, out=out)):
+        expected, q = call(query, None), query.clone()
+        assert call(q, q) is q and torch.equal(q, expected)
+
+
+FIRST_CALL = """
+import torch
+from megabake_b200 import PagedState, paged_append, paged_kv_attention, paged_prefill_attention
+state = PagedState(1, 2, 4096, 1, 64, device="cuda")
+counts = torch.ones(2, dtype=torch.int32, device="cuda")
+rows = torch.ones(2, 1, 64, dtype=torch.bfloat16, device="cuda")
+pools = (state.key_pages[0], state.value_pages[0])
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    batch = state.reserve(counts, 2)
+    a = paged_kv_attention(rows, rows, rows, *pools, state.block_table, state.lengths, batch.rows)
+    paged_append(rows, rows, *pools, batch.slots)
+    b = paged_prefill_attention(rows, *pools, state.block_table, state.lengths, batch.offsets)
+for step in range(3):
+    graph.replay()
+torch.cuda.synchronize()
+assert state.lengths.tolist() == [3, 3] and bool((a == 1).all()) and bool((b == 1).all())
+print("captured")
+"""
+
+
+def test_the_first_call_of_a_process_is_captured():
+    import subprocess
+    import sys
+
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL], capture_output=True, text=True, timeout=250)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
 # ---------------------------------------------------------------------------------------
 # Together, as a server uses them
 # ---------------------------------------------------------------------------------------
