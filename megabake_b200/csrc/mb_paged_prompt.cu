@@ -563,18 +563,22 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                             mbar_arrive_expect_tx(&ctl->full[stage], boxes * kChunks * rows * 128);
                         __syncwarp();
                         unsigned char* to = ring + static_cast<size_t>(stage) * C::kTileBytes;
-#pragma unroll 1
-                        for (int i = 0; i < per_block; ++i) {
-                            const int id = __shfl_sync(0xffffffffu, mine, (j << per_shift) + i);
+                        const CUtensorMap* map = kind == 0 ? &key_map : &value_map;
+                        if (per_block == 1) {
+                            const int id = __shfl_sync(0xffffffffu, mine, j);
                             if (id >= 0 && elect_one()) {
 #pragma unroll
                                 for (int c = 0; c < kChunks; ++c)
-                                    tma_load_column(to + c * kBlock * 128 + i * rows * 128,
-                                                    kind == 0 ? &key_map : &value_map, c * 64, place, u.head, id,
-                                                    &ctl->full[stage]);
+                                    tma_load_column(to + c * kBlock * 128, map, c * 64, place, u.head, id, &ctl->full[stage]);
                             }
-                            __syncwarp();
+                        } else {   // a box a lane: a table entry's rows of one 128-byte column
+                            const int box = lane & (per_block - 1), column = lane >> per_shift;
+                            const int id = __shfl_sync(0xffffffffu, mine, (j << per_shift) + box);
+                            if (column < kChunks && id >= 0)
+                                tma_load_column(to + (column * kBlock + (box << rows_shift)) * 128, map, column * 64, place,
+                                                u.head, id, &ctl->full[stage]);
                         }
+                        __syncwarp();
                         if (++stage == p.ring) {
                             stage = 0;
                             ++round;
