@@ -466,10 +466,10 @@ enum mb_element { MB_BF16 = 0, MB_FP16 = 1 };
  * last: -1, 0, -1.  granted[r]: tokens granted, or dropped (negative).                            */
 typedef struct mb_paged_reserve_args {
     int32_t requests;         /* rows, at most 2048                                       */
-    int32_t width;            /* pages per row of the table; width * page_size < 2^31     */
+    int32_t width;            /* pages per row of the table; width * page_size <= 2^30    */
     int32_t pages;            /* of the pool: entries of free_pages                       */
     int32_t page_size;
-    int32_t max_tokens;       /* entries of slots, positions and rows; may be 0           */
+    int32_t max_tokens;       /* entries of slots, positions and rows: 0 .. 2^30          */
     int32_t reserved;
     uint64_t counts;          /* int32 [requests]                                         */
     uint64_t lengths;         /* int32 [requests], updated                                */
@@ -516,7 +516,7 @@ typedef struct mb_paged_attention_args {
     int32_t tokens;           /* rows of query                                            */
     int32_t requests;         /* rows of the block table                                  */
     int32_t heads, kv_heads, head_dim;
-    int32_t width, pages, page_size;
+    int32_t width, pages, page_size;   /* width * page_size <= 2^30                       */
     int32_t zero_rest;        /* mb_paged_prefill                                         */
     float scale;
     int32_t reserved;

@@ -12,6 +12,8 @@ namespace mb {
 namespace paged {
 
 constexpr int kMaxRows = 2048;   // requests of a table, and tokens of a step of one token a request
+// Of a row of the table, and places of mb_paged_reserve: what is rounded up to a block or a grid's stride stays an int.
+constexpr int kMaxTokens = 1 << 30;
 
 struct Strides2 {
     long long token, head;   // elements
@@ -33,7 +35,7 @@ struct AttentionArgs {
 };
 
 // Weights are 2^(log2(e) (score - highest) + shift).  fp16: up by 2^15, so that small ones keep their digits when they
-// are rounded to 16 bits; bf16: down by 2^31, so that no sum over a context, which has fewer than 2^31 keys,
+// are rounded to 16 bits; bf16: down by 2^31, so that no sum over a context, which has at most 2^30 keys,
 // overflows whatever the values are (fp16 values cannot).
 constexpr float kLog2e = 1.4426950408889634f;
 template <typename T>

@@ -34,7 +34,10 @@ constexpr int kWholeKeys = 1024;       // rows of the table that hold no more ar
 constexpr unsigned int kTmemColumns = 512;
 // A row's maximum may lag behind by this many powers of two before its sums are rescaled.
 constexpr float kLag = 8.f;
-constexpr int kPassAt = 48;            // keys of a block whose exponentials are done when the turn passes
+// Keys of a block whose exponentials are done when the turn passes to the other tile's warp (8,192 tokens of 128-wide heads:
+// 520 us at the end of the block, 505 anywhere from 40 on; 517 without turns where it is 490 with them: both warps of a
+// scheduler then do their exponentials at the same time, and everything else).
+constexpr int kPassAt = 48;
 // As kWeightShift, with room for the lag.
 template <typename T>
 constexpr float kPromptShift = 7.f;
@@ -342,6 +345,15 @@ __device__ __forceinline__ bool wait_warp(unsigned long long* bar, unsigned int 
 // as they lie in the pages (rows are the reduction).  A thread has a row: no shuffles.  Outputs stay in tensor
 // memory and are rescaled only when a row's maximum has grown by more than 2^8 since the last time.  256-wide
 // heads: one query tile.
+//
+// Measured (us; floor at the measured GEMM rate): 8,192 tokens, 32/8 heads of 128: 488 in a graph of few passes (332), 1.13
+// PFLOP/s; 509 tokens after 16,000, 8/1 heads of 256: 94 (41); seven prompts of up to 1,031, 32/8 heads of 64, pages of
+// 16: 60 (8).  What bounds it: a block of 64 keys takes 1,700 to 1,900 cycles, of which the exponentials of its two tiles,
+// 8 cycles a warp and instruction, are 1,024, and the products 1,280 (64 keys a product of scores read the queries from shared
+// memory for 64 columns, at two thirds of the rate that 128 columns reach); between units there are the
+// outputs.  Blocks of 128 keys leave one slot a tile, and the chain scores -> weights -> outputs -> scores of a tile then
+// takes 3,300 cycles (558 us).  A quarter to five eighths of the exponentials by a polynomial on the multipliers took 562
+// to 675 us instead of 553.  The code matters as much: a third less of it around the same loops was worth 520 -> 508 us.
 // ---------------------------------------------------------------------------------------
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -590,8 +602,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         }
     } else if (warp == 9 || (kTiles == 2 && warp == 10)) {
         // ---- products of one query tile.  One thread issues them, in one place for the scores and one for the outputs: what
-        // it does between two products is time the tensor core waits, unless the other tile's thread has something for
-        // it ({MMA_NOTE}).
+        // it does between two products is time the tensor core waits, unless the other tile's thread has something for it.
+        // (One thread for both tiles was busy 3,000 cycles a block and softmax warps waited 1,900 of them; with a thread a
+        // tile a block takes 1,700 to 1,900 and they wait 150.)
         constexpr unsigned int kFormat = std::is_same_v<T, __half> ? 0u : (1u << 7) | (1u << 10);
         constexpr unsigned int kIdescS = (1u << 4) | kFormat | (static_cast<unsigned int>(kBlock >> 3) << 17) |
                                          (static_cast<unsigned int>(kRows >> 4) << 24);

@@ -38,6 +38,8 @@ __all__ = ["PagedBatch", "PagedState", "paged_append", "paged_kv_attention", "pa
 _ELEMENTS = {torch.bfloat16: 0, torch.float16: 1}
 _HEAD_DIMS = (64, 128, 256)
 _MAX_REQUESTS = 2048
+_MAX_TOKENS = 1 << 30     # of a row of the table, and places of a reservation
+_MAX_COUNT = 0x7fffffff   # of pages, and of tokens
 
 
 class PagedBatch(NamedTuple):
@@ -164,7 +166,8 @@ def _inference_only(*tensors) -> None:
 
 def _pools(key_pages: torch.Tensor, value_pages: torch.Tensor) -> tuple:
     if key_pages.dtype not in _ELEMENTS or key_pages.dim() != 4 or key_pages.shape[3] not in _HEAD_DIMS or \
-            not _page_size_covered(key_pages.shape[1]) or key_pages.shape[0] < 1 or key_pages.shape[2] < 1:
+            not _page_size_covered(key_pages.shape[1]) or not 1 <= key_pages.shape[0] <= _MAX_COUNT or \
+            key_pages.shape[2] < 1:
         fail("input-binding", "key_pages must be bf16 or fp16 [pages, page_size, kv_heads, head_dim] with head_dim 64, "
                               "128 or 256 and page_size a power of two from 8 to 1024, got "
                               f"{key_pages.dtype} {tuple(key_pages.shape)}")
@@ -221,9 +224,10 @@ def _reserve_fields(counts, lengths, block_table, free_pages, free_count, page_s
     device = counts.device
     requests, width = block_table.shape
     if device.type != "cuda" or not 1 <= requests <= _MAX_REQUESTS or width < 1 or not _page_size_covered(page_size) or \
-            max_tokens < 0 or max_tokens > 0x7fffffff or width * page_size > 0x7fffffff or free_pages.numel() < 1:
+            max_tokens < 0 or max_tokens > _MAX_TOKENS or width * page_size > _MAX_TOKENS or \
+            not 1 <= free_pages.numel() <= _MAX_COUNT:
         fail("input-binding", f"paged_reserve needs 1..{_MAX_REQUESTS} requests on a CUDA device, pages of 8 to 1024 tokens "
-                              "(a power of two), rows below 2**31 tokens and max_tokens >= 0, got "
+                              "(a power of two), rows of at most 2**30 tokens and max_tokens up to that, got "
                               f"{tuple(block_table.shape)} pages of {page_size} on {device}, max_tokens {max_tokens}")
     for name, tensor, numel in (("counts", counts, requests), ("lengths", lengths, requests),
                                 ("block_table", block_table, requests * width),
@@ -260,7 +264,7 @@ _APPEND_ADDRESSES = struct.Struct("=5Q")
 def _append_fields(key, value, key_pages, value_pages, slots) -> tuple:
     kpool, vpool = _pools(key_pages, value_pages)
     pages, page_size, kv_heads, head_dim = key_pages.shape
-    if key.dim() != 3 or key.device.type != "cuda":
+    if key.dim() != 3 or key.shape[0] > _MAX_COUNT or key.device.type != "cuda":
         fail("input-binding", f"key must be [tokens, kv_heads, head_dim] on a CUDA device, got {tuple(key.shape)} on "
                               f"{key.device}")
     tokens = key.shape[0]
@@ -311,12 +315,12 @@ def _attention_fields(what, query, key, value, key_pages, value_pages, block_tab
     pages, page_size, kv_heads, head_dim = key_pages.shape
     device = query.device
     if query.dim() != 3 or query.shape[2] != head_dim or query.shape[1] % kv_heads or query.shape[1] < 1 or \
-            device.type != "cuda":
+            query.shape[0] > _MAX_COUNT or device.type != "cuda":
         fail("input-binding", f"query must be [tokens, heads, {head_dim}] on a CUDA device with heads a multiple of "
                               f"{kv_heads}, got {tuple(query.shape)} on {device}")
     tokens, heads = query.shape[0], query.shape[1]
-    if block_table.dim() != 2 or min(block_table.shape) < 1 or block_table.shape[1] * page_size > 0x7fffffff:
-        fail("input-binding", f"block_table must be [requests, width] with rows below 2**31 tokens, got "
+    if block_table.dim() != 2 or min(block_table.shape) < 1 or block_table.shape[1] * page_size > _MAX_TOKENS:
+        fail("input-binding", f"block_table must be [requests, width] with rows of at most 2**30 tokens, got "
                               f"{tuple(block_table.shape)} pages of {page_size}")
     requests, width = block_table.shape
     if requests > _MAX_REQUESTS or (not prefill and tokens > _MAX_REQUESTS):

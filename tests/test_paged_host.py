@@ -43,7 +43,8 @@ def _attention_args(**changes):
     (dict(counts=0), INVALID), (dict(free_count=0), INVALID), (dict(slots=0), INVALID), (dict(rows=0), INVALID),
     (dict(slots=4100), INVALID), (dict(lengths=4097), INVALID), (dict(requests=2049), UNSUPPORTED),
     (dict(page_size=4), UNSUPPORTED), (dict(page_size=48), UNSUPPORTED), (dict(page_size=2048), UNSUPPORTED),
-    (dict(width=1 << 27, page_size=16), UNSUPPORTED),
+    (dict(width=1 << 27, page_size=16), UNSUPPORTED), (dict(width=(1 << 26) + 1, page_size=16), UNSUPPORTED),
+    (dict(max_tokens=(1 << 30) + 1), UNSUPPORTED),
 ])
 def test_reserve_entry_refuses(changes, code):
     assert rt.load_library().mb_paged_reserve(ctypes.byref(_reserve_args(**changes)), None) == code
@@ -64,6 +65,7 @@ def test_append_entry_refuses(changes, code):
     (dict(value=0), INVALID), (dict(out=8), INVALID), (dict(query_head=4), INVALID), (dict(block_table=0), INVALID),
     (dict(block_table=4098), INVALID), (dict(key_pages=4104), INVALID), (dict(element=2), UNSUPPORTED),
     (dict(head_dim=80), UNSUPPORTED), (dict(page_size=24), UNSUPPORTED), (dict(width=1 << 27), UNSUPPORTED),
+    (dict(width=(1 << 26) + 1), UNSUPPORTED),
 ])
 def test_attention_entries_refuse(prefill, changes, code):
     lib = rt.load_library()
