@@ -36,9 +36,10 @@ constexpr int kThreads = 32 * (kWarps<D> + 1);
 constexpr int kMaxStages = 16;
 constexpr int kSmemLimit = 227 * 1024;
 constexpr int kConsumerBarrier = 1;
-constexpr int kLeastBlocks = 2;     // of a run
-// Rows of the table that hold no more are not cut: one launch and no scratch (33 keys: 6.6 -> 5.7 us on the device and 2.5 us
-// less of the host), and a CTA has eight blocks within about the time that joining pieces takes.
+// Of a run, where units are cut (one of 2,048 keys, 9/3 heads of 64: 7.4 us; 1: 7.7, 4: 8.0).
+constexpr int kLeastBlocks = 2;
+// Rows of the table that hold no more are not cut: one launch and no scratch (33 keys: 6.7 -> 4.4 us on the
+// device), and a CTA has eight blocks within about the time that joining pieces takes.
 constexpr int kWholeBlocks = 8;
 
 // What a CTA leaves behind about the unit that it began and others finish.
@@ -194,7 +195,7 @@ __device__ __forceinline__ float finite_base(float m) { return m == -INFINITY ? 
 // Measured (us; floor at the measured copy bandwidth): 64 requests of 8,192 keys, 32/8 heads of 128: 318 to 326 (328), 6.6
 // TB/s; one of 131,071: 89 to 91 (82); 37 ragged ones of up to 4,099, 14/2 heads of 64, pages of 16: 20 (6), of which about 9 stream
 // and the rest is latency: 4,400 cycles until the first keys are asked for and 1,700 until they are there, two merges of
-// 2,000, the joining launch; one of 33 keys: 5.7.  Boxes issued by one lane, with 64-bit division for their places, instead
+// 2,000, the joining launch; one of 33 keys: 4.4.  Boxes issued by one lane, with 64-bit division for their places, instead
 // of a box a lane and 32-bit: 24.0 us for the ragged ones, then 22.0.
 // ---------------------------------------------------------------------------------------
 template <typename T, int D, int N>   // N: 8-query columns of a unit
@@ -266,7 +267,7 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
     deal.total = static_cast<long long>(first_block[p.a.tokens]) * deal.units;
     deal.per = deal.total >> 31 == 0 ? (static_cast<unsigned int>(deal.total) + gridDim.x - 1) / gridDim.x
                                      : (deal.total + gridDim.x - 1) / gridDim.x;
-    deal.per = max(deal.per, static_cast<long long>(kLeastBlocks));
+    deal.per = max(deal.per, p.splits != nullptr ? static_cast<long long>(kLeastBlocks) : 1);
     long long run_begin = min(blockIdx.x * deal.per, deal.total);
     long long run_end = min(run_begin + deal.per, deal.total);
     if (p.splits == nullptr) {   // no unit is cut: runs go from unit to unit

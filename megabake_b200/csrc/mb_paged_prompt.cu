@@ -29,8 +29,12 @@ constexpr int kSmemLimit = 227 * 1024;
 // What a unit costs besides its keys, in keys: its outputs, and the way from one to the next.  With 128 and 256, 8,192
 // tokens of 128-wide heads took 510 and 481 us (192: 492, 320: 484), seven prompts of 64-wide ones 72 and 78.
 __host__ __device__ constexpr int tile_cost(int head_dim) { return head_dim == 64 ? 128 : 256; }
-constexpr int kLeastKeys = 512;        // of a run, where units are cut
-constexpr int kWholeKeys = 1024;       // rows of the table that hold no more are not cut
+// Keys of a run at least, where units are cut.  A prompt of 1,000 tokens, 9/3 heads of 64: 128 keys 21.3 us, 256 21.8, 512
+// 24.2; 300 tokens after 2,000: 21.5, 20.5, 24.2; 64 after 3,000, 32/8 heads of 128: 29.5, 28.6, 30.0.
+constexpr int kLeastKeys = 256;
+// Rows of the table that hold no more are not cut: one launch and no scratch (19 tokens: 9.2 us, cut 15.6).  Rows of up to
+// 1,024 keys: 8 x 40 tokens after 700 uncut 27.9 us, cut 24.7; 4 x 600 36.2 and 34.0; one of 500 18.8 and 20.5.
+constexpr int kWholeKeys = 512;
 constexpr unsigned int kTmemColumns = 512;
 // A row's maximum may lag behind by this many powers of two before its sums are rescaled.
 constexpr float kLag = 8.f;
@@ -53,8 +57,9 @@ struct Config {
     static constexpr int kColumnO = 2 * kTiles * kBlock;     // tensor memory: two slots of scores a tile, then the outputs
 };
 
+// What a CTA leaves behind about the unit that it began and others finish.
 struct Split {
-    int request, head, tile, pieces;
+    int first, head, tokens, pieces;
 };
 
 struct PromptArgs {
@@ -347,8 +352,8 @@ __device__ __forceinline__ bool wait_warp(unsigned long long* bar, unsigned int 
 // heads: one query tile.
 //
 // Measured (us; floor at the measured GEMM rate): 8,192 tokens, 32/8 heads of 128: 488 in a graph of few passes (332), 1.13
-// PFLOP/s; 509 tokens after 16,000, 8/1 heads of 256: 94 (41); seven prompts of up to 1,031, 32/8 heads of 64, pages of
-// 16: 60 (8).  What bounds it: a block of 64 keys takes 1,700 to 1,900 cycles, of which the exponentials of its two tiles,
+// PFLOP/s; 509 tokens after 16,000, 8/1 heads of 256: 85 (41); seven prompts of up to 1,031, 32/8 heads of 64, pages of
+// 16: 59 (8).  What bounds it: a block of 64 keys takes 1,700 to 1,900 cycles, of which the exponentials of its two tiles,
 // 8 cycles a warp and instruction, are 1,024, and the products 1,280 (64 keys a product of scores read the queries from shared
 // memory for 64 columns, at two thirds of the rate that 128 columns reach); between units there are the
 // outputs.  Blocks of 128 keys leave one slot a tile, and the chain scores -> weights -> outputs -> scores of a tile then
@@ -990,7 +995,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                 *reinterpret_cast<float2*>(
                     p.stats + (static_cast<size_t>(blockIdx.x * 2 + (begin == 0 ? 1 : 0)) * kTiles * kRows + tile * kRows + r) * 2) =
                     make_float2(any && l != 0.f ? m : -INFINITY, l);
-                if (begin == 0) split = {u->request, u->head, u->tile, u->pieces};
+                if (begin == 0) split = {u->first, u->head, u->tokens, u->pieces};
             }
             prefill::tc_fence_before();
             __syncwarp();
@@ -1002,7 +1007,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             release_work();
         }
         if (tid == 0 && p.splits != nullptr)
-            *reinterpret_cast<int4*>(p.splits + blockIdx.x) = make_int4(split.request, split.head, split.tile, split.pieces);
+            *reinterpret_cast<int4*>(p.splits + blockIdx.x) = make_int4(split.first, split.head, split.tokens, split.pieces);
         if (p.a.zero_rest != 0) {   // queries of no request
             const size_t row = static_cast<size_t>(p.a.heads) * D / 8;
             int end = 0;
@@ -1027,45 +1032,66 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
     if (warp == 11) prefill::tmem_dealloc(tmem, kTmemColumns);
 }
 
-// The pieces of a unit that several CTAs share, in the order of its keys.
+// The pieces of a unit that several CTAs share, in the order of its keys.  A thread has one row and D / 64 groups of four
+// columns.  Latency bounds it, so loads of several pieces are under way at a time (509 tokens after 16,000, 8/1 heads of 256:
+// 94.7 us with one piece after the other, 85.4; 16 pieces ahead, loads of pieces that are not there among them: 8,192
+// tokens 507 us instead of 488).
 constexpr int kJoinThreads = 256;
 constexpr int kJoinRows = 16;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) prompt_join_kernel(const __grid_constant__ PromptArgs p) {
-    constexpr int kUnitRows = Config<D>::kTiles * kRows, kColumns = D / 4;
+    constexpr int kUnitRows = Config<D>::kTiles * kRows, kGroups = D / 64, kAhead = 2;
+    constexpr int kGroupColumns = kJoinThreads / kJoinRows * 4;
+    static_assert(kGroups * kGroupColumns == D, "a thread has a group of columns of every kGroupColumns");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int4 raw = __ldcg(reinterpret_cast<const int4*>(p.splits + blockIdx.x));
-    const int request = raw.x, head = raw.y, unit = raw.z, pieces = raw.w;
-    if (pieces == 0) return;
-    const int group = p.a.heads / p.a.kv_heads, unit_tokens = p.tile_tokens * Config<D>::kTiles;
-    const int first = min(max(p.a.index[request], 0), p.a.tokens);
-    const int tokens = min(max(p.a.index[request + 1], first), p.a.tokens) - first;
-    auto slot_of = [&](int i) { return (static_cast<size_t>(blockIdx.x) + i) * 2 + (i == 0 ? 1 : 0); };
-    for (int i = threadIdx.x; i < kJoinRows * kColumns; i += kJoinThreads) {
-        const int r = blockIdx.y * kJoinRows + i % kJoinRows, c = i / kJoinRows * 4;
-        const int tile = r / kRows, in_tile = r % kRows, token = in_tile / group;
-        const int mine = unit * unit_tokens + tile * p.tile_tokens + token;
-        if (token >= p.tile_tokens || mine >= tokens) continue;
-        float highest = -INFINITY;
-        for (int q = 0; q < pieces; ++q) highest = fmaxf(highest, __ldcg(p.stats + (slot_of(q) * kUnitRows + r) * 2));
-        float total = 0.f;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int q = 0; q < pieces; ++q) {
-            const float2 s = __ldcg(reinterpret_cast<const float2*>(p.stats + (slot_of(q) * kUnitRows + r) * 2));
-            if (s.x == -INFINITY) continue;   // nothing of it was written
-            const float w = prefill::exp2_approx(s.x - highest);
-            const float4 v =
-                __ldcg(reinterpret_cast<const float4*>(p.partial + slot_of(q) * kUnitRows * D + (c / 4 * kUnitRows + r) * 4));
-            total = fmaf(w, s.y, total);
-            sum.x = fmaf(w, v.x, sum.x);
-            sum.y = fmaf(w, v.y, sum.y);
-            sum.z = fmaf(w, v.z, sum.z);
-            sum.w = fmaf(w, v.w, sum.w);
+    const Split split = {raw.x, raw.y, raw.z, raw.w};
+    const int group = p.a.heads / p.a.kv_heads;
+    const int r = blockIdx.y * kJoinRows + threadIdx.x % kJoinRows, c = threadIdx.x / kJoinRows * 4;
+    const int tile = r / kRows, in_tile = r % kRows, token = in_tile / group, mine = tile * p.tile_tokens + token;
+    if (split.pieces == 0 || token >= p.tile_tokens || mine >= split.tokens) return;
+    auto row_of = [&](int i) {   // of piece i, among the rows of all pieces
+        return ((static_cast<size_t>(blockIdx.x) + i) * 2 + (i == 0 ? 1 : 0)) * kUnitRows;
+    };
+    const float2* stats = reinterpret_cast<const float2*>(p.stats) + r;
+    const float4* partial = reinterpret_cast<const float4*>(p.partial) + c / 4 * kUnitRows + r;
+    float highest = -INFINITY;
+#pragma unroll 4
+    for (int q = 0; q < split.pieces; ++q) highest = fmaxf(highest, __ldcg(stats + row_of(q)).x);
+    float total = 0.f;
+    float4 sum[kGroups];
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) sum[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int q0 = 0; q0 < split.pieces; q0 += kAhead) {
+        float2 of[kAhead];
+        float4 v[kAhead][kGroups];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (q0 + i >= split.pieces) continue;
+            const size_t at = row_of(q0 + i);
+            of[i] = __ldcg(stats + at);
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) v[i][g] = __ldcg(partial + at * (D / 4) + g * (kGroupColumns / 4) * kUnitRows);
         }
-        store_output<T>(p.a.out + (static_cast<size_t>(first + mine) * p.a.heads + head * group + in_tile % group) * D + c,
-                        sum, total);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (q0 + i >= split.pieces || of[i].x == -INFINITY) continue;   // nothing of it was written
+            const float w = prefill::exp2_approx(of[i].x - highest);
+            total = fmaf(w, of[i].y, total);
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                sum[g].x = fmaf(w, v[i][g].x, sum[g].x);
+                sum[g].y = fmaf(w, v[i][g].y, sum[g].y);
+                sum[g].z = fmaf(w, v[i][g].z, sum[g].z);
+                sum[g].w = fmaf(w, v[i][g].w, sum[g].w);
+            }
+        }
     }
+    unsigned short* out =
+        p.a.out + (static_cast<size_t>(split.first + mine) * p.a.heads + split.head * group + in_tile % group) * D + c;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) store_output<T>(out + g * kGroupColumns, sum[g], total);
 }
 
 // ---------------------------------------------------------------------------------------
