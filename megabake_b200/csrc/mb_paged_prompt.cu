@@ -30,7 +30,8 @@ constexpr int kSmemLimit = 227 * 1024;
 // tokens of 128-wide heads took 510 and 481 us (192: 492, 320: 484), seven prompts of 64-wide ones 72 and 78.
 __host__ __device__ constexpr int tile_cost(int head_dim) { return head_dim == 64 ? 128 : 256; }
 // Keys of a run at least, where units are cut.  A prompt of 1,000 tokens, 9/3 heads of 64: 128 keys 21.3 us, 256 21.8, 512
-// 24.2; 300 tokens after 2,000: 21.5, 20.5, 24.2; 64 after 3,000, 32/8 heads of 128: 29.5, 28.6, 30.0.
+// 24.2; 300 tokens after 2,000: 21.5, 20.5, 24.2; 64 after 3,000, 32/8 heads of 128: 29.5, 28.6, 30.0 (before the join
+// took less).
 constexpr int kLeastKeys = 256;
 // Rows of the table that hold no more are not cut: one launch and no scratch (19 tokens: 9.2 us, cut 15.6).  Rows of up to
 // 1,024 keys: 8 x 40 tokens after 700 uncut 27.9 us, cut 24.7; 4 x 600 36.2 and 34.0; one of 500 18.8 and 20.5.
@@ -351,8 +352,8 @@ __device__ __forceinline__ bool wait_warp(unsigned long long* bar, unsigned int 
 // memory and are rescaled only when a row's maximum has grown by more than 2^8 since the last time.  256-wide
 // heads: one query tile.
 //
-// Measured (us; floor at the measured GEMM rate): 8,192 tokens, 32/8 heads of 128: 488 in a graph of few passes (332), 1.13
-// PFLOP/s; 509 tokens after 16,000, 8/1 heads of 256: 85 (41); seven prompts of up to 1,031, 32/8 heads of 64, pages of
+// Measured (us; floor at the measured GEMM rate): 8,192 tokens, 32/8 heads of 128: 485 in a graph of few passes (332), 1.13
+// PFLOP/s; 509 tokens after 16,000, 8/1 heads of 256: 84 (41); seven prompts of up to 1,031, 32/8 heads of 64, pages of
 // 16: 59 (8).  What bounds it: a block of 64 keys takes 1,700 to 1,900 cycles, of which the exponentials of its two tiles,
 // 8 cycles a warp and instruction, are 1,024, and the products 1,280 (64 keys a product of scores read the queries from shared
 // memory for 64 columns, at two thirds of the rate that 128 columns reach); between units there are the
@@ -1033,52 +1034,64 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
 }
 
 // The pieces of a unit that several CTAs share, in the order of its keys.  A thread has one row and D / 64 groups of four
-// columns.  Latency bounds it, so loads of several pieces are under way at a time (509 tokens after 16,000, 8/1 heads of 256:
-// 94.7 us with one piece after the other, 85.4; 16 pieces ahead, loads of pieces that are not there among them: 8,192
-// tokens 507 us instead of 488).
-constexpr int kJoinThreads = 256;
-constexpr int kJoinRows = 16;
+// columns.  Latency bounds it, trips to L2 of about 800 cycles: the first two pieces are read before it is known whether a
+// unit was cut here, statistics of all pieces at once, and sums of four pieces at a time (with two 16 tokens after 9,000,
+// 18 pieces a unit, take 27.3 us instead of 25.8, with six 26.1, where 8 x 40 after 700 take 26.7, not 25.6).  One piece
+// after the other it took 509 tokens after 16,000, 8/1 heads of 256, from 84 to 95 us.
+constexpr int kJoinThreads = 128;
+constexpr int kJoinRows = 8;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) prompt_join_kernel(const __grid_constant__ PromptArgs p) {
-    constexpr int kUnitRows = Config<D>::kTiles * kRows, kGroups = D / 64, kAhead = 2;
+    extern __shared__ float2 statistics[];   // [pieces][kJoinRows]
+    constexpr int kUnitRows = Config<D>::kTiles * kRows, kGroups = D / 64, kAhead = D == 256 ? 2 : 4;
     constexpr int kGroupColumns = kJoinThreads / kJoinRows * 4;
     static_assert(kGroups * kGroupColumns == D, "a thread has a group of columns of every kGroupColumns");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int4 raw = __ldcg(reinterpret_cast<const int4*>(p.splits + blockIdx.x));
-    const Split split = {raw.x, raw.y, raw.z, raw.w};
     const int group = p.a.heads / p.a.kv_heads;
-    const int r = blockIdx.y * kJoinRows + threadIdx.x % kJoinRows, c = threadIdx.x / kJoinRows * 4;
+    const int row = threadIdx.x % kJoinRows, r = blockIdx.y * kJoinRows + row, c = threadIdx.x / kJoinRows * 4;
     const int tile = r / kRows, in_tile = r % kRows, token = in_tile / group, mine = tile * p.tile_tokens + token;
-    if (split.pieces == 0 || token >= p.tile_tokens || mine >= split.tokens) return;
-    auto row_of = [&](int i) {   // of piece i, among the rows of all pieces
+    auto rows_of = [&](int i) {   // where the rows of piece i begin, among those of all pieces
         return ((static_cast<size_t>(blockIdx.x) + i) * 2 + (i == 0 ? 1 : 0)) * kUnitRows;
     };
     const float2* stats = reinterpret_cast<const float2*>(p.stats) + r;
     const float4* partial = reinterpret_cast<const float4*>(p.partial) + c / 4 * kUnitRows + r;
+    float4 v[kAhead][kGroups];
+    auto load = [&](int i, int q) {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+            v[i][g] = __ldcg(partial + rows_of(q) * (D / 4) + g * (kGroupColumns / 4) * kUnitRows);
+    };
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 raw = __ldcg(reinterpret_cast<const int4*>(p.splits + blockIdx.x));
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (blockIdx.x + i < gridDim.x && token < p.tile_tokens) load(i, i);
+    const Split split = {raw.x, raw.y, raw.z, raw.w};
+    if (split.pieces == 0) return;
+    for (int q = threadIdx.x / kJoinRows; q < split.pieces; q += kJoinThreads / kJoinRows)
+        statistics[q * kJoinRows + row] = __ldcg(stats + rows_of(q));
+    const bool counts = token < p.tile_tokens && mine < split.tokens;
+    if (counts) {
+#pragma unroll
+        for (int i = 2; i < kAhead; ++i)
+            if (i < split.pieces) load(i, i);
+    }
+    __syncthreads();
+    if (!counts) return;
     float highest = -INFINITY;
-#pragma unroll 4
-    for (int q = 0; q < split.pieces; ++q) highest = fmaxf(highest, __ldcg(stats + row_of(q)).x);
+    for (int q = 0; q < split.pieces; ++q) highest = fmaxf(highest, statistics[q * kJoinRows + row].x);
     float total = 0.f;
     float4 sum[kGroups];
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) sum[g] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int q0 = 0; q0 < split.pieces; q0 += kAhead) {
-        float2 of[kAhead];
-        float4 v[kAhead][kGroups];
+    for (int q0 = 0;;) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            if (q0 + i >= split.pieces) continue;
-            const size_t at = row_of(q0 + i);
-            of[i] = __ldcg(stats + at);
-#pragma unroll
-            for (int g = 0; g < kGroups; ++g) v[i][g] = __ldcg(partial + at * (D / 4) + g * (kGroupColumns / 4) * kUnitRows);
-        }
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            if (q0 + i >= split.pieces || of[i].x == -INFINITY) continue;   // nothing of it was written
-            const float w = prefill::exp2_approx(of[i].x - highest);
-            total = fmaf(w, of[i].y, total);
+            if (q0 + i >= split.pieces) break;
+            const float2 of = statistics[(q0 + i) * kJoinRows + row];
+            if (of.x == -INFINITY) continue;   // nothing of it was written
+            const float w = prefill::exp2_approx(of.x - highest);
+            total = fmaf(w, of.y, total);
 #pragma unroll
             for (int g = 0; g < kGroups; ++g) {
                 sum[g].x = fmaf(w, v[i][g].x, sum[g].x);
@@ -1087,6 +1100,11 @@ __global__ void __launch_bounds__(kJoinThreads) prompt_join_kernel(const __grid_
                 sum[g].w = fmaf(w, v[i][g].w, sum[g].w);
             }
         }
+        q0 += kAhead;
+        if (q0 >= split.pieces) break;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (q0 + i < split.pieces) load(i, q0 + i);
     }
     unsigned short* out =
         p.a.out + (static_cast<size_t>(split.first + mine) * p.a.heads + split.head * group + in_tile % group) * D + c;
@@ -1145,8 +1163,8 @@ cudaError_t launch_prompt(const CUtensorMap& queries, const CUtensorMap& keys, c
     cudaError_t err = launch_early(prompt_attention_kernel<T, D>, dim3(s.ctas), kThreads, s.smem, 1, stream, queries, keys,
                                    values, args);
     if (err == cudaSuccess && s.joined)
-        err = launch_early(prompt_join_kernel<T, D>, dim3(s.ctas, Config<D>::kTiles * kRows / kJoinRows), kJoinThreads, 0,
-                           1, stream, args);
+        err = launch_early(prompt_join_kernel<T, D>, dim3(s.ctas, Config<D>::kTiles * kRows / kJoinRows), kJoinThreads,
+                           s.ctas * kJoinRows * static_cast<int>(sizeof(float2)), 1, stream, args);
     return err;
 }
 
