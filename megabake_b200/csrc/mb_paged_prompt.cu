@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cstdint>
 
 #include "mb_device.cuh"
@@ -993,9 +994,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                 }
             }
             if (!whole) {
+                // Minus infinity says that nothing was written.  A maximum passes NaN by: where all scores of the piece are NaN
+                // it is minus infinity too, and the sum says so.
                 *reinterpret_cast<float2*>(
                     p.stats + (static_cast<size_t>(blockIdx.x * 2 + (begin == 0 ? 1 : 0)) * kTiles * kRows + tile * kRows + r) * 2) =
-                    make_float2(any && l != 0.f ? m : -INFINITY, l);
+                    make_float2(any ? fmaxf(m, -FLT_MAX) : -INFINITY, l);
                 if (begin == 0) split = {u->first, u->head, u->tokens, u->pieces};
             }
             prefill::tc_fence_before();
