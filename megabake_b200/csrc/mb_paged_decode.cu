@@ -143,23 +143,35 @@ __device__ __forceinline__ void mma<__half>(float (&d)[4], const unsigned int (&
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A weight as the sum of two 16-bit numbers: what the first leaves out is at most half a step of it, and the second keeps
-// that to half a step of its own, so the product with the values sees weights of 16 (bf16) or 22 bits.  One
-// 16-bit number would put as much error into the output as rounding the output does; the second product costs
+// A weight as the sum of two 16-bit numbers, neither negative: the first is cut off, what that leaves out is less than a step
+// of it, and the second keeps that to half a step of its own, so the product with the values sees weights of 16 (bf16) or
+// 22 bits.  One 16-bit number would put as much error into the output as rounding the output does; the second product costs
 // nothing here, where the matrix units wait for HBM.
+//
+// Both parts meet the same values, and an infinity times zero, or two of opposite signs, would be NaN.  So the second is at
+// least the smallest number that counts, 2^-126 or 2^-24 beside weights of up to 2^-31 or 2^15, wherever the first is not zero.
 template <typename T>
 __device__ __forceinline__ void split_pair(float x, float y, unsigned int& high, unsigned int& low);
+__device__ __forceinline__ unsigned int at_least_where(unsigned int v, unsigned int least, unsigned int where) {
+    unsigned int r;
+    asm("{\n\t.reg .b32 t;\n\t"
+        "min.u16x2 t, %2, %3;\n\t"
+        "max.u16x2 %0, %1, t;\n\t}"
+        : "=r"(r)
+        : "r"(v), "r"(least), "r"(where));
+    return r;
+}
 template <>
 __device__ __forceinline__ void split_pair<__nv_bfloat16>(float x, float y, unsigned int& high, unsigned int& low) {
-    high = prefill::pack_bf16_pair(x, y);
-    low = prefill::pack_bf16_pair(x - lo_bf16(high), y - hi_bf16(high));
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(high) : "f"(y), "f"(x));
+    low = at_least_where(prefill::pack_bf16_pair(x - lo_bf16(high), y - hi_bf16(high)), 0x00800080u, high);
 }
 template <>
 __device__ __forceinline__ void split_pair<__half>(float x, float y, unsigned int& high, unsigned int& low) {
-    const __half2 h = __floats2half2_rn(x, y);
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(high) : "f"(y), "f"(x));
+    const __half2 h = *reinterpret_cast<const __half2*>(&high);
     const __half2 l = __floats2half2_rn(x - __low2float(h), y - __high2float(h));
-    high = *reinterpret_cast<const unsigned int*>(&h);
-    low = *reinterpret_cast<const unsigned int*>(&l);
+    low = at_least_where(*reinterpret_cast<const unsigned int*>(&l), 0x00010001u, high);
 }
 
 __device__ __forceinline__ void tma_load_page(void* dst, const CUtensorMap* map, int place, int head, int page,

@@ -5,7 +5,7 @@ import torch
 
 from megabake_b200 import paged_kv_attention, paged_prefill_attention
 from tests import paged_reference as reference
-from tests.test_gpu_paged import BF16, Cache, _check, _int32, _normal
+from tests.test_gpu_paged import BF16, FP16, Cache, _check, _int32, _normal
 
 pytestmark = [pytest.mark.gpu, pytest.mark.timeout(300)]
 
@@ -62,3 +62,35 @@ def test_prompt_pieces_without_weight(heads):
     for t in range(5):
         expected = reference.attend(query[t], *cache.pools, without[0], 4000 - 5 + t + 1, dim ** -0.5)
         _check(out[t], expected, 4000, BF16, reference.prompt_rounding(BF16))
+
+
+@pytest.mark.parametrize("heads,cached", [((4, 2, 64), 40), ((9, 3, 64), 4000), ((32, 8, 128), 300), ((24, 1, 128), 3000),
+                                          ((8, 1, 256), 2000), ((12, 1, 256), 90)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_decode_values_that_are_no_numbers(heads, cached, dtype):
+    """Infinities and NaN among the values reach all queries of their key head, in their columns, and nobody else's:
+    infinities as such, unless there are both.  (Weights here are far above what 16 bits resolve.)"""
+    count, kv_heads, dim = heads
+    cache = Cache([cached, cached], kv_heads, dim, 16, dtype, cached)
+    query = _normal((2, count, dim), cache.g, dtype)
+    inf, nan = float("inf"), float("nan")
+    odd = {0: {1: inf, 2: -inf, 3: nan, 4: inf}, cached // 2: {4: -inf, 1: inf}, cached // 2 + 1: {dim - 1: -inf},
+           cached - 1: {7: inf, dim - 2: nan}}
+    odd.update({cached // 3 + i: {10 + i: inf if i % 2 else -inf} for i in range(10)})
+    seen = {}
+    for position, columns in odd.items():
+        slot = cache.slots[0][position]
+        for column, value in columns.items():
+            cache.pools[1][slot // 16, slot % 16, kv_heads - 1, column] = value
+            seen[column] = seen.get(column, 0.0) + value
+    finite = [p.clone() for p in cache.pools]
+    finite[1].nan_to_num_(0.0, 0.0, 0.0)
+    out = paged_kv_attention(query, None, None, *cache.pools, cache.table, cache.lengths)
+    mine = torch.arange(count, device="cuda") // (count // kv_heads) == kv_heads - 1
+    for t in range(2):
+        got, expected = out[t].clone(), reference.attend(query[t], *finite, cache.table[t], cached, dim ** -0.5)
+        for column, value in seen.items() if t == 0 else ():
+            there = got[mine, column]
+            assert bool(there.isnan().all() if value != value else there.eq(value).all()), column
+            got[mine, column] = expected[0][mine, column].to(dtype)
+        _check(got, expected, cached, dtype, reference.decode_rounding(dtype))
