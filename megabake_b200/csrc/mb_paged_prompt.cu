@@ -1012,14 +1012,14 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         }
         if (tid == 0 && p.splits != nullptr)
             *reinterpret_cast<int4*>(p.splits + blockIdx.x) = make_int4(split.first, split.head, split.tokens, split.pieces);
-        if (p.a.zero_rest != 0) {   // queries of no request
+        if (p.a.zero_rest != 0) {   // queries of no request: before the first one and behind the last one
             const size_t row = static_cast<size_t>(p.a.heads) * D / 8;
-            int end = 0;
-            for (int q = 0; q < p.a.requests; ++q) end = max(end, requests[q].first + requests[q].tokens);
-            uint4* rest = reinterpret_cast<uint4*>(p.a.out) + end * row;
-            const size_t all = (p.a.tokens - end) * row;
+            const Request last = requests[p.a.requests - 1];
+            const size_t front = requests[0].first * row, back = (last.first + last.tokens) * row;
+            const size_t all = front + p.a.tokens * row - back;
+            uint4* to = reinterpret_cast<uint4*>(p.a.out);
             for (size_t i = blockIdx.x * kTiles * 128 + tid; i < all; i += gridDim.x * kTiles * 128)
-                rest[i] = make_uint4(0u, 0u, 0u, 0u);
+                to[i < front ? i : i - front + back] = make_uint4(0u, 0u, 0u, 0u);
         }
     }
     if (!ok && lane == 0) {

@@ -388,9 +388,10 @@ def paged_prefill_attention(query: torch.Tensor, key_pages: torch.Tensor, value_
     -> ``[tokens, heads, head_dim]``.
 
     Request ``r`` has the queries ``offsets[r] .. offsets[r + 1] - 1`` (int32 ``[requests + 1]``, as ``paged_reserve``
-    gives them): its last positions, whose keys and values have been appended.  The one at position ``p`` attends the
-    keys ``0 .. p`` that lie on pages of the pool: whole prompts, or a chunk after what is cached.  Queries behind
-    the last request are zero in a new output; rows of an ``out`` that is given stay as they were there.  ``scale`` and
+    gives them, or any from 0 to ``tokens`` that do not fall): its last positions, whose keys and values have been appended.
+    The one at position ``p`` attends the keys ``0 .. p`` that lie on pages of the pool: whole prompts, or a chunk after what
+    is cached.  Queries before the first request and behind the last one are zero in a new output; rows of an ``out`` that is
+    given stay as they were there.  ``scale`` and
     ``status`` as for ``paged_kv_attention``."""
     return _attention("mb_paged_prefill", query, None, None, key_pages, value_pages, block_table, lengths, offsets, scale,
                       out, status)

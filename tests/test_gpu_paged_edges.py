@@ -1,0 +1,46 @@
+"""Calls of the paged operators at the edges of what they take."""
+
+import pytest
+import torch
+
+from megabake_b200 import paged_append, paged_kv_attention, paged_prefill_attention
+from tests import paged_reference as reference
+from tests.test_gpu_paged import BF16, Cache, _check, _int32, _normal
+
+pytestmark = [pytest.mark.gpu, pytest.mark.timeout(300)]
+
+
+@pytest.mark.parametrize("heads,width", [((4, 2, 64), 8), ((4, 2, 64), 60), ((5, 1, 128), 60), ((2, 1, 256), 60)])
+@pytest.mark.parametrize("first", [1, 7, 300])
+def test_prompt_queries_before_the_first_request(heads, width, first):
+    """Queries of no request are zero in a new output on both sides of the requests, and stay in one that is given."""
+    count, kv_heads, dim = heads
+    cache = Cache([50, 33], kv_heads, dim, 16, BF16, first)
+    cache.table = torch.nn.functional.pad(cache.table, (0, width - cache.table.shape[1]), value=-1).contiguous()
+    tokens = first + 30 + 21 + 4
+    query = _normal((tokens, count, dim), cache.g, BF16)
+    offsets = _int32([first, first + 30, first + 51])
+    junk = torch.full_like(query, float("nan"))   # what the allocator hands out next
+    del junk
+    new = paged_prefill_attention(query, *cache.pools, cache.table, cache.lengths, offsets)
+    given = paged_prefill_attention(query, *cache.pools, cache.table, cache.lengths, offsets, out=torch.full_like(query, 5.0))
+    assert new[:first].eq(0).all() and new[first + 51:].eq(0).all()
+    assert given[:first].eq(5).all() and given[first + 51:].eq(5).all()
+    assert torch.equal(new[first:first + 51], given[first:first + 51])
+    for r, at, n, length in ((0, first, 30, 50), (1, first + 30, 21, 33)):
+        for j in (0, n // 2, n - 1):
+            keys = length - n + j + 1
+            expected = reference.attend(query[at + j], *cache.pools, cache.table[r], keys, dim ** -0.5)
+            _check(new[at + j], expected, keys, BF16, reference.prompt_rounding(BF16))
+
+
+def test_prompt_requests_that_end_before_the_last_row():
+    """Requests without queries at the end of the table; all queries belong to none."""
+    cache = Cache([50, 33, 20], 2, 64, 16, BF16, 0)
+    query = _normal((40, 4, 64), cache.g, BF16)
+    out = paged_prefill_attention(query, *cache.pools, cache.table, cache.lengths, _int32([5, 9, 9, 9]))
+    assert out[:5].eq(0).all() and out[9:].eq(0).all() and not out[5:9].eq(0).all(-1).any()
+    out = paged_prefill_attention(query, *cache.pools, cache.table, cache.lengths, _int32([40, 40, 40, 40]))
+    assert out.eq(0).all()
+    out = paged_prefill_attention(query, *cache.pools, cache.table, cache.lengths, _int32([0, 0, 0, 0]))
+    assert out.eq(0).all()
