@@ -302,13 +302,13 @@ template <typename T>
 __device__ __forceinline__ unsigned int without_odd(unsigned int v) {
     return (not_finite<T>(v & 0xffffu) ? 0u : v & 0xffffu) | (not_finite<T>(v & 0xffff0000u) ? 0u : v & 0xffff0000u);
 }
-// The infinities and NaN that were taken out of blocks `from` .. `end` - 1 of a unit, 32 columns of them from `column` on,
+// The infinities and NaN that were taken out of blocks `from` .. `stop` - 1 of a unit, 32 columns of them from `column` on,
 // added to the outputs of a query at `position`.  `info` is that of block `end`.
 template <typename T, int kBlock>
 __device__ __noinline__ void give_back(float* o, const AttentionArgs& a, const PromptControl* ctl, const Work* u, int info,
-                                       int from, int end, int column, int position) {
+                                       int from, int stop, int end, int column, int position) {
 #pragma unroll 1
-    for (int b = from; b < end; ++b) {
+    for (int b = from; b < stop; ++b) {
         const int block_info = (info + 2 * kInfos - (end - b)) % kInfos;
         if (ctl->odd[block_info] == 0) continue;
 #pragma unroll 1
@@ -931,8 +931,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             const bool whole = begin == 0 && end == u->blocks;
             const int unit_tokens = u->tokens;
             const int diagonal = max(begin, max(u->position, 0) / kBlock);   // the first block that a query may not see whole
+            // Only of blocks whose products with values have been waited for: what is behind them is still being written.
+            const int waited = alone ? end : blocks;
             bool any_odd = false;
-            for (int b = diagonal; b < end; ++b) any_odd |= ctl->odd[(info + 2 * kInfos - (end - b)) % kInfos] != 0;
+            for (int b = diagonal; b < waited; ++b) any_odd |= ctl->odd[(info + 2 * kInfos - (end - b)) % kInfos] != 0;
+            any_odd = __any_sync(0xffffffffu, any_odd);
             const float inverse = l == 0.f ? 0.f : 1.f / l;
             if (whole) keep *= inverse, other *= inverse;
             if (ok && any) {
@@ -962,7 +965,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                         float given[32];
 #pragma unroll
                         for (int i = 0; i < 32; ++i) given[i] = o[i];
-                        if (l != 0.f) give_back<T, kBlock>(given, p.a, ctl, u, info, diagonal, end, c, position);
+                        if (l != 0.f) give_back<T, kBlock>(given, p.a, ctl, u, info, diagonal, waited, end, c, position);
+                        __syncwarp();   // lanes come back at different times, and what follows is for all of them
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] = given[i];
                     }
