@@ -129,11 +129,12 @@ def _native_device(device: torch.device) -> int:
     return device.index
 
 
-def _whole(name: str, tensor: torch.Tensor, dtype: torch.dtype, numel: int, device: torch.device) -> None:
-    """A contiguous tensor of whole numbers."""
-    if tensor.dtype != dtype or tensor.device != device or tensor.numel() != numel or not tensor.is_contiguous():
-        fail("input-binding", f"{name} must be a contiguous {dtype} tensor of {numel} on {device}, got "
-                              f"{tensor.dtype} {tuple(tensor.shape)} on {tensor.device}")
+def _whole(name: str, tensor: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
+    """A contiguous tensor of whole numbers; the shape of a single one does not matter."""
+    if tensor.dtype != dtype or tensor.device != device or not tensor.is_contiguous() or \
+            tensor.shape != shape and not (shape == (1,) and tensor.numel() == 1):
+        fail("input-binding", f"{name} must be a contiguous {dtype} tensor {list(shape)} on {device}, got "
+                              f"{tensor.dtype} {list(tensor.shape)} on {tensor.device}")
 
 
 def _rows(name: str, tensor: torch.Tensor, shape: tuple, like: torch.Tensor) -> tuple:
@@ -223,16 +224,16 @@ def _reserve_fields(counts, lengths, block_table, free_pages, free_count, page_s
         fail("input-binding", f"block_table must be [requests, width], got {tuple(block_table.shape)}")
     device = counts.device
     requests, width = block_table.shape
+    for name, tensor, shape in (("counts", counts, (requests,)), ("lengths", lengths, (requests,)),
+                                ("block_table", block_table, (requests, width)),
+                                ("free_pages", free_pages, (free_pages.numel(),)), ("free_count", free_count, (1,))):
+        _whole(name, tensor, torch.int32, shape, device)
     if device.type != "cuda" or not 1 <= requests <= _MAX_REQUESTS or width < 1 or not _page_size_covered(page_size) or \
             max_tokens < 0 or max_tokens > _MAX_TOKENS or width * page_size > _MAX_TOKENS or \
             not 1 <= free_pages.numel() <= _MAX_COUNT:
         fail("input-binding", f"paged_reserve needs 1..{_MAX_REQUESTS} requests on a CUDA device, pages of 8 to 1024 tokens "
                               "(a power of two), rows of at most 2**30 tokens and max_tokens up to that, got "
                               f"{tuple(block_table.shape)} pages of {page_size} on {device}, max_tokens {max_tokens}")
-    for name, tensor, numel in (("counts", counts, requests), ("lengths", lengths, requests),
-                                ("block_table", block_table, requests * width),
-                                ("free_pages", free_pages, free_pages.numel()), ("free_count", free_count, 1)):
-        _whole(name, tensor, torch.int32, numel, device)
     args = rt.PagedReserveArgs(requests, width, free_pages.numel(), page_size, max_tokens)
     return bytes(args)[:rt.PagedReserveArgs.counts.offset], _native_device(device)
 
@@ -270,7 +271,7 @@ def _append_fields(key, value, key_pages, value_pages, slots) -> tuple:
     tokens = key.shape[0]
     k = _rows("key", key, (tokens, kv_heads, head_dim), key_pages)
     v = _rows("value", value, (tokens, kv_heads, head_dim), key_pages)
-    _whole("slots", slots, torch.int64, tokens, key.device)
+    _whole("slots", slots, torch.int64, (tokens,), key.device)
     args = rt.PagedAppendArgs(tokens, kv_heads, head_dim, pages, page_size, 0, *k, *v, *kpool, *vpool)
     return bytes(args)[:rt.PagedAppendArgs.key.offset], _native_device(key.device)
 
@@ -334,15 +335,15 @@ def _attention_fields(what, query, key, value, key_pages, value_pages, block_tab
             fail("input-binding", "key and value come together")
         k = _rows("key", key, (tokens, kv_heads, head_dim), key_pages)
         v = _rows("value", value, (tokens, kv_heads, head_dim), key_pages)
-    _whole("block_table", block_table, torch.int32, requests * width, device)
-    _whole("lengths", lengths, torch.int32, requests, device)
+    _whole("block_table", block_table, torch.int32, (requests, width), device)
+    _whole("lengths", lengths, torch.int32, (requests,), device)
     if index is not None:
-        _whole(index_name, index, torch.int32, requests + 1 if prefill else tokens, device)
+        _whole(index_name, index, torch.int32, (requests + 1 if prefill else tokens,), device)
     if out is not None and (out.dtype != query.dtype or out.shape != query.shape or out.device != device or
                             not out.is_contiguous()):
         fail("input-binding", f"out must be a contiguous {query.dtype} {tuple(query.shape)} tensor on {device}")
     if status is not None:
-        _whole("status", status, torch.int32, 1, device)
+        _whole("status", status, torch.int32, (1,), device)
     device_index = _native_device(device)
     args = rt.PagedAttentionArgs(_ELEMENTS[query.dtype], tokens, requests, heads, kv_heads, head_dim, width, pages, page_size,
                                  out is None, head_dim ** -0.5 if scale is None else scale, 0, *q, *k, *v, *kpool, *vpool)
