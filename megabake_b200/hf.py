@@ -346,8 +346,55 @@ class StatefulPrefill(StatefulDecoder):
         return super().forward(input_ids, positions, *state)
 
 
+# What PagedDecoder's loop goes through, by the names that Hugging Face gives it ...
+_COMPUTED_MODULES = (
+    ("model", {"embed_tokens", "layers", "norm", "rotary_emb"}),
+    ("layer", {"self_attn", "mlp", "input_layernorm", "post_attention_layernorm"}),
+    ("attention", {"q_proj", "k_proj", "v_proj", "o_proj"}),
+)
+# ... and settings that models of these modules apply outside of them, with the value that leaves the loop right.
+_NEUTRAL_SETTINGS = {
+    "attn_logit_softcapping": None, "final_logit_softcapping": None, "clip_qkv": None,
+    "embedding_multiplier": 1.0, "residual_multiplier": 1.0, "logits_scaling": 1.0, "logit_scale": 1.0,
+    "lm_head_multiplier": 1.0, "scale_emb": 1.0, "use_parallel_residual": False, "parallel_attn": False,
+}
+
+
+def _refuse_what_is_not_computed(model: torch.nn.Module, config) -> None:
+    """A model is computed by its parts, so one with other parts, or other uses of them, would come out wrong."""
+    for layer in model.layers:
+        attention = getattr(layer, "self_attn", None)
+        for (kind, computed), module in zip(_COMPUTED_MODULES, (model, layer, attention)):
+            name = type(module).__name__
+            missing = computed - set(getattr(module, "_modules", ())) - {"rotary_emb"}
+            if missing:
+                raise NotImplementedError(f"a paged decoder needs {sorted(missing)} in the {kind}, {name} has none")
+            other = (set(module._modules) | set(module._parameters)) - computed
+            if other:
+                raise NotImplementedError(f"a paged decoder does not compute {sorted(other)} of {name}")
+        name = type(attention).__name__
+        if not hasattr(attention, "scaling") or not hasattr(sys.modules[type(attention).__module__], "apply_rotary_pos_emb"):
+            raise NotImplementedError(f"a paged decoder needs a scaling and apply_rotary_pos_emb, {name} has none")
+        if not getattr(attention, "use_rope", True):
+            raise NotImplementedError(f"a paged decoder rotates in every layer, {name} does not")
+    for name, neutral in _NEUTRAL_SETTINGS.items():
+        value = getattr(config, name, neutral)
+        if value is not None and value != neutral:
+            raise NotImplementedError(f"a paged decoder does not compute {name} = {value}")
+    rope = getattr(config, "rope_parameters", None) or {}
+    if rope.get("llama_4_scaling_beta") is not None:
+        raise NotImplementedError("a paged decoder does not compute scores that are scaled by position")
+    # their frequencies follow the furthest position of a call, which may be another request's
+    if rope.get("rope_type") in ("dynamic", "longrope"):
+        raise NotImplementedError(f"a paged decoder does not compute {rope['rope_type']} rotary positions")
+
+
 class PagedDecoder(StatefulDecoder):
     """The loop of ``StatefulDecoder`` over a paged cache: ``forward(input_ids[tokens], batch, state) -> logits``.
+
+    For pre-norm models of an embedding, layers of two norms, attention with rotary positions and an MLP, and a last norm;
+    one that has more to it (norms of queries and keys, soft caps, multipliers, a sliding window shorter than the state's
+    capacity) is refused.
 
     ``batch`` is what ``state.reserve`` returned for these tokens: packed, one request after the other, each at its own
     length.  With ``one_token`` every request has one at most (a decode step): its key and value are appended on the
@@ -356,11 +403,25 @@ class PagedDecoder(StatefulDecoder):
     model's own modules, attention and the cache are the native operators; places behind the last token are computed like
     the others and mean nothing, so that a step of fixed size can be captured in a CUDA graph."""
 
+    def __init__(self, model: torch.nn.Module):
+        super().__init__(model)
+        _refuse_what_is_not_computed(self.model, self.config)
+        # where layers have kinds, none has a window
+        config = self.config
+        windowed = not getattr(config, "layer_types", None) and getattr(config, "use_sliding_window", True)
+        self.window = getattr(config, "sliding_window", None) if windowed else None
+
+    def _check_window(self, state: PagedState) -> None:
+        if self.window is not None and state.capacity > self.window:
+            raise NotImplementedError(f"cache capacity {state.capacity} exceeds the {self.window}-token sliding window")
+
     def make_paged_state(self, requests: int, capacity: int, **options) -> PagedState:
         """A ``PagedState`` of this model's layers and heads."""
         weight = self.model.embed_tokens.weight
         options = {"dtype": weight.dtype, "device": weight.device, **options}
-        return PagedState(self.layer_count, requests, capacity, self.kv_heads, self.head_dim, **options)
+        state = PagedState(self.layer_count, requests, capacity, self.kv_heads, self.head_dim, **options)
+        self._check_window(state)
+        return state
 
     @torch.no_grad()
     def forward(self, input_ids: torch.Tensor, batch: PagedBatch, state: PagedState, *, one_token: bool = False,
@@ -369,6 +430,7 @@ class PagedDecoder(StatefulDecoder):
             raise ValueError(f"{tuple(input_ids.shape)} ids for {batch.positions.numel()} places")
         if len(state.key_pages) != self.layer_count:
             raise ValueError(f"a state of {len(state.key_pages)} layers for {self.layer_count}")
+        self._check_window(state)
         hidden = self.model.embed_tokens(input_ids[None])
         rotary = self.model.rotary_emb(hidden, batch.positions[None])
         dim, count = self.head_dim, input_ids.shape[0]
