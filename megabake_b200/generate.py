@@ -145,7 +145,7 @@ class PagedGenerator:
     ``requests`` rows run at once; ``pages`` pages of ``page_size`` tokens are shared by them (default: enough for all
     of them to grow to ``capacity``).  A prompt is admitted when its row and the pages for all of its tokens are there, so
     no request is refused later.  Decode steps are one CUDA graph: pages, attention, projections and the greedy
-    pick, without the host; ids are read once at the end."""
+    pick, without the host; at the end it is checked once that no wait inside a kernel ran out (``CompilerError``)."""
 
     def __init__(self, model: torch.nn.Module, requests: int, capacity: int, *, page_size: int = 64,
                  pages: int | None = None):
@@ -257,4 +257,5 @@ class PagedGenerator:
                     free_pages += self._pages_of(prompts[index].numel() + count - 1)
                     self._produced[row] = 0
                 self.state.reserve(counts.to(self.device), 0)
+        self.state.check()
         return [done[index] for index in range(len(prompts))]

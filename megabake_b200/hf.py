@@ -401,7 +401,8 @@ class PagedDecoder(StatefulDecoder):
     way; otherwise requests may have any number (prompts, chunks of them, decoding requests among them).
     ``tokens`` (int64) selects the places whose logits are wanted.  Not compiled: projections, norms and the MLP are the
     model's own modules, attention and the cache are the native operators; places behind the last token are computed like
-    the others and mean nothing, so that a step of fixed size can be captured in a CUDA graph."""
+    the others and mean nothing, so that a step of fixed size can be captured in a CUDA graph.  Nothing is synchronised:
+    ``state.check()``, before results are used, says whether a wait inside a kernel ran out."""
 
     def __init__(self, model: torch.nn.Module):
         super().__init__(model)
@@ -444,11 +445,11 @@ class PagedDecoder(StatefulDecoder):
             pools = (state.key_pages[index], state.value_pages[index])
             if one_token:
                 mixed = paged_kv_attention(query[0], key[0], value, *pools, state.block_table, state.lengths,
-                                           batch.rows, scale=module.scaling)
+                                           batch.rows, scale=module.scaling, status=state.status)
             else:
                 paged_append(key[0], value, *pools, batch.slots)
                 mixed = paged_prefill_attention(query[0], *pools, state.block_table, state.lengths, batch.offsets,
-                                                scale=module.scaling)
+                                                scale=module.scaling, status=state.status)
             hidden = hidden + module.o_proj(mixed.view(1, count, -1))
             hidden = hidden + layer.mlp(layer.post_attention_layernorm(hidden))
         hidden = self.model.norm(hidden)[0]

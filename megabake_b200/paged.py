@@ -54,7 +54,8 @@ class PagedBatch(NamedTuple):
 
 
 class PagedState:
-    """The tensors of a paged cache: pools per layer, one block table, lengths and the stack of free pages.
+    """The tensors of a paged cache: pools per layer, one block table, lengths, the stack of free pages, and a status word for
+    the attention operators (``status=state.status``, read by ``check``).
 
     ``pages`` defaults to enough for every request to grow to ``capacity`` tokens; fewer pages share the memory
     between requests that do not all grow that long."""
@@ -80,15 +81,26 @@ class PagedState:
         self.lengths = torch.empty(requests, dtype=torch.int32, device=device)
         self.free_pages = torch.empty(pages, dtype=torch.int32, device=device)
         self.free_count = torch.empty(1, dtype=torch.int32, device=device)
+        self.status = torch.empty(1, dtype=torch.int32, device=device)
         self.reset()
 
     def reset(self) -> None:
-        """Every request empty, every page free; page 0 is handed out first."""
+        """Every request empty, every page free; page 0 is handed out first.  No fault is on record."""
         pages = self.free_pages.numel()
         self.block_table.fill_(-1)
         self.lengths.zero_()
         self.free_pages.copy_(torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=self.free_pages.device))
         self.free_count.fill_(pages)
+        self.status.zero_()
+
+    def check(self) -> None:
+        """Synchronise the device and raise ``CompilerError`` if a kernel that was given ``status`` recorded a fault (a wait
+        that ran out): outputs since the last check are not valid, nor is what was appended of them."""
+        code = int(self.status)
+        if code:
+            self.status.zero_()
+            fail("runtime", f"device status {rt.STATUS_NAMES.get(code, code)}: "
+                            f"{rt.load_library().mb_status_string(code).decode()}")
 
     def reserve(self, counts: torch.Tensor, max_tokens: int) -> PagedBatch:
         """``paged_reserve`` on these tensors."""

@@ -6,6 +6,7 @@ import torch
 
 import megabake_b200.hf as hf
 from megabake_b200 import PagedBatch, PagedDecoder, paged
+from megabake_b200.diagnostics import CompilerError
 from tests import paged_reference as reference
 
 transformers = pytest.importorskip("transformers")
@@ -100,3 +101,34 @@ def test_a_window_shorter_than_the_capacity_is_refused(plain_operators, kind):
     ids = torch.zeros(1, dtype=torch.int64)
     with pytest.raises(NotImplementedError, match="30-token"):
         decoder(ids, PagedBatch(None, ids, ids, None, None), state)
+
+
+@pytest.mark.parametrize("one_token", [False, True])
+def test_the_state_has_the_status_word_of_every_layer(plain_operators, monkeypatch, one_token):
+    given = []
+
+    def attend(query, *_, status, **__):
+        given.append(status)
+        return torch.zeros_like(query)
+
+    monkeypatch.setattr(hf, "paged_kv_attention", attend)
+    monkeypatch.setattr(hf, "paged_prefill_attention", attend)
+    decoder = PagedDecoder(_model("llama")).eval()
+    state = decoder.make_paged_state(1, 32, page_size=PAGE, device="cpu")
+    place = torch.zeros(1, dtype=torch.int64)
+    batch = PagedBatch(torch.tensor([0, 1], dtype=torch.int32), place, place, place.int(), place.int())
+    decoder(place, batch, state, one_token=one_token)
+    assert len(given) == 2 and all(status is state.status for status in given)
+
+
+def test_a_recorded_fault_is_raised_once():
+    state = paged.PagedState(1, 1, 32, 2, 64, page_size=PAGE, device="cpu")
+    state.check()
+    state.status.fill_(2)   # what a kernel writes when a wait ran out
+    with pytest.raises(CompilerError, match="status pipeline-timeout") as info:
+        state.check()
+    assert info.value.diagnostic.stage == "runtime"
+    state.check()
+    state.status.fill_(2)
+    state.reset()
+    state.check()
