@@ -799,6 +799,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             const int own = alone ? 0 : tile;                    // query tile
             const int first_block = alone ? begin + tile : begin, blocks = tile == 0 ? u->stop0 : end;
             const int first_position = u->position + own * p.tile_tokens, position = first_position + token;
+            // Rows of no query hold whatever lies in shared memory, or the next request's queries: no say in what others do.
+            const bool counts = token < min(u->tokens - own * p.tile_tokens, p.tile_tokens);
             float m = -INFINITY, l = 0.f;
             // turns are taken for as many steps as both tiles have
             unsigned int step = 0, turns = 0;
@@ -841,7 +843,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                 const float now = fmaxf(fmaxf(highest[0], highest[1]), fmaxf(highest[2], highest[3])) * multiplier;
                 if (b == first_block) {
                     m = now;
-                } else if (__any_sync(0xffffffffu, now > m + kLag || (m == -INFINITY && now > m))) {
+                } else if (__any_sync(0xffffffffu, counts && (now > m + kLag || (m == -INFINITY && now > m)))) {
                     const float grown = fmaxf(m, now);
                     const float base = grown == -INFINITY ? 0.f : grown;
                     const float factor = prefill::exp2_approx(m - base);

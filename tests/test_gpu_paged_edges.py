@@ -5,7 +5,7 @@ import torch
 
 from megabake_b200 import paged_append, paged_kv_attention, paged_prefill_attention
 from tests import paged_reference as reference
-from tests.test_gpu_paged import BF16, Cache, _check, _int32, _normal
+from tests.test_gpu_paged import BF16, FP16, Cache, _check, _int32, _normal
 
 pytestmark = [pytest.mark.gpu, pytest.mark.timeout(300)]
 
@@ -44,3 +44,26 @@ def test_prompt_requests_that_end_before_the_last_row():
     assert out.eq(0).all()
     out = paged_prefill_attention(query, *cache.pools, cache.table, cache.lengths, _int32([0, 0, 0, 0]))
     assert out.eq(0).all()
+
+
+@pytest.mark.parametrize("heads", [(34, 2, 128), (9, 3, 64), (5, 1, 128), (24, 1, 64), (7, 1, 256)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_prompt_bits_do_not_depend_on_rows_of_no_query(heads, dtype):
+    """128 rows of a tile are not a multiple of these groups, and requests end inside of tiles: what lies in the rows that are
+    left over, from an earlier launch or of the next request, changes nothing."""
+    count, kv_heads, dim = heads
+    cache = Cache([5000, 700], kv_heads, dim, 16, dtype, count)
+    query = _normal((59, count, dim), cache.g, dtype)
+    offsets = _int32([0, 39, 59])
+    full = _normal((600, 128 * kv_heads, dim), cache.g, dtype)     # fills every row of a tile
+    results = []
+    for factor in (0.0, 1.0, 30.0, -30.0, 1000.0):
+        paged_prefill_attention(full * factor, *cache.pools, cache.table, cache.lengths, _int32([0, 600, 600]))
+        results.append(paged_prefill_attention(query, *cache.pools, cache.table, cache.lengths, offsets))
+        other = query.clone()
+        other[39:] *= factor
+        results.append(paged_prefill_attention(other, *cache.pools, cache.table, cache.lengths, offsets))
+    for result in results[1:]:
+        assert torch.equal(result[:39], results[0][:39])
+    for result in results[2::2]:
+        assert torch.equal(result, results[0])
