@@ -519,7 +519,7 @@ typedef struct mb_paged_attention_args {
     int32_t width, pages, page_size;   /* width * page_size <= 2^30                       */
     int32_t zero_rest;        /* mb_paged_prefill                                         */
     float scale;
-    int32_t reserved;
+    int32_t wait_limit_ns;    /* bound of every wait inside a kernel; 0: 2 s              */
     int64_t query_token, query_head, key_token, key_head, value_token, value_head;
     int64_t kpool_page, kpool_token, kpool_head, vpool_page, vpool_token, vpool_head;
     uint64_t query;           /* [tokens, heads, head_dim]                                */

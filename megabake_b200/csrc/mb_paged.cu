@@ -298,7 +298,7 @@ int attention_args(const mb_paged_attention_args* a, bool prefill, AttentionArgs
     if (a->tokens < 1 || a->requests < 1 || a->kv_heads < 1 || a->heads < 1 || a->heads % a->kv_heads != 0 ||
         a->width < 1 || a->pages < 1 || a->query == 0 || a->key_pages == 0 || a->value_pages == 0 || a->block_table == 0 ||
         a->lengths == 0 || a->out == 0 || (a->key == 0) != (a->value == 0) ||
-        (prefill && (a->index == 0 || a->key != 0)))
+        (prefill && (a->index == 0 || a->key != 0)) || a->wait_limit_ns < 0)
         return MB_ERR_INVALID;
     if ((a->element != MB_BF16 && a->element != MB_FP16) || !page_size_covered(a->page_size) ||
         (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) ||
@@ -337,6 +337,7 @@ int attention_args(const mb_paged_attention_args* a, bool prefill, AttentionArgs
     p.index = reinterpret_cast<const int*>(a->index);
     p.out = reinterpret_cast<unsigned short*>(a->out);
     p.status = reinterpret_cast<int*>(a->status);
+    p.wait_limit_ns = a->wait_limit_ns != 0 ? a->wait_limit_ns : static_cast<int>(kPipeTimeoutNs);
     return prefill ? prompt_admitted(p) : decode_admitted(p);
 }
 

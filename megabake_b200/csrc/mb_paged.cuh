@@ -8,6 +8,8 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "mb_device.cuh"
+
 namespace mb {
 namespace paged {
 
@@ -32,7 +34,30 @@ struct AttentionArgs {
     const int *table, *lengths, *index;
     unsigned short* out;
     int* status;
+    int wait_limit_ns;
 };
+
+// Whether a phase is there, without waiting for it: try_wait suspends the thread for some time.
+__device__ __forceinline__ bool mbar_test_wait(unsigned long long* bar, unsigned int parity) {
+    unsigned int done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+// The wait for a phase that was not there: it ends after the limit, or when another one of the CTA did.  A limit of less than
+// a millisecond is looked at all the time, without suspending.
+__device__ __forceinline__ bool wait_within(unsigned long long* bar, unsigned int parity, volatile int* abort_flag, int limit_ns) {
+    if (limit_ns >= 1000000) return mbar_wait_bounded(bar, parity, abort_flag, limit_ns);
+    const unsigned long long start = global_timer_ns();
+    while (!mbar_test_wait(bar, parity))
+        if (*abort_flag || global_timer_ns() - start > static_cast<unsigned long long>(limit_ns)) return false;
+    return true;
+}
 
 // Weights are 2^(log2(e) (score - highest) + shift).  fp16: up by 2^15, so that small ones keep their digits when they
 // are rounded to 16 bits; bf16: down by 2^31, so that no sum over a context, which has at most 2^30 keys,

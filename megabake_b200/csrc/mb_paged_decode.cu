@@ -287,6 +287,10 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
         run_end = unit_boundary(deal, run_end);
     }
 
+    auto wait_warp = [&](unsigned long long* bar, unsigned int parity) {   // all lanes come to the same result
+        return __all_sync(0xffffffffu, mbar_test_wait(bar, parity) ||
+                                           wait_within(bar, parity, &ctl->abort_flag, p.a.wait_limit_ns)) != 0;
+    };
     if (warp == kWarps) {
         // ---- copies
         int stage = 0;
@@ -316,7 +320,7 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
                 const int mine = next;
                 next = entry_of(b + batch);
                 for (int j = 0; j < batch && b < piece.end; ++j, ++b) {
-                    if (round > 0 && !prefill::mbar_wait_warp(&ctl->empty[stage], (round - 1) & 1, &ctl->abort_flag)) {
+                    if (round > 0 && !wait_warp(&ctl->empty[stage], (round - 1) & 1)) {
                         ok = false;
                         break;
                     }
@@ -426,7 +430,7 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
                     }
                     continue;
                 }
-                ok = ok && prefill::mbar_wait_warp(&ctl->full[stage], round & 1, &ctl->abort_flag);
+                ok = ok && wait_warp(&ctl->full[stage], round & 1);
                 if (!ok) continue;   // the barriers below are for all warps
                 unsigned char* keys = ring + static_cast<size_t>(stage) * 2 * kTile;
                 unsigned char* values = keys + kTile;

@@ -90,6 +90,11 @@ constexpr int kQueue = 4;
 constexpr int kMasked = 1, kDiagonal = 2;
 constexpr int kStaging = 32 * 64;    // of a softmax warp's outputs
 
+struct Waits {
+    int abort_flag;              // one of the CTA's ran out
+    int limit_ns;
+};
+
 struct PromptControl {
     Work work[kQueue];
     unsigned long long work_full[kQueue], work_empty[kQueue];
@@ -103,7 +108,7 @@ struct PromptControl {
     int odd[kInfos];             // values that are no numbers were taken out of it
     long long warp_sums[kThreads / 32];
     unsigned int tmem;
-    int abort_flag;
+    Waits waits;
 };
 
 struct Request {
@@ -333,15 +338,15 @@ __device__ __noinline__ void give_back(float* o, const AttentionArgs& a, const P
 
 // Bounded waits.  What a wait that does not succeed at once does is one function for all of them: inlined into every one
 // it is a good part of the code that has to stay in the instruction cache.
-__device__ __noinline__ bool wait_on(unsigned long long* bar, unsigned int parity, volatile int* abort_flag) {
-    return mbar_wait_bounded(bar, parity, abort_flag);
+__device__ __noinline__ bool wait_on(unsigned long long* bar, unsigned int parity, volatile Waits* waits) {
+    return wait_within(bar, parity, &waits->abort_flag, waits->limit_ns);
 }
-__device__ __forceinline__ bool wait_thread(unsigned long long* bar, unsigned int parity, volatile int* abort_flag) {
-    return mbar_try_wait(bar, parity) || wait_on(bar, parity, abort_flag);
+__device__ __forceinline__ bool wait_thread(unsigned long long* bar, unsigned int parity, volatile Waits* waits) {
+    return mbar_try_wait(bar, parity) || wait_on(bar, parity, waits);
 }
 // Of a whole warp.
-__device__ __forceinline__ bool wait_warp(unsigned long long* bar, unsigned int parity, volatile int* abort_flag) {
-    return __all_sync(0xffffffffu, wait_thread(bar, parity, abort_flag)) != 0;
+__device__ __forceinline__ bool wait_warp(unsigned long long* bar, unsigned int parity, volatile Waits* waits) {
+    return __all_sync(0xffffffffu, wait_thread(bar, parity, waits)) != 0;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -401,7 +406,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         for (int w = 0; w < 8; ++w) mbar_init(&ctl->turn[w >> 2][w & 3], 1);
         mbar_init(&ctl->half_ready, 4);
         mbar_init(&ctl->half_taken, 4);
-        ctl->abort_flag = 0;
+        ctl->waits.abort_flag = 0;
+        ctl->waits.limit_ns = p.a.wait_limit_ns;
         mbar_init_fence();
     }
     if (warp == 11) prefill::tmem_alloc(&ctl->tmem, kTmemColumns);
@@ -455,14 +461,14 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         run_begin = unit_boundary(deal, run_begin);
         run_end = unit_boundary(deal, run_end);
     }
-    volatile int* abort_flag = &ctl->abort_flag;
+    volatile Waits* waits = &ctl->waits;
     bool ok = true;
 
     // The next piece, for a warp that all comes to; it keeps what it needs of it, or lets go of it later.
     int queue = 0;
     unsigned int queue_round = 0;
     auto next_work = [&]() -> const Work* {
-        ok = ok && wait_warp(&ctl->work_full[queue], queue_round & 1, abort_flag);
+        ok = ok && wait_warp(&ctl->work_full[queue], queue_round & 1, waits);
         return ok && ctl->work[queue].end >= 0 ? &ctl->work[queue] : nullptr;
     };
     auto release_work = [&]() {
@@ -486,7 +492,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         // a piece ahead of the copies, so that nobody waits for the arithmetic
         auto publish = [&]() {
             if (queue_round > 0)
-                ok = wait_warp(&ctl->work_empty[queue], (queue_round - 1) & 1, abort_flag);
+                ok = wait_warp(&ctl->work_empty[queue], (queue_round - 1) & 1, waits);
             if (!ok) return;
             Work w = {};
             w.end = -1;
@@ -528,7 +534,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             publish();
             if (!ok) break;
             if (u.begin >= u.end) continue;
-            if (units > 0) ok = wait_warp(&ctl->q_empty, (units - 1) & 1, abort_flag);
+            if (units > 0) ok = wait_warp(&ctl->q_empty, (units - 1) & 1, waits);
             if (!ok) break;
             ++units;
             const int tiles = kTiles == 2 && !u.alone ? 2 : 1;
@@ -561,7 +567,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     const int boxes = __popc(valid & ((2u << (per_block - 1)) - 1));
 #pragma unroll 1
                     for (int kind = 0; kind < 2; ++kind) {   // keys, then values
-                        if (round > 0) ok = wait_warp(&ctl->empty[stage], (round - 1) & 1, abort_flag);
+                        if (round > 0) ok = wait_warp(&ctl->empty[stage], (round - 1) & 1, waits);
                         if (!ok) break;
                         if (kind == 0 && lane < kBlock / 32) {
                             // which keys of the block count: on a page, and seen by any query of the unit
@@ -640,7 +646,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             unsigned int p_phase = 0;                // bit: slot
             unsigned int clean_phase = 0;            // bit: stage of the ring
             while (ok) {
-                ok = wait_thread(&ctl->work_full[queue], queue_round & 1, abort_flag);
+                ok = wait_thread(&ctl->work_full[queue], queue_round & 1, waits);
                 if (!ok) break;
                 const int begin = ctl->work[queue].begin, end = ctl->work[queue].end;
                 if (end < 0) break;
@@ -652,7 +658,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     ++queue_round;
                 }
                 if (begin >= end) continue;
-                ok = wait_thread(&ctl->q_full, units & 1, abort_flag);
+                ok = wait_thread(&ctl->q_full, units & 1, waits);
                 ++units;
                 auto takes = [&](int b) { return alone ? ((b - begin) & 1) == tile : b < tile_stop; };
                 const unsigned int q = low + ((queries_at + (alone ? 0 : tile * C::kQueryBytes)) >> 4);
@@ -662,7 +668,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     if (bs < end && scored - done < 2) {
                         // scores go where the weights of two steps ago were; not waited for while there is something to do
                         const bool idle = bs == bv;
-                        if (idle ? ok = wait_thread(&ctl->full[key_stage], key_round & 1, abort_flag)
+                        if (idle ? ok = wait_thread(&ctl->full[key_stage], key_round & 1, waits)
                                  : mbar_try_wait(&ctl->full[key_stage], key_round & 1)) {
                             if (takes(bs)) {
                                 const int slot = scored & 1;
@@ -687,16 +693,16 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                         }
                         if (!ok) break;
                     }
-                    ok = wait_thread(&ctl->full[value_stage], value_round & 1, abort_flag);
+                    ok = wait_thread(&ctl->full[value_stage], value_round & 1, waits);
                     if (ok && takes(bv)) {
                         const int slot = done & 1;
                         if (done == 0 && outputs_used++ > 0)   // the outputs before have been taken
-                            ok = wait_thread(&ctl->o_empty[tile], outputs_used & 1, abort_flag);
+                            ok = wait_thread(&ctl->o_empty[tile], outputs_used & 1, waits);
                         if (ok && ctl->special[info] != 0) {
-                            ok = wait_thread(&ctl->clean[value_stage], (clean_phase >> value_stage) & 1, abort_flag);
+                            ok = wait_thread(&ctl->clean[value_stage], (clean_phase >> value_stage) & 1, waits);
                             clean_phase ^= 1u << value_stage;
                         }
-                        ok = ok && wait_thread(&ctl->p_full[tile * 2 + slot], (p_phase >> slot) & 1, abort_flag);
+                        ok = ok && wait_thread(&ctl->p_full[tile * 2 + slot], (p_phase >> slot) & 1, waits);
                         if (!ok) break;
                         p_phase ^= 1u << slot;
                         prefill::tc_fence_after();
@@ -732,7 +738,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             for (int b = 0; ok && b < blocks; ++b) {
 #pragma unroll 1
                 for (int kind = 0; kind < 2; ++kind) {
-                    ok = ok && wait_warp(&ctl->full[stage], round & 1, abort_flag);
+                    // the one wait that is never suspended, so that a short limit means something: 2 % if all are like that
+                    ok = ok && __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[stage], round & 1) ||
+                                                           wait_on(&ctl->full[stage], round & 1, waits));
                     if (!ok) break;
                     const int special = kind == 1 ? ctl->special[info] : 0;
                     if (special != 0) {
@@ -810,7 +818,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             }
             for (int b = first_block; b < blocks; b += alone ? 2 : 1, ++step) {
                 const int slot = tile * 2 + (step & 1);
-                ok = ok && wait_warp(&ctl->s_full[slot], (phase >> slot) & 1, abort_flag);
+                ok = ok && wait_warp(&ctl->s_full[slot], (phase >> slot) & 1, waits);
                 if (!ok) break;
                 phase ^= 1u << slot;
                 prefill::tc_fence_after();
@@ -850,7 +858,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     m = grown;
                     l *= factor;
                     // the product before is in the outputs; the one before that is, since these scores are there
-                    ok = wait_warp(&ctl->pv_done[slot ^ 1], ((phase >> (slot ^ 1)) & 1) ^ 1, abort_flag);
+                    ok = wait_warp(&ctl->pv_done[slot ^ 1], ((phase >> (slot ^ 1)) & 1) ^ 1, waits);
                     if (!ok) break;
                     prefill::tc_fence_after();
 #pragma unroll 1
@@ -865,7 +873,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     tmem_wait_store();
                 }
                 if (step < turns) {
-                    ok = wait_warp(&ctl->turn[tile][warp & 3], turn & 1, abort_flag);
+                    ok = wait_warp(&ctl->turn[tile][warp & 3], turn & 1, waits);
                     if (!ok) break;
                     ++turn;
                 }
@@ -903,14 +911,14 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
             const bool any = first_block < blocks;
             if (any) {
                 const int slot = tile * 2 + ((step - 1) & 1);
-                ok = ok && wait_warp(&ctl->pv_done[slot], ((phase >> slot) & 1) ^ 1, abort_flag);
+                ok = ok && wait_warp(&ctl->pv_done[slot], ((phase >> slot) & 1) ^ 1, waits);
                 prefill::tc_fence_after();
             }
             float keep = 1.f, other = 0.f;   // factors of these outputs and of the other half's
             bool other_any = false;
             if (alone) {
                 if (tile == 1) {
-                    if (halves > 0) ok = ok && wait_warp(&ctl->half_taken, (halves - 1) & 1, abort_flag);
+                    if (halves > 0) ok = ok && wait_warp(&ctl->half_taken, (halves - 1) & 1, waits);
                     ++halves;
                     ctl->half[r][0] = m;
                     ctl->half[r][1] = l;
@@ -920,7 +928,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     release_work();
                     continue;
                 }
-                ok = ok && wait_warp(&ctl->half_ready, halves & 1, abort_flag);
+                ok = ok && wait_warp(&ctl->half_ready, halves & 1, waits);
                 ++halves;
                 prefill::tc_fence_after();
                 other_any = end - begin > 1;
@@ -1029,12 +1037,12 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         }
     }
     if (!ok && lane == 0) {
-        *abort_flag = 1;
+        waits->abort_flag = 1;
         if (p.a.status != nullptr) *p.a.status = MB_ST_PIPE_TIMEOUT;
     }
     prefill::tc_fence_before();
     __syncthreads();
-    if (*abort_flag != 0) {   // copies and products that are under way end before the memory goes
+    if (waits->abort_flag != 0) {   // copies and products that are under way end before the memory goes
         const unsigned long long start = global_timer_ns();
         while (global_timer_ns() - start < 200000ull) __nanosleep(1000);
         __syncthreads();

@@ -174,7 +174,7 @@ class PagedAttentionArgs(ctypes.Structure):
     _fields_ = [(name, ctypes.c_int32) for name in
                 ("element", "tokens", "requests", "heads", "kv_heads", "head_dim", "width", "pages",
                  "page_size", "zero_rest")] + [
-        ("scale", ctypes.c_float), ("reserved", ctypes.c_int32)] + [
+        ("scale", ctypes.c_float), ("wait_limit_ns", ctypes.c_int32)] + [
         (name, ctypes.c_int64) for name in
         ("query_token", "query_head", "key_token", "key_head", "value_token", "value_head",
          "kpool_page", "kpool_token", "kpool_head", "vpool_page", "vpool_token", "vpool_head")] + [

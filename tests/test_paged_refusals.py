@@ -1,9 +1,12 @@
 """Arguments that the paged operators refuse, without a device."""
 
+import ctypes
+
 import pytest
 import torch
 
-from megabake_b200 import PagedState, paged_append, paged_kv_attention, paged_prefill_attention, paged_reserve
+from megabake_b200 import paged_reserve
+from megabake_b200 import runtime as rt
 from megabake_b200.diagnostics import CompilerError
 
 INT32 = torch.int32
@@ -28,3 +31,10 @@ def test_reserve_takes_one_number_a_request(requests, name):
         _refused(f"{name} must be",
                  lambda: paged_reserve(**{**tensors, name: tensors[name][:, None]}, page_size=16, max_tokens=2))
     _refused("CUDA", lambda: paged_reserve(**tensors, page_size=16, max_tokens=2))
+
+
+@pytest.mark.parametrize("entry", ["mb_paged_attention", "mb_paged_prefill"])
+def test_a_limit_below_zero_is_refused(entry):
+    args = rt.PagedAttentionArgs(0, 4, 4, 4, 2, 64, 8, 32, 16, 0, 0.125, -1, 256, 64, 0, 0, 0, 0, 2048, 128, 64,
+                                 2048, 128, 64, 4096, 0, 0, *[4096 * (i + 1) for i in range(6)], 0, 0)
+    assert getattr(rt.load_library(), entry)(ctypes.byref(args), None) == 1   # MB_ERR_INVALID
