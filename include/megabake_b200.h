@@ -466,7 +466,7 @@ enum mb_element { MB_BF16 = 0, MB_FP16 = 1 };
  * last: -1, 0, -1.  granted[r]: tokens granted, or dropped (negative).                            */
 typedef struct mb_paged_reserve_args {
     int32_t requests;         /* rows, at most 2048                                       */
-    int32_t width;            /* pages per row of the table; width * page_size <= 2^30    */
+    int32_t width;            /* pages per row of the table; width * page_size <= 2^30, requests * width < 2^31 */
     int32_t pages;            /* of the pool: entries of free_pages                       */
     int32_t page_size;
     int32_t max_tokens;       /* entries of slots, positions and rows: 0 .. 2^30          */

@@ -356,7 +356,8 @@ int mb_paged_reserve(const mb_paged_reserve_args* a, void* stream) {
         (a->slots | a->positions | a->rows) % 16)
         return MB_ERR_INVALID;
     if (a->requests > kMaxRows || a->max_tokens > kMaxTokens || !page_size_covered(a->page_size) ||
-        static_cast<int64_t>(a->width) * a->page_size > kMaxTokens)
+        static_cast<int64_t>(a->width) * a->page_size > kMaxTokens ||
+        static_cast<int64_t>(a->requests) * a->width > INT32_MAX)   // pages of all rows, whatever the lengths say
         return MB_ERR_UNSUPPORTED;
     ReserveArgs p;
     p.requests = a->requests;

@@ -242,9 +242,10 @@ def _reserve_fields(counts, lengths, block_table, free_pages, free_count, page_s
         _whole(name, tensor, torch.int32, shape, device)
     if device.type != "cuda" or not 1 <= requests <= _MAX_REQUESTS or width < 1 or not _page_size_covered(page_size) or \
             max_tokens < 0 or max_tokens > _MAX_TOKENS or width * page_size > _MAX_TOKENS or \
-            not 1 <= free_pages.numel() <= _MAX_COUNT:
+            requests * width > _MAX_COUNT or not 1 <= free_pages.numel() <= _MAX_COUNT:
         fail("input-binding", f"paged_reserve needs 1..{_MAX_REQUESTS} requests on a CUDA device, pages of 8 to 1024 tokens "
-                              "(a power of two), rows of at most 2**30 tokens and max_tokens up to that, got "
+                              "(a power of two), rows of at most 2**30 tokens, max_tokens up to that and fewer than 2**31 "
+                              "entries of the table, got "
                               f"{tuple(block_table.shape)} pages of {page_size} on {device}, max_tokens {max_tokens}")
     args = rt.PagedReserveArgs(requests, width, free_pages.numel(), page_size, max_tokens)
     return bytes(args)[:rt.PagedReserveArgs.counts.offset], _native_device(device)

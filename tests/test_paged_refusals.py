@@ -38,3 +38,10 @@ def test_a_limit_below_zero_is_refused(entry):
     args = rt.PagedAttentionArgs(0, 4, 4, 4, 2, 64, 8, 32, 16, 0, 0.125, -1, 256, 64, 0, 0, 0, 0, 2048, 128, 64,
                                  2048, 128, 64, 4096, 0, 0, *[4096 * (i + 1) for i in range(6)], 0, 0)
     assert getattr(rt.load_library(), entry)(ctypes.byref(args), None) == 1   # MB_ERR_INVALID
+
+
+@pytest.mark.parametrize("requests,width", [(2048, 1 << 20), (2048, (1 << 27) - 1), (17, 1 << 27)])
+def test_reserve_takes_tables_whose_entries_an_int_counts(requests, width):
+    """Pages of all rows together are counted in 32 bits."""
+    args = rt.PagedReserveArgs(requests, width, 32, 8, 64, 0, *[4096 * (i + 1) for i in range(10)])
+    assert rt.load_library().mb_paged_reserve(ctypes.byref(args), None) == 3   # MB_ERR_UNSUPPORTED
