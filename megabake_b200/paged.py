@@ -150,11 +150,12 @@ def _whole(name: str, tensor: torch.Tensor, dtype: torch.dtype, shape: tuple, de
 
 
 def _rows(name: str, tensor: torch.Tensor, shape: tuple, like: torch.Tensor) -> tuple:
-    """Strides of ``[..., head_dim]`` values that are read 16 bytes at a time."""
+    """Strides of ``[..., head_dim]`` values that are read 16 bytes at a time; that of a single place, which is never gone
+    along, as if the next one followed at once."""
     if tensor.dtype != like.dtype or tensor.device != like.device or tensor.shape != shape:
         fail("input-binding", f"{name} must be {like.dtype} {tuple(shape)} on {like.device}, got {tensor.dtype} "
                               f"{tuple(tensor.shape)} on {tensor.device}")
-    strides = tensor.stride()
+    strides = tuple(shape[-1] if places == 1 else stride for places, stride in zip(shape, tensor.stride()))
     if strides[-1] != 1 or any(stride % 8 for stride in strides[:-1]):
         _misaligned(name)
     return strides[:-1]

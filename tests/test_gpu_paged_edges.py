@@ -67,3 +67,29 @@ def test_prompt_bits_do_not_depend_on_rows_of_no_query(heads, dtype):
         assert torch.equal(result[:39], results[0][:39])
     for result in results[2::2]:
         assert torch.equal(result, results[0])
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_strides_of_single_places_mean_nothing(dim):
+    """One token of one request with one key head, on one page: strides of these dimensions are any numbers."""
+    g = torch.Generator(device="cuda").manual_seed(dim)
+
+    def odd(x, strides):
+        flat = torch.empty(x.numel() + 64, dtype=x.dtype, device="cuda")
+        return flat.as_strided(x.shape, strides).copy_(x)
+
+    query, key, value = (_normal((1, n, dim), g, BF16) for n in (3, 1, 1))
+    pools = [_normal((1, 16, 1, dim), g, BF16) for _ in range(2)]
+    table, lengths, offsets, slots = _int32([[0]]), _int32([9]), _int32([0, 1]), torch.tensor([8], device="cuda")
+    results = []
+    for again in (False, True):
+        p = [x.clone() for x in pools]
+        q, k, v = query, key, value
+        if again:
+            p = [odd(x, (3, dim, 7, 1)) for x in p]
+            q, k, v = odd(q, (3 * dim + 1, dim, 1)), odd(k, (5, 2 * dim + 3, 1)), odd(v, (1, 1, 1))
+        out = paged_kv_attention(q, k, v, *p, table, lengths)
+        paged_append(v, k, *p, slots)
+        results.append([out, paged_prefill_attention(q, *p, table, lengths, offsets), *p])
+    for one, other in zip(*results):
+        assert torch.equal(one, other)

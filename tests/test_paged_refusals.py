@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from megabake_b200 import paged_reserve
+from megabake_b200 import paged_append, paged_reserve
 from megabake_b200 import runtime as rt
 from megabake_b200.diagnostics import CompilerError
 
@@ -45,3 +45,15 @@ def test_reserve_takes_tables_whose_entries_an_int_counts(requests, width):
     """Pages of all rows together are counted in 32 bits."""
     args = rt.PagedReserveArgs(requests, width, 32, 8, 64, 0, *[4096 * (i + 1) for i in range(10)])
     assert rt.load_library().mb_paged_reserve(ctypes.byref(args), None) == 3   # MB_ERR_UNSUPPORTED
+
+
+def test_strides_of_single_places_mean_nothing():
+    """One token, one head or one page: what lies between it and the next is never looked at."""
+    def one(shape, strides):
+        return torch.zeros(4096, dtype=torch.bfloat16).as_strided(shape, strides)
+
+    slots = torch.zeros(1, dtype=torch.int64)
+    pool = one((1, 16, 1, 64), (3, 64, 5, 1))
+    _refused("CUDA", lambda: paged_append(one((1, 1, 64), (195, 67, 1)), one((1, 1, 64), (1, 0, 1)), pool, pool, slots))
+    _refused("16-byte", lambda: paged_append(one((1, 1, 64), (195, 67, 1)), one((1, 1, 64), (1, 0, 1)), pool,
+                                             one((1, 16, 1, 64), (64, 68, 64, 1)), slots))
