@@ -144,12 +144,14 @@ class PagedGenerator:
 
     ``requests`` rows run at once; ``pages`` pages of ``page_size`` tokens are shared by them (default: enough for all
     of them to grow to ``capacity``).  A prompt is admitted when its row and the pages for all of its tokens are there, so
-    no request is refused later.  Decode steps are one CUDA graph: pages, attention, projections and the greedy
+    no request is refused later.  Prompts admitted together go through the model in one pass, of ``prompt_tokens`` tokens at
+    most where there are several: its activations do not grow with how many prompts wait.  Decode steps are one CUDA graph: pages, attention, projections and the greedy
     pick, without the host; at the end it is checked once that no wait inside a kernel ran out (``CompilerError``)."""
 
     def __init__(self, model: torch.nn.Module, requests: int, capacity: int, *, page_size: int = 64,
-                 pages: int | None = None):
+                 pages: int | None = None, prompt_tokens: int = 8192):
         self.decoder = PagedDecoder(model).eval()
+        self.prompt_tokens = prompt_tokens
         self.state = self.decoder.make_paged_state(requests, capacity, page_size=page_size, pages=pages)
         self.requests, self.pages = requests, self.state.free_pages.numel()
         self.device = self.state.lengths.device
@@ -224,14 +226,16 @@ class PagedGenerator:
         waiting, running, done = list(range(len(prompts))), {}, {}   # running: row -> [prompt, ids produced]
         free_pages, active = self.pages, None
         while waiting or running:
-            admitted = {}
+            admitted, tokens = {}, 0
             for row in range(self.requests):
                 if not waiting or row in running:
                     continue
-                need = self._pages_of(prompts[waiting[0]].numel() + wanted[waiting[0]] - 1)
-                if need > free_pages:
+                length = prompts[waiting[0]].numel()
+                need = self._pages_of(length + wanted[waiting[0]] - 1)
+                if need > free_pages or (admitted and tokens + length > self.prompt_tokens):
                     break
                 free_pages -= need
+                tokens += length
                 index = waiting.pop(0)
                 running[row] = [index, 1]
                 admitted[row] = prompts[index]
