@@ -494,12 +494,12 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
                                 }
                             }
                         }
-                        const float base0 = finite_base(m[c][0]) - kWeightShift<T>;
-                        const float base1 = finite_base(m[c][1]) - kWeightShift<T>;
-                        s[c][0] = prefill::exp2_approx(s[c][0] - base0);
-                        s[c][1] = prefill::exp2_approx(s[c][1] - base1);
-                        s[c][2] = prefill::exp2_approx(s[c][2] - base0);
-                        s[c][3] = prefill::exp2_approx(s[c][3] - base1);
+                        // the maximum first: a large one would swallow the shift
+                        const float base0 = finite_base(m[c][0]), base1 = finite_base(m[c][1]);
+                        s[c][0] = prefill::exp2_approx(s[c][0] - base0 + kWeightShift<T>);
+                        s[c][1] = prefill::exp2_approx(s[c][1] - base1 + kWeightShift<T>);
+                        s[c][2] = prefill::exp2_approx(s[c][2] - base0 + kWeightShift<T>);
+                        s[c][3] = prefill::exp2_approx(s[c][3] - base1 + kWeightShift<T>);
                         l[c][0] += s[c][0] + s[c][2];
                         l[c][1] += s[c][1] + s[c][3];
 #pragma unroll

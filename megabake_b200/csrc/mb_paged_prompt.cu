@@ -792,8 +792,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         unsigned int halves = 0;                        // lone tiles so far
         unsigned int turn = 0;                          // turns taken so far
         Split split = {0, 0, 0, 0};
-        const bool premultiply = p.scale_log2 <= 0.f;   // the largest score is not that of the largest product
-        const float multiplier = premultiply ? 1.f : p.scale_log2;
+        // The largest score is not that of the largest product.  Otherwise maxima are of products, without the scale.
+        const bool premultiply = p.scale_log2 <= 0.f;
+        const float multiplier = premultiply ? 1.f : p.scale_log2, lag = kLag / multiplier;
         while (const Work* u = next_work()) {
             const int begin = u->begin, end = u->end;
             if (begin >= end) {
@@ -848,13 +849,13 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                 for (int c = 0; c < kBlock; c += 8)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) highest[i] = fmaxf(fmaxf(highest[i], s[c + i]), s[c + 4 + i]);
-                const float now = fmaxf(fmaxf(highest[0], highest[1]), fmaxf(highest[2], highest[3])) * multiplier;
+                const float now = fmaxf(fmaxf(highest[0], highest[1]), fmaxf(highest[2], highest[3]));
                 if (b == first_block) {
                     m = now;
-                } else if (__any_sync(0xffffffffu, counts && (now > m + kLag || (m == -INFINITY && now > m)))) {
+                } else if (__any_sync(0xffffffffu, counts && (now > m + lag || (m == -INFINITY && now > m)))) {
                     const float grown = fmaxf(m, now);
                     const float base = grown == -INFINITY ? 0.f : grown;
-                    const float factor = prefill::exp2_approx(m - base);
+                    const float factor = prefill::exp2_approx((m - base) * multiplier);
                     m = grown;
                     l *= factor;
                     // the product before is in the outputs; the one before that is, since these scores are there
@@ -877,8 +878,10 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     if (!ok) break;
                     ++turn;
                 }
-                const float base = (m == -INFINITY ? 0.f : m) - kPromptShift<T>;
+                // the maximum first, unscaled: what is left is small where a weight is not, whatever the maximum is
+                const float base = m == -INFINITY ? 0.f : m;
                 const unsigned long long multiplier2 = pair_of(multiplier, multiplier), base2 = pair_of(-base, -base);
+                const unsigned long long shift2 = pair_of(kPromptShift<T>, kPromptShift<T>);
                 unsigned long long sum0 = pair_of(0.f, 0.f), sum1 = sum0;
 #pragma unroll
                 for (int c = 0; c < kBlock; c += 32) {
@@ -887,8 +890,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                     for (int i = 0; i < 32; i += 4) {
                         // the other tile's begin while the last of these are under way
                         if (c + i == kPassAt && step + tile < turns && lane == 0) mbar_arrive(&ctl->turn[tile ^ 1][warp & 3]);
-                        const unsigned long long e0 = fma_pair(pair_of(s[c + i], s[c + i + 1]), multiplier2, base2);
-                        const unsigned long long e1 = fma_pair(pair_of(s[c + i + 2], s[c + i + 3]), multiplier2, base2);
+                        const unsigned long long d0 = add_pair(pair_of(s[c + i], s[c + i + 1]), base2);
+                        const unsigned long long d1 = add_pair(pair_of(s[c + i + 2], s[c + i + 3]), base2);
+                        const unsigned long long e0 = fma_pair(d0, multiplier2, shift2), e1 = fma_pair(d1, multiplier2, shift2);
                         const float x0 = prefill::exp2_approx(pair_low(e0)), y0 = prefill::exp2_approx(pair_high(e0));
                         const float x1 = prefill::exp2_approx(pair_low(e1)), y1 = prefill::exp2_approx(pair_high(e1));
                         sum0 = add_pair(sum0, pair_of(x0, y0));
@@ -933,8 +937,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                 prefill::tc_fence_after();
                 other_any = end - begin > 1;
                 const float m1 = ctl->half[r][0], grown = fmaxf(m, m1), base = grown == -INFINITY ? 0.f : grown;
-                keep = prefill::exp2_approx(m - base);
-                other = prefill::exp2_approx(m1 - base);
+                keep = prefill::exp2_approx((m - base) * multiplier);
+                other = prefill::exp2_approx((m1 - base) * multiplier);
                 l = l * keep + ctl->half[r][1] * other;
                 m = grown;
             }
@@ -1012,7 +1016,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                 // it is minus infinity too, and the sum says so.
                 *reinterpret_cast<float2*>(
                     p.stats + (static_cast<size_t>(blockIdx.x * 2 + (begin == 0 ? 1 : 0)) * kTiles * kRows + tile * kRows + r) * 2) =
-                    make_float2(any ? fmaxf(m, -FLT_MAX) : -INFINITY, l);
+                    make_float2(any ? fmaxf(m * multiplier, -FLT_MAX) : -INFINITY, l);
                 if (begin == 0) split = {u->first, u->head, u->tokens, u->pieces};
             }
             prefill::tc_fence_before();

@@ -93,3 +93,14 @@ def test_strides_of_single_places_mean_nothing(dim):
         results.append([out, paged_prefill_attention(q, *p, table, lengths, offsets), *p])
     for one, other in zip(*results):
         assert torch.equal(one, other)
+
+
+def test_queries_that_are_broadcast():
+    """One query for all heads, or for all tokens: strides of zero."""
+    cache = Cache([200, 700], 2, 64, 16, BF16, 1)
+    offsets = _int32([0, 10, 30])
+    for shape in ((1, 4, 64), (30, 1, 64)):
+        query = _normal(shape, cache.g, BF16).expand(30, 4, 64)
+        for call in (lambda q: paged_prefill_attention(q, *cache.pools, cache.table, cache.lengths, offsets),
+                     lambda q: paged_kv_attention(q[:2], q[:2, :2], q[:2, 2:], *cache.clone(), cache.table, cache.lengths)):
+            assert torch.equal(call(query), call(query.contiguous()))
