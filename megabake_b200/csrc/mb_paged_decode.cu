@@ -71,7 +71,6 @@ struct Control4 {
 // ---------------------------------------------------------------------------------------
 struct Deal {
     const int* first_block;   // [tokens + 1] blocks (of one unit) before the token
-    const int *length, *row;  // [tokens]
     int tokens, units;        // units of a token
     long long total, per;
 };
@@ -272,8 +271,6 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __gri
     const int group = p.a.heads / p.a.kv_heads;
     Deal deal;
     deal.first_block = first_block;
-    deal.length = lengths;
-    deal.row = table_rows;
     deal.tokens = p.a.tokens;
     deal.units = p.a.kv_heads * p.subgroups;
     deal.total = static_cast<long long>(first_block[p.a.tokens]) * deal.units;

@@ -76,7 +76,7 @@ struct PromptArgs {
 
 // A piece of a unit, as the warp that copies tells the others.
 struct Work {
-    int request, head, tile;
+    int request, head;
     int begin, end, blocks;      // blocks of this piece, and of the unit; end < 0: nothing more
     int first, tokens;           // queries of the unit
     int position;                // of its first query
@@ -141,7 +141,7 @@ __device__ __forceinline__ long long request_length(const Request& q, int unit_t
 }
 
 struct Piece {
-    int request, head, tile;
+    int request, head;
     int begin, end, blocks;      // blocks of this piece, and of the unit
     int first, tokens;           // queries of the unit
     int position;                // of its first query
@@ -175,7 +175,7 @@ struct Piece {
             else
                 upper = middle;
         }
-        tile = lower;
+        const int tile = lower;
         const long long start = length_before(q, d.unit_tokens, d.cost, tile);
         const long long end_of = tile + 1 == units ? length : length_before(q, d.unit_tokens, d.cost, tile + 1);
         const long long unit_begin = at - (rest - start);
@@ -309,7 +309,7 @@ __device__ __forceinline__ unsigned int without_odd(unsigned int v) {
 }
 // The infinities and NaN that were taken out of blocks `from` .. `stop` - 1 of a unit, 32 columns of them from `column` on,
 // added to the outputs of a query at `position`.  `info` is that of block `end`.
-template <typename T, int kBlock>
+template <typename T>
 __device__ __noinline__ void give_back(float* o, const AttentionArgs& a, const PromptControl* ctl, const Work* u, int info,
                                        int from, int stop, int end, int column, int position) {
 #pragma unroll 1
@@ -484,7 +484,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         // ---- copies
         int stage = 0, info = 0;
         unsigned int round = 0, units = 0;
-        constexpr int kBlockShift = kBlock == 128 ? 7 : 6;
+        constexpr int kBlockShift = 6;
+        static_assert(1 << kBlockShift == kBlock);
         const int rows_shift = min(shift, kBlockShift), rows = 1 << rows_shift;
         const int per_shift = kBlockShift - rows_shift, per_block = 1 << per_shift;   // table entries of a block
         const int batch = 32 >> per_shift;                                            // blocks whose entries the lanes hold
@@ -503,7 +504,6 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                 at = u.next;
                 w.request = u.request;
                 w.head = u.head;
-                w.tile = u.tile;
                 w.begin = u.begin;
                 w.end = u.end;
                 w.blocks = u.blocks;
@@ -979,7 +979,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
                         float given[32];
 #pragma unroll
                         for (int i = 0; i < 32; ++i) given[i] = o[i];
-                        if (l != 0.f) give_back<T, kBlock>(given, p.a, ctl, u, info, diagonal, waited, end, c, position);
+                        if (l != 0.f) give_back<T>(given, p.a, ctl, u, info, diagonal, waited, end, c, position);
                         __syncwarp();   // lanes come back at different times, and what follows is for all of them
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] = given[i];
