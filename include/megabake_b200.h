@@ -486,7 +486,8 @@ typedef struct mb_paged_reserve_args {
 int mb_paged_reserve(const mb_paged_reserve_args* args, void* stream);
 
 /* Token t goes to page slots[t] / page_size, place slots[t] % page_size; slots outside
- * 0..pages * page_size - 1 are skipped.  Of two tokens with one slot either may end up there.   */
+ * 0..pages * page_size - 1 are skipped.  Slots of one call are distinct: where two tokens name one, its place holds
+ * parts of both.                                                                                  */
 typedef struct mb_paged_append_args {
     int32_t tokens, kv_heads, head_dim, pages, page_size, reserved;
     int64_t key_token, key_head, value_token, value_head;             /* strides          */
@@ -501,11 +502,16 @@ int mb_paged_append(const mb_paged_append_args* args, void* stream);
 /* Query t belongs to request rows[t] (t where rows is 0; a row outside 0..requests-1: none) and attends all of its
  * `lengths` keys that lie on pages of the pool; where there is none its output is zero.  With `key` and `value`
  * the last of them is the token's own and is written to its place in the pools first; rows then name a request
- * once.  Scores, softmax statistics and sums are fp32; outputs are rounded once.
+ * once.  A length outside 0..width * page_size counts as the nearer of the two.  Scores, softmax statistics and sums are
+ * fp32; a weight meets the values as the sum of two 16-bit numbers (16 bits of it for bf16, 22 for fp16); outputs are rounded
+ * once.  An infinity among the values is one in the outputs, if the key's weight is more than 2^-95 (bf16) or 2^-39 (fp16) of
+ * the largest, and NaN below that.
  *
  * mb_paged_prefill: request r has the queries offsets[r] .. offsets[r + 1] - 1, its last positions, already
  * appended: the one at position p attends the keys 0..p.  A query before position 0 has none.  Queries of
- * no request: zero where zero_rest is set, else left as they were.  offsets do not fall and lie in 0..tokens.
+ * no request: zero where zero_rest is set, else left as they were.  offsets do not fall and lie in 0..tokens.  A weight
+ * meets the values as one 16-bit number, rounded to half a step (in fp16, weights of 2^-21 of a query's largest and
+ * less to fewer digits, below 2^-32 to none).  Infinities among values as above, down to 2^-87 and 2^-32.
  *
  * At most 2048 requests and, for mb_paged_attention, 2048 tokens, whose rows of the table hold fewer than 2^37
  * positions together.  workspace: as many bytes as the _workspace call says (0: none), 256-byte aligned, not shared by calls that

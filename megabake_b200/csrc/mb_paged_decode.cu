@@ -38,8 +38,9 @@ constexpr int kSmemLimit = 227 * 1024;
 constexpr int kConsumerBarrier = 1;
 // Of a run, where units are cut (one of 2,048 keys, 9/3 heads of 64: 7.4 us; 1: 7.7, 4: 8.0).
 constexpr int kLeastBlocks = 2;
-// Rows of the table that hold no more are not cut: one launch and no scratch (33 keys: 6.7 -> 4.4 us on the
-// device), and a CTA has eight blocks within about the time that joining pieces takes.
+// Rows of the table that hold no more are not cut, whatever lengths are, which the host does not know: one launch and no
+// scratch (33 keys: 4.5 us on the device in a table of 4 pages of 64, 7.2 to 7.6 in one of 128), and a CTA has eight blocks
+// within about the time that joining pieces takes.
 constexpr int kWholeBlocks = 8;
 
 // What a CTA leaves behind about the unit that it began and others finish.
@@ -203,10 +204,11 @@ __device__ __forceinline__ float finite_base(float m) { return m == -INFINITY ? 
 // of 8 x 8 (movmatrix) makes them the second product's columns, and values are read transposed (ldmatrix.trans) as its
 // rows: o^T = v^T p^T, whose columns are queries again, so that rescaling is by the lane's own two queries.
 //
-// Measured (us; floor at the measured copy bandwidth): 64 requests of 8,192 keys, 32/8 heads of 128: 318 to 326 (328), 6.6
-// TB/s; one of 131,071: 89 to 91 (82); 37 ragged ones of up to 4,099, 14/2 heads of 64, pages of 16: 20 (6), of which about 9 stream
+// Measured (us; floor at the measured copy bandwidth): 64 requests of 8,192 keys, 32/8 heads of 128: 313 to 348, by run (328),
+// 6.2 to 6.9 TB/s, a few percent of it from L2 where passes follow one another; one of 131,071: 89 to 92 (82); 37 ragged ones
+// of up to 4,099, 14/2 heads of 64, pages of 16: 20 (6), of which about 9 stream
 // and the rest is latency: 4,400 cycles until the first keys are asked for and 1,700 until they are there, two merges of
-// 2,000, the joining launch; one of 33 keys: 4.4.  Boxes issued by one lane, with 64-bit division for their places, instead
+// 2,000, the joining launch; one of 33 keys: 4.5.  Boxes issued by one lane, with 64-bit division for their places, instead
 // of a box a lane and 32-bit: 24.0 us for the ragged ones, then 22.0.
 // ---------------------------------------------------------------------------------------
 template <typename T, int D, int N>   // N: 8-query columns of a unit

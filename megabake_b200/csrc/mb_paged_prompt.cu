@@ -34,8 +34,8 @@ __host__ __device__ constexpr int tile_cost(int head_dim) { return head_dim == 6
 // 24.2; 300 tokens after 2,000: 21.5, 20.5, 24.2; 64 after 3,000, 32/8 heads of 128: 29.5, 28.6, 30.0 (before the join
 // took less).
 constexpr int kLeastKeys = 256;
-// Rows of the table that hold no more are not cut: one launch and no scratch (19 tokens: 9.2 us, cut 15.6).  Rows of up to
-// 1,024 keys: 8 x 40 tokens after 700 uncut 27.9 us, cut 24.7; 4 x 600 36.2 and 34.0; one of 500 18.8 and 20.5.
+// Rows of the table that hold no more are not cut, whatever lengths are, which the host does not know: one launch and no
+// scratch (19 tokens: 9.2 us in a table of 4 pages of 64, 14.4 to 15.2 in one of 128).  Rows of up to 1,024 keys: 8 x 40 tokens after 700 uncut 27.9 us, cut 24.7; 4 x 600 36.2 and 34.0; one of 500 18.8 and 20.5.
 constexpr int kWholeKeys = 512;
 constexpr unsigned int kTmemColumns = 512;
 // A row's maximum may lag behind by this many powers of two before its sums are rescaled.
@@ -358,9 +358,14 @@ __device__ __forceinline__ bool wait_warp(unsigned long long* bar, unsigned int 
 // memory and are rescaled only when a row's maximum has grown by more than 2^8 since the last time.  256-wide
 // heads: one query tile.
 //
-// Measured (us; floor at the measured GEMM rate): 8,192 tokens, 32/8 heads of 128: 485 in a graph of few passes (332), 1.13
-// PFLOP/s; 509 tokens after 16,000, 8/1 heads of 256: 84 (41); seven prompts of up to 1,031, 32/8 heads of 64, pages of
-// 16: 59 (8).  What bounds it: a block of 64 keys takes 1,700 to 1,900 cycles, of which the exponentials of its two tiles,
+// A weight is one 16-bit number in the second product, off by up to half a step of its type, while the sum below it has 32 bits.
+// Errors against 64 bits (2-norm) are 0.0017 to 0.0023 for bf16, of which rounding the output is 0.0015 to 0.0017; a second
+// number, as decode has, would be half as many products again in the kernel that they bound.  fp16 weights are 2^7 to 2^15
+// at the maximum: one of 2^-21 of it and less has fewer digits, one below 2^-32 none.
+//
+// Measured (us; floor at the measured GEMM rate): 8,192 tokens, 32/8 heads of 128: 575 to 580 a pass among many (332), 0.95
+// PFLOP/s, at the power limit; 486 to 497 in a graph of few, 1.1 PFLOP/s; 509 tokens after 16,000, 8/1 heads of 256: 84 to 88
+// (41); seven prompts of up to 1,031, 32/8 heads of 64, pages of 16: 59 (8).  What bounds it: a block of 64 keys takes 1,700 to 1,900 cycles, of which the exponentials of its two tiles,
 // 8 cycles a warp and instruction, are 1,024, and the products 1,280 (64 keys a product of scores read the queries from shared
 // memory for 64 columns, at two thirds of the rate that 128 columns reach); between units there are the
 // outputs.  Blocks of 128 keys leave one slot a tile, and the chain scores -> weights -> outputs -> scores of a tile then

@@ -15,8 +15,9 @@ are the first ``free_count`` (int32 ``[1]``) entries of the stack ``free_pages``
 Each is one call into the native library on torch's current stream: nothing is synchronised, all of them can be
 captured in a CUDA graph, and a scratch buffer is the call's own.  bf16 and fp16; heads of 64, 128 or 256;
 any number of query heads per key head (128 for prompts); pages of 8 to 1,024 tokens (a power of two); pools and rows may have any
-strides that are multiples of 16 bytes.  Scores, softmax statistics and sums are fp32 and outputs are rounded
-once -- unlike ``kv_attention``, whose rounding points are the reference's eager ones.  Inference only.
+strides that are multiples of 16 bytes.  Scores, softmax statistics and sums are fp32, weights meet the values as two 16-bit
+numbers for single tokens (16 bits for bf16, 22 for fp16) and as one for prompts, and outputs are rounded once --
+unlike ``kv_attention``, whose rounding points are the reference's eager ones.  Inference only.
 
 The reference has one contiguous cache and one length per batch (``fx_handler/hf_attention.py:194-196``);
 per-request state is a step of its roadmap (``docs/roadmap.md:178``).
@@ -255,8 +256,8 @@ def _reserve_fields(counts, lengths, block_table, free_pages, free_count, page_s
 def paged_append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
                  slots: torch.Tensor) -> None:
     """Write ``key`` and ``value`` (``[tokens, kv_heads, head_dim]``) into the slots (int64 ``[tokens]``) of the pools.
-    A slot outside the pool, as -1 behind the last token, is skipped; slots of one call are distinct (of two tokens
-    with one slot either may be the one that stays)."""
+    A slot outside the pool, as -1 behind the last token, is skipped; slots of one call are distinct (where two tokens
+    name one slot, its place holds parts of both)."""
     if torch.is_grad_enabled():
         _inference_only(key, value, key_pages, value_pages)
     signature = (key.dtype, key.get_device(), key.shape, key.stride(), value.dtype, value.get_device(), value.shape,
@@ -385,7 +386,7 @@ def paged_kv_attention(query: torch.Tensor, key: torch.Tensor | None, value: tor
     ``[tokens, heads, head_dim]``.
 
     Query ``t`` belongs to request ``rows[t]`` (int32 ``[tokens]``; ``t`` itself without ``rows``) and attends all
-    ``lengths`` keys of that request; positions on pages outside the pool do not count.  Where nothing is left (an idle
+    ``lengths`` keys of that request (a row of the table at most); positions on pages outside the pool do not count.  Where nothing is left (an idle
     place with row -1, length 0) its output is zero.  With ``key`` and ``value`` (``[tokens, kv_heads, head_dim]``) the
     last position of the request is the token's own, appended first in the same call: ``lengths`` counts it already
     (``paged_reserve`` does), and ``rows`` names no request twice.  Without them several queries may read one
