@@ -415,12 +415,14 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap query_map, const __g
         ctl->waits.limit_ns = p.a.wait_limit_ns;
         mbar_init_fence();
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // Not before the wait: the kernel that it is for may be anybody's, and one that let this launch begin before it allocated
+    // would wait for these columns.  For the same reason the next launch may begin only when they are taken.
     if (warp == 11) prefill::tmem_alloc(&ctl->tmem, kTmemColumns);
     prefill::tc_fence_before();
     __syncthreads();
     prefill::tc_fence_after();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     const unsigned int tmem = ctl->tmem;
 
     Deal deal;
