@@ -97,6 +97,8 @@ class PagedState:
     def check(self) -> None:
         """Synchronise the device and raise ``CompilerError`` if a kernel that was given ``status`` recorded a fault (a wait
         that ran out): outputs since the last check are not valid, nor is what was appended of them."""
+        if self.status.is_cuda:
+            torch.cuda.synchronize(self.status.device)   # steps may run on any stream
         code = int(self.status)
         if code:
             self.status.zero_()

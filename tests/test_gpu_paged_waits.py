@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import megabake_b200.hf as hf
-from megabake_b200 import PagedGenerator, models, paged_kv_attention, paged_prefill_attention
+from megabake_b200 import PagedGenerator, PagedState, models, paged_kv_attention, paged_prefill_attention
 from megabake_b200 import runtime as rt
 from megabake_b200.diagnostics import CompilerError
 from tests.test_gpu_paged import BF16, FP16, Cache, _int32, _normal
@@ -76,3 +76,15 @@ def test_generation_tells_when_a_kernel_recorded_a_fault(monkeypatch, operator):
     monkeypatch.undo()
     generator._graph = None        # the step that was captured with the other function
     assert [ids.numel() for ids in generator(prompts, 5)] == [5, 5]
+
+
+def test_a_fault_of_another_stream_is_seen():
+    state = PagedState(1, 1, 16, 1, 64, device="cuda")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(20_000_000)      # cycles: about ten milliseconds of a step
+        state.status.fill_(2)
+    with pytest.raises(CompilerError, match="pipeline-timeout"):
+        state.check()
+    state.check()
