@@ -35,7 +35,8 @@ __host__ __device__ constexpr int tile_cost(int head_dim) { return head_dim == 6
 // took less).
 constexpr int kLeastKeys = 256;
 // Rows of the table that hold no more are not cut, whatever lengths are, which the host does not know: one launch and no
-// scratch (19 tokens: 9.2 to 9.7 us in a table of 4 pages of 64, 14.4 to 15.2 in one of 128).  Rows of up to 1,024 keys: 8 x 40 tokens after 700 uncut 27.9 us, cut 24.7; 4 x 600 36.2 and 34.0; one of 500 18.8 and 20.5.
+// scratch (19 tokens: 9.2 to 9.7 us in a table of 4 pages of 64, 14.4 to 15.2 in one of 128).  Rows of up to 1,024 keys:
+// 8 x 40 tokens after 700 uncut 27.9 us, cut 24.7; 4 x 600 36.2 and 34.0; one of 500 18.8 and 20.5.
 constexpr int kWholeKeys = 512;
 constexpr unsigned int kTmemColumns = 512;
 // A row's maximum may lag behind by this many powers of two before its sums are rescaled.
@@ -365,8 +366,9 @@ __device__ __forceinline__ bool wait_warp(unsigned long long* bar, unsigned int 
 //
 // Measured (us; floor at the measured GEMM rate): 8,192 tokens, 32/8 heads of 128: 570 to 581 a pass among many (332), 0.95
 // PFLOP/s, at the power limit; 497 to 521 in a graph of few, 1.08 PFLOP/s; 509 tokens after 16,000, 8/1 heads of 256: 84 to 88
-// (41); seven prompts of up to 1,031, 32/8 heads of 64, pages of 16: 59 (8).  What bounds it: a block of 64 keys takes 1,700 to 1,900 cycles, of which the exponentials of its two tiles,
-// 8 cycles a warp and instruction, are 1,024, and the products 1,280 (64 keys a product of scores read the queries from shared
+// (41); seven prompts of up to 1,031, 32/8 heads of 64, pages of 16: 59 (8).
+//
+// What bounds it: a block of 64 keys takes 1,700 to 1,900 cycles, of which the exponentials of its two tiles, 8 cycles a warp and instruction, are 1,024, and the products 1,280 (64 keys a product of scores read the queries from shared
 // memory for 64 columns, at two thirds of the rate that 128 columns reach); between units there are the
 // outputs.  Blocks of 128 keys leave one slot a tile, and the chain scores -> weights -> outputs -> scores of a tile then
 // takes 3,300 cycles (558 us).  A quarter to five eighths of the exponentials by a polynomial on the multipliers took 562

@@ -145,8 +145,9 @@ class PagedGenerator:
     ``requests`` rows run at once; ``pages`` pages of ``page_size`` tokens are shared by them (default: enough for all
     of them to grow to ``capacity``).  A prompt is admitted when its row and the pages for all of its tokens are there, so
     no request is refused later.  Prompts admitted together go through the model in one pass, of ``prompt_tokens`` tokens at
-    most where there are several: its activations do not grow with how many prompts wait.  Decode steps are one CUDA graph: pages, attention, projections and the greedy
-    pick, without the host; at the end it is checked once that no wait inside a kernel ran out (``CompilerError``)."""
+    most where there are several: its activations do not grow with how many prompts wait.  Decode steps are one CUDA graph:
+    pages, attention, projections and the greedy pick, without the host; at the end it is checked once that no wait inside
+    a kernel ran out (``CompilerError``)."""
 
     def __init__(self, model: torch.nn.Module, requests: int, capacity: int, *, page_size: int = 64,
                  pages: int | None = None, prompt_tokens: int = 8192):

@@ -382,11 +382,12 @@ def _refuse_what_is_not_computed(model: torch.nn.Module, config) -> None:
         if value is not None and value != neutral:
             raise NotImplementedError(f"a paged decoder does not compute {name} = {value}")
     rope = getattr(config, "rope_parameters", None) or {}
-    if rope.get("llama_4_scaling_beta") is not None:
-        raise NotImplementedError("a paged decoder does not compute scores that are scaled by position")
-    # their frequencies follow the furthest position of a call, which may be another request's
-    if rope.get("rope_type") in ("dynamic", "longrope"):
-        raise NotImplementedError(f"a paged decoder does not compute {rope['rope_type']} rotary positions")
+    for kind in (rope, *(value for value in rope.values() if isinstance(value, dict))):   # of all layers, or by their kind
+        if kind.get("llama_4_scaling_beta") is not None:
+            raise NotImplementedError("a paged decoder does not compute scores that are scaled by position")
+        # their frequencies follow the furthest position of a call, which may be another request's
+        if kind.get("rope_type") in ("dynamic", "longrope"):
+            raise NotImplementedError(f"a paged decoder does not compute {kind['rope_type']} rotary positions")
 
 
 class PagedDecoder(StatefulDecoder):

@@ -89,6 +89,14 @@ def test_soft_caps_are_refused():
     PagedDecoder(model)
 
 
+def test_rotary_positions_are_looked_at_in_every_kind_of_layer():
+    model = _model("llama")
+    for rope, match in (({"rope_type": "longrope"}, "longrope"), ({"llama_4_scaling_beta": 0.1}, "scaled by position")):
+        model.config.rope_parameters = {"full_attention": {"rope_type": "default", **rope}}
+        with pytest.raises(NotImplementedError, match=match):
+            PagedDecoder(model)
+
+
 @pytest.mark.parametrize("kind", ["mistral", "starcoder2", "mixtral"])
 def test_a_window_shorter_than_the_capacity_is_refused(plain_operators, kind):
     """Rows hold whole pages, and requests may grow to all of them."""
