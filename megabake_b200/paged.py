@@ -392,8 +392,8 @@ def paged_kv_attention(query: torch.Tensor, key: torch.Tensor | None, value: tor
     Where nothing is left (an idle place with row -1, length 0) its output is zero.  With ``key`` and ``value``
     (``[tokens, kv_heads, head_dim]``) the last position of the request is the token's own, appended first in the same
     call: ``lengths`` counts it already (``paged_reserve`` does), and ``rows`` names no request twice.  Without them several
-    queries may read one request.  ``scale`` defaults to ``head_dim ** -0.5``.  ``status`` (int32 ``[1]``) receives a status code if a wait
-    inside the kernel ran out."""
+    queries may read one request.  ``scale`` defaults to ``head_dim ** -0.5``.  ``status`` (int32 ``[1]``) receives a status
+    code if a wait inside the kernel ran out."""
     return _attention("mb_paged_attention", query, key, value, key_pages, value_pages, block_table, lengths, rows, scale,
                       out, status)
 
